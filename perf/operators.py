@@ -304,9 +304,9 @@ def _plain_append(s):
 
 
 def _plain_sample(s):
-    """Weights 2^32 exp(x - max x) as whole numbers, so that every sum is the same in any order; the filters each keep
-    a first part of the tokens in order (larger x first, lower index first); the token is drawn over the kept ones in
-    the order of their indexes."""
+    """Weights 2^32 exp(-(max x - x)) as whole numbers, so that every sum is the same in any order; the filters each keep
+    a first part of the tokens in order (smaller max x - x first, then lower index); the token is drawn over the kept
+    ones in the order of their indexes."""
     logits, temperature = s["logits"].float(), s["temperature"]
     b, v = logits.shape
     inv = 1.0 / temperature
@@ -314,10 +314,10 @@ def _plain_sample(s):
     x = logits * torch.where(greedy, 1.0, inv)[:, None]
     x = torch.where(torch.isnan(x), -math.inf, x)
     top = x.amax(1, keepdim=True)
-    e = torch.where(x == top, 1.0, torch.exp(x - top))
-    e = torch.where(x == -math.inf, 0.0, e)
+    below = torch.where(x == top, 0.0, top - x)
+    e = torch.where(x == -math.inf, 0.0, torch.exp(-below))
     w = (e * 2.0 ** 32).long()
-    order = torch.sort(x, dim=1, descending=True, stable=True).indices
+    order = torch.sort(below, dim=1, stable=True).indices
     sorted_w, sorted_e = w.gather(1, order), e.gather(1, order)
     before = sorted_w.cumsum(1) - sorted_w
     rank = torch.arange(v, device=x.device)
@@ -405,8 +405,9 @@ def _exact_sample(s, c):
             tokens.append(int(torch.nonzero(x == x.max())[0, 0]))
             probs.append(1.0)
             continue
-        e = torch.where(x == x.max(), 0.0, x - x.max()).double().exp()
-        value, at = torch.sort(x, descending=True, stable=True)
+        below = torch.where(x == x.max(), 0.0, x.max() - x)
+        e = (-below.double()).exp()
+        at = torch.sort(below, stable=True).indices
         w = torch.floor(e[at] * 2.0 ** 32)
         n = c["vocab"]
         k = int(s["top_k"][b]) if s["top_k"] is not None else 0
