@@ -476,6 +476,114 @@ int tmac_model_prefill(tmac_model_t m, const int* tokens, int n_seq, int len, in
                        void* stream);
 int tmac_model_free(tmac_model_t m);
 
+/* ------------------------------------------------------------------------ */
+/* The batched decode step: several sequences at once over a paged cache (the
+ * reference decodes one sequence over one private cache,
+ * forward_layer_with_cache, sim/tmac_gguf.cpp:1559-1711).  Elements are F32, F16
+ * or BF16; arithmetic, softmax and sums are 32-bit, rounded once to the type.
+ * All pointers are device pointers on the cache's device; every call is
+ * asynchronous on `stream` and keeps no state between calls, so calls on
+ * several streams need no order among themselves unless they share buffers.
+ * Indexes that a kernel reads from the device and finds out of range (a
+ * position, a page, a length) touch no memory: TMAC_ERR_BOUNDS is recorded
+ * (tmac_device_error) and the place counts as given below. */
+#define TMAC_TYPE_BF16 30
+
+/* k and v: [n_pages][kv_heads][page_size][head_dim], contiguous, 16-byte
+ * aligned.  page_size: a power of two up to 256. */
+typedef struct tmac_paged_cache {
+    void* k;
+    void* v;
+    int64_t n_pages;
+    int type; /* TMAC_TYPE_F32, _F16 or _BF16 */
+    int kv_heads;
+    int page_size;
+    int head_dim;
+    int device;
+} tmac_paged_cache;
+
+/*
+ * Bias, position rotation, and k and v appended to the cache, in one launch
+ * (bias + apply_rope + the cache writes, sim/tmac_gguf.cpp:1528-1554, :1590-1622).
+ *   q, k, v:  [tokens] rows of `heads` / kv_heads heads of head_dim values of
+ *             `type`; *_stride is the distance of two tokens in elements, so the
+ *             three may lie in one projection's rows.  head_dim even, 2..1024.
+ *   bias:     optional float [(heads + 2 kv_heads) * head_dim], q's then k's then v's.
+ *   seq:      int32 [tokens], the token's row of `tables`; NULL: token t is
+ *             sequence t's.  Negative: padding, its q_out row is zero and nothing
+ *             is stored.
+ *   pos:      int32 [tokens], absolute positions, 0 <= pos < max_pos; others:
+ *             q_out row zero, nothing stored, error recorded.
+ *   starts:   optional int32 [n_seq], the position of each sequence's first own
+ *             key (its shared prefix's length); NULL: 0.  The token's k and v go to
+ *             page tables[seq][(pos - start) / page_size], row (pos - start) %
+ *             page_size; outside the table or the pool: not stored, error recorded.
+ *   cos, sin: float [max_pos][rot_dim / 2].  The first rot_dim (even) values of
+ *             each q and k head turn, in pairs (2i, 2i + 1) if interleaved, else
+ *             (i, i + rot_dim / 2); the others pass through.
+ *   q_out:    [tokens][heads][head_dim] of the cache's type, contiguous.
+ * Two tokens of one call must not go to one place.
+ */
+int tmac_rope_append(const tmac_paged_cache* cache, int type, const void* q, int64_t q_stride, const void* k,
+                     int64_t k_stride, const void* v, int64_t v_stride, int heads, int tokens, const float* bias,
+                     const int32_t* seq, const int32_t* pos, const int32_t* starts, const int32_t* tables, int n_seq,
+                     int table_width, const float* cos, const float* sin, int max_pos, int rot_dim, int interleaved,
+                     void* q_out, void* stream);
+
+/*
+ * Attention of a batch whose sequences share a prefix; the prefix's keys and
+ * values are read once for all of them.  Query token i of sequence b (n_q
+ * tokens, the last of the sequence) sees the first prefix_lens[b] positions of the
+ * prefix and the first own_lens[b] - n_q + 1 + i of the sequence's own; a token
+ * that sees none gets zeros.  Keys that a row does not see do not reach its
+ * result, whatever they hold.
+ *   q, out:       [tokens] rows of `heads` heads of head_dim (64 or 128) values of the
+ *                 cache's type, token strides in elements; query heads
+ *                 h * heads / kv_heads .. share key/value head h.
+ *   q_start:      int32 [batch + 1], non-decreasing: sequence b's tokens are
+ *                 q_start[b] .. q_start[b + 1], at most max_q; NULL: one each
+ *                 (batch = tokens, max_q = 1).
+ *   prefix_pages: int32, the pages of the prefix's prefix_len positions in order.
+ *   prefix_lens:  optional int32 [batch], how much of it each sequence shares;
+ *                 NULL: all.  Larger than prefix_len: counts as prefix_len, recorded.
+ *   tables:       int32 [batch][table_width], the pages of each sequence's own
+ *                 positions in order; entries past its length are not read.
+ *   own_lens:     int32 [batch], 0 .. max_own (larger: counts as max_own, recorded).
+ *   workspace:    tmac_prefix_attention_workspace bytes, 16-byte aligned, free
+ *                 for other use when the call's kernels have run.
+ * Rows of a page outside the pool count as zeros (recorded).
+ */
+int tmac_prefix_attention(const tmac_paged_cache* cache, const void* q, int64_t q_stride, int heads, int tokens,
+                          int batch, const int32_t* q_start, int max_q, const int32_t* prefix_pages, int prefix_len,
+                          const int32_t* prefix_lens, const int32_t* tables, int table_width, const int32_t* own_lens,
+                          int max_own, float scale, void* out, int64_t out_stride, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int tmac_prefix_attention_workspace(const tmac_paged_cache* cache, int heads, int tokens, int batch, int max_q,
+                                    int prefix_len, int max_own, size_t* bytes);
+
+/*
+ * The next token of each row of logits from a given uniform number (stands in
+ * for sample_token, sim/tmac_gguf.cpp:1974-1990, top-k 40 with rand()).
+ *   x = logit * (1 / temperature);  d = max x - x;  w = floor(2^32 exp(-d))
+ * with x and d in 32 bits (NaN counts as -inf) and whole-number sums, so the token
+ * does not depend on the order of the sums.  In the order of (d, index):
+ *   top_k:  the first top_k tokens (<= 0: all);
+ *   top_p:  the shortest first part whose weight reaches top_p times the weight of
+ *           what top_k kept, one token at least (>= 1: all);
+ *   min_p:  those with exp(-d) >= min_p, as 1 if larger (<= 0: all).
+ * A token must pass all three.  The result is the first kept index whose running
+ * weight exceeds floor(u * kept weight); probs is its weight over the kept weight.
+ * temperature not above 0 (or its reciprocal infinite): the lowest index of the
+ * largest logit.  A row without any logit above -inf: token -1, probability 0.
+ *   logits: [batch] rows of `vocab` (up to 720000) values of `type`, row_stride in
+ *           elements.  temperature, top_p, min_p: optional float [batch]; top_k:
+ *           optional int32 [batch]; u: float [batch] in [0, 1).
+ *   tokens: int32 [batch]; probs: float [batch].
+ */
+int tmac_sample(const void* logits, int type, int64_t row_stride, int batch, int vocab, const float* u,
+                const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                int32_t* tokens, float* probs, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ interface for the hot path (sim/tmac_gguf.cpp:466-493):
 * ``matmul_fpga_q8 / _q5_0 / _q4_k / _q6_k / _int16(A, x, y, rows, cols)``
 * ``matmul(A, x, y, rows, cols)``    -- the dispatch switch, driven by ``switches``
 * ``Weight``                          -- a registered device-resident weight
+* ``PagedCache``, ``rope_append``, ``prefix_attention``, ``sample`` -- the batched decode step (serving.py)
 
 There is no CPU fallback: if the library or a B200 is missing, calls raise.
 """
@@ -20,7 +21,9 @@ from dataclasses import dataclass, field
 
 import numpy as np
 
+from . import serving
 from . import synth  # noqa: F401  (seeded synthetic inputs)
+from .serving import BF16, PagedCache, prefix_attention, rope_append, rope_table, sample  # noqa: F401
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libtmac_cuda.so")
@@ -102,6 +105,7 @@ def lib():
             "tmac_gemv_xq": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, _P]),
             "tmac_chain_run": (ctypes.c_int, [_P, ctypes.c_size_t, ctypes.c_uint32, _P, ctypes.c_uint32,
                                               ctypes.c_int, ctypes.POINTER(ChainStats), _P]),
+            **serving.SIGNATURES,
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)
