@@ -9,7 +9,10 @@
 // rot_dim pass through.  Products and sums are 32-bit, rounded once to the
 // cache's type.
 //
-// Bound: HBM, every value is read once and written once.
+// Bound: HBM, every value is read once and written once.  Where the pointers,
+// strides and head parts allow it a thread takes 8 adjoining values (16 bytes of a
+// 16-bit type), or 8 pairs of halves, so a warp moves whole lines; other layouts
+// take one pair per thread.
 #include "serving.cuh"
 
 #include <algorithm>
@@ -112,12 +115,133 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a)
     }
 }
 
+// 8 adjoining elements, in 16-byte (or, in 32 bits, two 16-byte) accesses.
+template <typename T>
+TMAC_DEV void load8(const T* p, float (&x)[8])
+{
+    constexpr int kVec = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; i += kVec) {
+        T r[kVec];
+        *reinterpret_cast<uint4*>(r) = __ldg(reinterpret_cast<const uint4*>(p + i));
+#pragma unroll
+        for (int j = 0; j < kVec; j++) x[i + j] = Elem<T>::load(r + j);
+    }
+}
+template <typename T>
+TMAC_DEV void store8(T* p, const float (&x)[8])
+{
+    constexpr int kVec = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 8; i += kVec) {
+        T r[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; j++) Elem<T>::store(r + j, x[i + j]);
+        *reinterpret_cast<uint4*>(p + i) = *reinterpret_cast<const uint4*>(r);
+    }
+}
+TMAC_DEV void add8(float (&x)[8], const float* bias)
+{
+    float b[8];
+    load8(bias, b);
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = __fadd_rn(x[i], b[i]);
+}
+
+// Units of a token: for each q and k head, 8 values at a time (interleaved), or 8
+// pairs at a time of the rotated part and 8 values at a time of the rest; for
+// each v head, 8 values at a time.
+template <typename T, typename C, bool kInterleaved>
+__global__ void __launch_bounds__(256) rope_append_vec_kernel(RopeArgs a)
+{
+    const int d = a.cache.dim, hk = a.cache.kv_heads, pairs8 = kInterleaved ? 0 : a.rot / 16;
+    const int per_head = pairs8 + (kInterleaved ? d : d - a.rot) / 8, per_v = d / 8;
+    const int turned = (a.heads + hk) * per_head, per_token = turned + hk * per_v;
+    const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, stride = (int64_t)gridDim.x * blockDim.x;
+    const int64_t step_t = stride / per_token;
+    const int step_u = (int)(stride - step_t * per_token);
+    int64_t t = first / per_token;
+    for (int u = (int)(first - t * per_token); t < a.tokens; t += step_t, u += step_u) {
+        if (u >= per_token) {
+            u -= per_token;
+            if (++t >= a.tokens) break;
+        }
+        const bool is_v = u >= turned;
+        const int at = is_v ? u - turned : u, per = is_v ? per_v : per_head;
+        const int row = at / per, unit = at - row * per;  // of q and k together, or of v
+        const bool is_q = !is_v && row < a.heads;
+        const int head = is_v || is_q ? row : row - a.heads;
+        const bool halves = !is_v && unit < pairs8;
+        const int d0 = halves ? unit * 8 : is_v || kInterleaved ? unit * 8 : a.rot + (unit - pairs8) * 8;
+        const int d1 = d0 + a.rot / 2;
+        const T* src = is_q   ? (const T*)a.q + t * a.q_stride
+                       : is_v ? (const T*)a.v + t * a.v_stride
+                              : (const T*)a.k + t * a.k_stride;
+        src += (int64_t)head * d;
+        float x[8], z[8];
+        load8(src + d0, x);
+        if (halves) load8(src + d1, z);
+        if (a.bias) {
+            const float* bias = a.bias + (int64_t)(is_v ? a.heads + hk + row : row) * d;
+            add8(x, bias + d0);
+            if (halves) add8(z, bias + d1);
+        }
+        const Place p = place_of(a, t);
+        C* dst;
+        if (is_q)
+            dst = (C*)a.q_out + (t * a.heads + head) * d;
+        else if (p.page >= 0)
+            dst = (C*)(is_v ? a.cache.v : a.cache.k) + (((p.page * hk + head) << a.cache.page_shift) + p.slot) * d;
+        else
+            continue;
+        if (!p.ok) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = z[i] = 0.0f;
+        } else if (halves) {
+            float c[8], s[8];
+            load8(a.cos + (int64_t)p.pos * (a.rot / 2) + d0, c);
+            load8(a.sin + (int64_t)p.pos * (a.rot / 2) + d0, s);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float xr = __fadd_rn(__fmul_rn(x[i], c[i]), -__fmul_rn(z[i], s[i]));
+                z[i] = __fadd_rn(__fmul_rn(x[i], s[i]), __fmul_rn(z[i], c[i]));
+                x[i] = xr;
+            }
+        } else if (kInterleaved && !is_v && d0 < a.rot) {
+            const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + (int64_t)p.pos * (a.rot / 2) + d0 / 2));
+            const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.sin + (int64_t)p.pos * (a.rot / 2) + d0 / 2));
+            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float xr = __fadd_rn(__fmul_rn(x[2 * i], c[i]), -__fmul_rn(x[2 * i + 1], s[i]));
+                x[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i], s[i]), __fmul_rn(x[2 * i + 1], c[i]));
+                x[2 * i] = xr;
+            }
+        }
+        store8(dst + d0, x);
+        if (halves) store8(dst + d1, z);
+    }
+}
+
+// Whether the 16-byte accesses of the vector kernel are aligned.
+template <typename T, typename C>
+bool vectors_fit(const RopeArgs& a, bool interleaved)
+{
+    auto aligned = [](const void* p) { return (uintptr_t)p % 16 == 0; };
+    const int64_t vec = 16 / (int64_t)sizeof(T);
+    return a.cache.dim % 8 == 0 && a.rot % (interleaved ? 8 : 16) == 0 && aligned(a.q) && aligned(a.k) && aligned(a.v) &&
+           a.q_stride % vec == 0 && a.k_stride % vec == 0 && a.v_stride % vec == 0 && aligned(a.q_out) &&
+           aligned(a.bias) && aligned(a.cos) && aligned(a.sin);
+}
+
 template <typename T, typename C>
 int launch_rope(const RopeArgs& a, bool interleaved, int sms, cudaStream_t s)
 {
-    const int64_t n = a.tokens * (a.heads + 2 * a.cache.kv_heads) * (a.cache.dim / 2);
+    const bool vec = vectors_fit<T, C>(a, interleaved);
+    const int64_t n = a.tokens * (a.heads + 2 * a.cache.kv_heads) * (a.cache.dim / (vec ? 8 : 2));
     const int grid = (int)std::min<int64_t>((n + 255) / 256, (int64_t)sms * 8);
-    auto fn = interleaved ? rope_append_kernel<T, C, true> : rope_append_kernel<T, C, false>;
+    auto fn = vec ? interleaved ? rope_append_vec_kernel<T, C, true> : rope_append_vec_kernel<T, C, false>
+                  : interleaved ? rope_append_kernel<T, C, true> : rope_append_kernel<T, C, false>;
     fn<<<grid, 256, 0, s>>>(a);
     TMAC_CUDA_TRY(cudaGetLastError());
     return TMAC_OK;
