@@ -13,14 +13,16 @@
 // the token is the first kept index whose running weight passes u times the
 // kept weight.
 //
-// One cluster of CTAs per row holds the row's d in shared memory, so the logits
-// are read from HBM once.  The cut of top-k / top-p lies within a few units of
-// the largest logit as a rule: one pass counts how many tokens lie within 1, 2, 4
-// and 8 of it, and where at most kList of them hold the cut they are gathered in
-// one CTA, sorted, and the draw ends there.  Otherwise (flat rows) the cut is
-// found by radix selection on the bits of d over the whole cluster: a 1024-bin
-// histogram of counts and weights per round, at most five rounds, each bin
-// summed through distributed shared memory.
+// One cluster of CTAs per row holds the row's x in shared memory, so the logits
+// are read from HBM once.  Three ways to the cut:
+//  * top-k: the k-th largest of the threads' own maxima bounds the k-th largest
+//    logit from below, and closely, since a thread holds a few dozen logits.  The
+//    tokens above the bound are gathered in one CTA, sorted, and the draw ends there.
+//  * top-p alone: its cut may lie anywhere, so a histogram of the weights over d
+//    (bins of 1/22) is summed through distributed shared memory; every CTA then
+//    gathers and sorts the tokens of the one bin that holds the cut.
+//  * where the tokens to gather do not fit (many equal ones, a large k): radix
+//    selection on the bits of d, one histogram per round, at most five rounds.
 //
 // Bound: HBM for large batches (every logit is read once), latency for one row.
 #include "serving.cuh"
@@ -34,12 +36,16 @@ namespace cg = cooperative_groups;
 namespace tmac {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024;
-constexpr float kBinScale = 45.5f;  // bins per unit of d in the first round; d < 22.2 where w > 0
+#ifndef KFLIGHT
+#define KFLIGHT 4
+#endif
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 512;
+constexpr float kBinScale = 22.5f;  // bins per unit of d in the first round; d < 22.2 where w > 0
 constexpr int kMaxCluster = 16, kMaxSlice = 45000;
-constexpr int kList = 2048, kWindows = 4;  // window i: d < 2^i
+constexpr int kList = 2048, kLocal = 512;  // tokens gathered in one CTA, listed by each
+constexpr int kSteps = 64, kFirstStep = (127 - 4) << 3;  // bounds on d, eight to an octave from 1/16 to 16
+static_assert(kThreads >= kBins && kThreads * kMaxCluster / kBins <= 32, "the threads of a bin are lanes of a warp");
 static_assert(kBins / kMaxCluster % 32 == 0, "a share's bins go to the lanes of a warp");
-static_assert(kMaxSlice / kThreads < 255, "a thread's counts are bytes");
 
 struct SampleArgs {
     const void* logits;
@@ -52,54 +58,57 @@ struct SampleArgs {
     float* probs;
 };
 
-struct Histogram {
-    uint32_t cnt[kBins], hi[kBins], lo[kBins];  // this CTA's: counts, weights in two halves
+struct Shared {
+    uint32_t cnt[kBins], hi[kBins], lo[kBins];  // this CTA's histogram: counts, weights in two halves
     uint32_t mcnt[kBins];                       // this CTA's share of the bins, summed over the cluster
     unsigned long long mw[kBins];
-};
-struct List {
-    unsigned long long key[kList], sorted[kList];  // bits(d) << 32 | index; by index, and in order
-};
-struct Shared {
-    union {
-        Histogram h;
-        List list;
-    };
+    unsigned long long key[kList], local[kLocal];  // bits(d) << 32 | index
     unsigned long long share_w, red_w[kWarps];
     uint32_t share_c, red_c[kWarps];
     float red_f[kWarps], cta_max;
     int cta_min_index;
-    uint32_t warp_count[kWarps][kWindows], count[kWindows];  // tokens in each window: by warp, of the CTA
-    uint32_t tie_count;
-    unsigned long long kept;
+    alignas(8) uint32_t maxima[kSteps];  // the threads' maxima by their distance from the row's
+    uint32_t n_local;         // listed tokens; more than kLocal: not all of them
+    uint32_t tie_count, n_keep;
+    unsigned long long kept, cut_weight, cut_key;
     // broadcast of a search
     int found_bin, tie_index;
     uint32_t found_c, before_c;
     unsigned long long found_w, before_w;
-    uint32_t n_keep;
 };
 
 TMAC_DEV float weight_exp(float d) { return expf(-d); }
 TMAC_DEV unsigned long long weight_of(float e)
 {
-    return e >= 1.0f ? 0x100000000ull : (unsigned long long)(uint32_t)__fmul_rn(e, 4294967296.0f);
+    // the conversion saturates at 2^32 - 1, which e = 1 alone reaches
+    return (unsigned long long)(uint32_t)__float2uint_rz(__fmul_rn(e, 4294967296.0f)) + (e >= 1.0f);
 }
 TMAC_DEV int first_bin(float d) { return min((int)__fmul_rn(d, kBinScale), kBins - 1); }
 
 // The first part of a row's order that is kept: first_bin(d) < bin, or == bin and
-// bits(d) <= key; among bits(d) == key only indexes up to tie_index.
+// (bits(d), index) up to `last`.
+TMAC_DEV unsigned long long order_key(float d, int index)
+{
+    return (unsigned long long)__float_as_uint(d) << 32 | (uint32_t)index;
+}
 struct Cut {
-    int bin;
-    uint32_t key;
-    int tie_index;
-    unsigned long long weight;  // of what it keeps
+    int bin = kBins;
+    float from = INFINITY, to = INFINITY;  // bounds on the d of the bin, widened for the product's rounding
+    unsigned long long last = ~0ull;
+    unsigned long long weight = 0;  // of what it keeps
+    TMAC_DEV void set_bin(int b)
+    {
+        bin = b;
+        from = __fmul_rn(__fdiv_rn((float)b, kBinScale), 0.999999f);
+        to = __fmul_rn(__fdiv_rn((float)(b + 1), kBinScale), 1.000001f);
+    }
 };
 TMAC_DEV bool kept_by(const Cut& c, float d, int index)
 {
+    if (d < c.from) return true;
+    if (!(d < c.to)) return false;
     const int b = first_bin(d);
-    if (b != c.bin) return b < c.bin;
-    const uint32_t key = __float_as_uint(d);
-    return key < c.key || (key == c.key && index <= c.tie_index);
+    return b < c.bin || (b == c.bin && order_key(d, index) <= c.last);
 }
 
 template <typename V>
@@ -118,6 +127,34 @@ TMAC_DEV V warp_scan(V v)  // inclusive
     return v;
 }
 
+// Sorts keys[0 .. n), n up to kList, which must have room for the next power of two
+// (64 at least): a bitonic network, whose steps of distance 32 and less stay
+// within the 64 keys of a warp.
+TMAC_DEV void sort_keys(unsigned long long* keys, int count)
+{
+    int n = 64;
+    while (n < count) n <<= 1;
+    for (int i = count + threadIdx.x; i < n; i += kThreads) keys[i] = ~0ull;
+    __syncthreads();
+    for (int size = 2; size <= n; size <<= 1) {
+        for (int step = size >> 1; step > 0; step >>= 1) {
+            for (int t = threadIdx.x; t < n / 2; t += kThreads) {
+                const int i = 2 * t - (t & (step - 1)), j = i + step;
+                const unsigned long long x = keys[i], y = keys[j];
+                if ((x > y) == ((i & size) == 0)) {
+                    keys[i] = y;
+                    keys[j] = x;
+                }
+            }
+            if (step > 32 || (step == 1 && size >= 64))
+                __syncthreads();
+            else
+                __syncwarp();
+        }
+    }
+    __syncthreads();
+}
+
 // floor(u * total), inside [0, total) whatever u is
 TMAC_DEV unsigned long long pick_of(float u, unsigned long long total)
 {
@@ -126,59 +163,139 @@ TMAC_DEV unsigned long long pick_of(float u, unsigned long long total)
     return pick < total ? pick : total - 1;
 }
 
+// Exclusive running sum over the block of each thread's v; *total gets the sum of all.
+TMAC_DEV unsigned long long block_scan(unsigned long long v, unsigned long long* red, unsigned long long* total)
+{
+    const unsigned long long up = warp_scan(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 31) red[threadIdx.x >> 5] = up;
+    __syncthreads();
+    unsigned long long before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; i++) {
+        const unsigned long long r = red[i];
+        if (i < (int)(threadIdx.x >> 5)) before += r;
+        all += r;
+    }
+    *total = all;
+    return before + up - v;
+}
+
 struct Row {
     cg::cluster_group cl;
     Shared* sh;
-    float* d;        // this CTA's slice
-    int n, begin;    // its length and first index
+    float* x;        // this CTA's scaled logits
+    int n, begin;    // their number and first index
+    int pad;         // -inf before x (and after it), so that whole float4 are read
     int ranks, rank;
+    float mx;        // the row's largest
 
-    // Calls f(value, local index) over the warp's own contiguous part, in order, 32 at a time.
+    TMAC_DEV float d_of(float v) const { return __fsub_rn(mx, v); }
+
+    // Calls f(d, local index) over the thread's own contiguous part, in order.
+    // An odd number each: a warp's accesses fall on different banks.
     template <typename F>
-    TMAC_DEV void walk(F&& f) const
+    TMAC_DEV void each(F&& f) const
     {
-        const int per = (((n + kWarps - 1) / kWarps) + 31) & ~31;
-        const int from = (threadIdx.x >> 5) * per, to = min(n, from + per);
-        for (int i = from; i < to; i += 32) {
-            const int j = i + (threadIdx.x & 31);
-            f(j < to ? d[j] : INFINITY, j, j < to);
+        const int per = ((n + kThreads - 1) / kThreads) | 1;
+        const int from = threadIdx.x * per, to = min(n, from + per);
+        int i = from;
+        for (; i + 4 <= to; i += 4) {
+            const float v0 = x[i], v1 = x[i + 1], v2 = x[i + 2], v3 = x[i + 3];
+            f(d_of(v0), i);
+            f(d_of(v1), i + 1);
+            f(d_of(v2), i + 2);
+            f(d_of(v3), i + 3);
         }
+        for (; i < to; i++) f(d_of(x[i]), i);
     }
 
-    // Adds the counts and weights of the local elements for which bin_of gives a bin.
+    // Lists the tokens with from <= d < to for which `which` holds too, as long as
+    // they fit, in any order, and waits for the cluster's lists.
     template <typename F>
-    TMAC_DEV void histogram(F&& bin_of)
+    TMAC_DEV void list(float from, float to, F&& which)
     {
-        for (int i = threadIdx.x; i < kBins; i += kThreads) sh->h.cnt[i] = sh->h.hi[i] = sh->h.lo[i] = 0;
+        if (threadIdx.x == 0) sh->n_local = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const float v = d[i];
-            const unsigned long long w = weight_of(weight_exp(v));
-            if (!w) continue;
-            const int b = bin_of(v);
-            if (b < 0) continue;
-            // a slice has at most kMaxSlice elements of at most 2^16 in either half: no overflow
-            atomicAdd(&sh->h.cnt[b], 1u);
-            atomicAdd(&sh->h.hi[b], (uint32_t)(w >> 16));
-            atomicAdd(&sh->h.lo[b], (uint32_t)(w & 0xFFFF));
+        const float4* v = reinterpret_cast<const float4*>(x - pad);
+        const int vecs = (pad + n + 3) / 4;
+        const volatile uint32_t* listed = &sh->n_local;
+        for (int i = threadIdx.x; i < vecs; i += kThreads) {
+            const float4 q = v[i];
+            const float e[4] = {d_of(q.x), d_of(q.y), d_of(q.z), d_of(q.w)};
+            bool any = false;
+#pragma unroll
+            for (int c = 0; c < 4; c++) any |= e[c] < to && e[c] >= from;
+            if (any && *listed <= kLocal)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if (e[c] >= from && e[c] < to && which(e[c])) {
+                        const uint32_t at = atomicAdd(&sh->n_local, 1u);
+                        if (at < kLocal) sh->local[at] = order_key(e[c], begin + 4 * i + c - pad);
+                    }
         }
         cl.sync();
-        // this rank's share of the bins, over all ranks
-        const int share = kBins / ranks;
+    }
+    // The number of the cluster's listed tokens, or -1 if they do not fit in one CTA;
+    // this rank's come after `offset`.
+    TMAC_DEV int listed(uint32_t* offset) const
+    {
+        const int lane = threadIdx.x & 31;
+        const uint32_t c = lane < ranks ? cl.map_shared_rank(sh, lane)->n_local : 0, up = warp_scan(c);
+        const uint32_t all = __shfl_sync(0xffffffffu, up, 31);
+        *offset = __shfl_sync(0xffffffffu, up - c, rank);
+        return __any_sync(0xffffffffu, c > kLocal) || all > kList ? -1 : (int)all;
+    }
+    // Copies every rank's listed tokens into this CTA's keys.
+    TMAC_DEV void gather() const
+    {
+        uint32_t at = 0;
+        for (int r = 0; r < ranks; r++) {
+            const Shared* o = cl.map_shared_rank(sh, r);
+            const uint32_t c = o->n_local;
+            for (uint32_t i = threadIdx.x; i < c; i += kThreads) sh->key[at + i] = o->local[i];
+            at += c;
+        }
+        __syncthreads();
+    }
+
+    // Sums the weights (and with kCounts the numbers) of the elements for which bin_of gives a bin.
+    template <bool kCounts, typename F>
+    TMAC_DEV void histogram(F&& bin_of)
+    {
+        for (int i = threadIdx.x; i < kBins; i += kThreads) sh->cnt[i] = sh->hi[i] = sh->lo[i] = 0;
+        __syncthreads();
+        each([&](float v, int) {
+            const int b = bin_of(v);
+            if (b < 0) return;
+            const unsigned long long w = weight_of(weight_exp(v));
+            if (!w) return;
+            // a slice has at most kMaxSlice elements of at most 2^16 in either half: no overflow
+            if (kCounts) atomicAdd(&sh->cnt[b], 1u);
+            atomicAdd(&sh->hi[b], (uint32_t)(w >> 16));
+            atomicAdd(&sh->lo[b], (uint32_t)(w & 0xFFFF));
+        });
+        cl.sync();
+        // this rank's share of the bins, over all ranks: `each` threads to a bin
+        const int share = kBins / ranks, each = kThreads / share;
         uint32_t c_sum = 0;
         unsigned long long w_sum = 0;
-        for (int i = threadIdx.x; i < share; i += kThreads) {
-            uint32_t c = 0;
-            unsigned long long w = 0;
-            for (int r = 0; r < ranks; r++) {
-                const Shared* o = cl.map_shared_rank(sh, r);
-                c += o->h.cnt[rank * share + i];
-                w += ((unsigned long long)o->h.hi[rank * share + i] << 16) + o->h.lo[rank * share + i];
-            }
-            sh->h.mcnt[i] = c;
-            sh->h.mw[i] = w;
-            c_sum += c;
-            w_sum += w;
+        const int bin = threadIdx.x / each, part = threadIdx.x % each;
+        for (int r = part; r < ranks; r += each) {
+            const Shared* o = cl.map_shared_rank(sh, r);
+            c_sum += o->cnt[rank * share + bin];
+            w_sum += ((unsigned long long)o->hi[rank * share + bin] << 16) + o->lo[rank * share + bin];
+        }
+        for (int o = each / 2; o > 0; o >>= 1) {
+            c_sum += __shfl_xor_sync(0xffffffffu, c_sum, o);
+            w_sum += __shfl_xor_sync(0xffffffffu, w_sum, o);
+        }
+        if (part == 0) {
+            sh->mcnt[bin] = c_sum;
+            sh->mw[bin] = w_sum;
+        } else {
+            c_sum = 0;
+            w_sum = 0;
         }
         c_sum = warp_sum(c_sum);
         w_sum = warp_sum(w_sum);
@@ -224,8 +341,8 @@ struct Row {
                 c = 0;
                 w = 0;
                 for (int i = 0; i < per; i++) {
-                    c += o->h.mcnt[lane * per + i];
-                    w += o->h.mw[lane * per + i];
+                    c += o->mcnt[lane * per + i];
+                    w += o->mw[lane * per + i];
                 }
                 up_c = base_c + warp_scan(c);
                 up_w = base_w + warp_scan(w);
@@ -234,8 +351,8 @@ struct Row {
                     c = up_c - c;
                     w = up_w - w;
                     for (int i = lane * per;; i++) {
-                        const uint32_t bc = o->h.mcnt[i];
-                        const unsigned long long bw = o->h.mw[i];
+                        const uint32_t bc = o->mcnt[i];
+                        const unsigned long long bw = o->mw[i];
                         if (reached(c + bc, w + bw) || i + 1 == (lane + 1) * per) {
                             sh->found_bin = r * share + i;
                             sh->found_c = bc;
@@ -258,156 +375,142 @@ struct Row {
     TMAC_DEV int tie(uint32_t key, uint32_t m)
     {
         uint32_t c = 0;
-        walk([&](float v, int, bool in) { c += __popc(__ballot_sync(0xffffffffu, in && __float_as_uint(v) == key)); });
-        const int warp = threadIdx.x >> 5;
-        if ((threadIdx.x & 31) == 0) sh->red_c[warp] = c;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            uint32_t s = 0;
-            for (int i = 0; i < kWarps; i++) s += sh->red_c[i];
-            sh->tie_count = s;
-        }
+        each([&](float v, int) { c += __float_as_uint(v) == key; });
+        unsigned long long all;
+        uint32_t before = (uint32_t)block_scan(c, sh->red_w, &all);
+        if (threadIdx.x == 0) sh->tie_count = (uint32_t)all;
         cl.sync();
-        uint32_t before = 0;
         for (int r = 0; r < rank; r++) before += cl.map_shared_rank(sh, r)->tie_count;
-        for (int i = 0; i < warp; i++) before += sh->red_c[i];
         if (before < m && m <= before + c)
-            walk([&](float v, int j, bool in) {
-                const bool eq = in && __float_as_uint(v) == key;
-                const uint32_t mask = __ballot_sync(0xffffffffu, eq);
-                const uint32_t mine = before + __popc(mask & (0xFFFFFFFFu >> (31 - (threadIdx.x & 31))));
-                if (eq && mine == m)
+            each([&](float v, int j) {
+                if (__float_as_uint(v) == key && ++before == m)
                     for (int r = 0; r < ranks; r++) cl.map_shared_rank(sh, r)->tie_index = begin + j;
-                before += __popc(mask);
             });
         cl.sync();
         return sh->tie_index;
     }
 
-    // Cuts the order after its first k elements (k > 0), or after the element at
-    // which the running weight reaches t (k == 0).  Elements of weight 0 do not count.
-    TMAC_DEV Cut select(uint32_t k, double t)
+    // Cuts the order after its first k elements (k > 0), or after the element at which
+    // the running weight reaches p times the weight of the row (or of `of`, if not 0).
+    // Elements of weight 0 do not count.
+    TMAC_DEV Cut select(uint32_t k, float p, unsigned long long of)
     {
-        Cut cut = {kBins, 0xFFFFFFFFu, 0x7FFFFFFF, 0};
-        histogram([&](float v) { return first_bin(v); });
+        Cut cut;
+        // far tokens (all of weight 0) fill the last bin: leave them out
+        const auto bin_of = [&](float v) { const int c = first_bin(v); return c < kBins - 1 ? c : -1; };
+        if (k)
+            histogram<true>(bin_of);
+        else
+            histogram<false>(bin_of);
+        const int lane = threadIdx.x & 31;
+        const unsigned long long row_w = warp_sum(lane < ranks ? cl.map_shared_rank(sh, lane)->share_w : 0);
+        const double t = __dmul_rn((double)p, (double)(of ? of : row_w));
         if (!search(k, t, 0, 0)) {  // fewer than k: all of them
-            for (int r = 0; r < ranks; r++) cut.weight += cl.map_shared_rank(sh, r)->share_w;
+            cut.weight = row_w;
             return cut;
         }
-        cut.bin = sh->found_bin;
-        // bits of d that the bin can hold, a little widened for the product's rounding
-        uint32_t lo = __float_as_uint((float)cut.bin / kBinScale * 0.999999f);
-        uint32_t span = __float_as_uint((float)(cut.bin + 1) / kBinScale * 1.000001f) - lo + 1;
+        cut.set_bin(sh->found_bin);
+        uint32_t found_c = sh->found_c, before_c = sh->before_c;
+        unsigned long long found_w = sh->found_w, before_w = sh->before_w;
+        list(cut.from, cut.to, [&](float v) { return first_bin(v) == cut.bin; });
+        uint32_t offset;
+        const int n = listed(&offset);
+        if (n >= 0) {
+            gather();
+            cut_list(n, k ? k - before_c : 0, t, before_w);
+            cl.sync();  // the lists are free again
+            cut.last = sh->cut_key;
+            cut.weight = sh->cut_weight;
+            return cut;
+        }
+        uint32_t lo = __float_as_uint(cut.from), span = __float_as_uint(cut.to) - lo + 1;
         while (true) {
-            const uint32_t found_c = sh->found_c, before_c = sh->before_c;
-            const unsigned long long found_w = sh->found_w, before_w = sh->before_w;
-            if (found_c == 1 || (k && before_c + found_c == k) || span == 1) {
-                uint32_t m = found_c;
-                unsigned long long w = found_w;
-                if (span == 1) {
-                    const unsigned long long each = found_w / found_c;
-                    if (k)
-                        m = k - before_c;
-                    else  // the least m with before + m * each >= t
-                        for (uint32_t a = 1, b = found_c; a <= b;) {
-                            const uint32_t c = (a + b) / 2;
-                            if ((double)(before_w + c * each) >= t) {
-                                m = c;
-                                b = c - 1;
-                            } else {
-                                a = c + 1;
-                            }
-                        }
-                    w = m * each;
-                }
-                cut.weight = before_w + w;
-                cut.key = cut.key == 0xFFFFFFFFu && span != 1 ? cut.key : lo + span - 1;
-                if (m < found_c) cut.tie_index = tie(lo, m);
-                return cut;
-            }
             int shift = 0;
             while ((span - 1) >> shift >= kBins) shift++;
-            cut.key = 0;  // from here on `lo + span` bounds the keys
-            __syncthreads();  // every thread has read the last search
-            histogram([&](float v) {
+            histogram<true>([&](float v) {
                 const uint32_t o = __float_as_uint(v) - lo;
                 return first_bin(v) == cut.bin && o < span ? (int)(o >> shift) : -1;
             });
             if (!search(k, t, before_c, before_w)) return cut;  // cannot happen: the bin holds the cut
             lo += (uint32_t)sh->found_bin << shift;
             span = 1u << shift;
+            found_c = sh->found_c;
+            before_c = sh->before_c;
+            found_w = sh->found_w;
+            before_w = sh->before_w;
+            if (found_c == 1 || (k && before_c + found_c == k) || span == 1) break;
+            __syncthreads();  // every thread has read the search
         }
+        uint32_t m = found_c;
+        if (span == 1) {  // equal ones: the first m of them
+            const unsigned long long each = found_w / found_c;
+            if (k)
+                m = k - before_c;
+            else  // the least m with before + m * each >= t
+                for (uint32_t a = 1, b = found_c; a <= b;) {
+                    const uint32_t c = (a + b) / 2;
+                    if ((double)(before_w + c * each) >= t) {
+                        m = c;
+                        b = c - 1;
+                    } else {
+                        a = c + 1;
+                    }
+                }
+            found_w = m * each;
+        }
+        cut.weight = before_w + found_w;
+        cut.last = (unsigned long long)(lo + span - 1) << 32 | 0xFFFFFFFFu;
+        if (m < found_c) cut.last = (unsigned long long)lo << 32 | (uint32_t)tie(lo, m);
+        return cut;
+    }
+
+    // Cuts the n gathered tokens after their first k (k > 0), or where base plus their
+    // running weight reaches t: cut_key, and cut_weight with base.
+    TMAC_DEV void cut_list(int n, uint32_t k, double t, unsigned long long base)
+    {
+        constexpr int kPer = kList / kThreads;
+        sort_keys(sh->key, n);
+        unsigned long long w[kPer], sum = 0, all;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int at = threadIdx.x * kPer + i;
+            w[i] = at < n ? weight_of(weight_exp(__uint_as_float((uint32_t)(sh->key[at] >> 32)))) : 0;
+            sum += w[i];
+        }
+        unsigned long long before = base + block_scan(sum, sh->red_w, &all);
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int at = threadIdx.x * kPer + i;
+            const bool last = k ? at == (int)k - 1 : (double)before < t && (double)(before + w[i]) >= t;
+            if (at < n && last) {
+                sh->cut_key = sh->key[at];
+                sh->cut_weight = before + w[i];
+            }
+            before += w[i];
+        }
+        __syncthreads();
     }
 };
 
-// Exclusive running sum over the block of each thread's v; *total gets the sum of all.
-TMAC_DEV unsigned long long block_scan(unsigned long long v, unsigned long long* red, unsigned long long* total)
-{
-    const unsigned long long up = warp_scan(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 31) red[threadIdx.x >> 5] = up;
-    __syncthreads();
-    unsigned long long before = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; i++) {
-        const unsigned long long r = red[i];
-        if (i < (int)(threadIdx.x >> 5)) before += r;
-        all += r;
-    }
-    *total = all;
-    return before + up - v;
-}
-
-// Sorts keys[0 .. n), n a power of two of 64 at least: a bitonic network, whose
-// steps of distance 32 and less stay within the 64 keys of a warp.
-TMAC_DEV void sort_keys(unsigned long long* keys, int n)
-{
-    for (int size = 2; size <= n; size <<= 1) {
-        for (int step = size >> 1; step > 0; step >>= 1) {
-            for (int t = threadIdx.x; t < n / 2; t += kThreads) {
-                const int i = 2 * t - (t & (step - 1)), j = i + step;
-                const unsigned long long x = keys[i], y = keys[j];
-                if ((x > y) == ((i & size) == 0)) {
-                    keys[i] = y;
-                    keys[j] = x;
-                }
-            }
-            if (step > 32 || (step == 1 && size >= 64))
-                __syncthreads();
-            else
-                __syncwarp();
-        }
-    }
-    __syncthreads();
-}
-
-// The cut and the draw over the n gathered tokens (in the order of their indexes).
-// total: the row's weight when top_k is off.  false: top_p's cut lies beyond them.
-TMAC_DEV bool draw_from_list(const SampleArgs& a, Shared* sh, int b, int n, int k, float p, float m, unsigned long long total)
+// The cuts and the draw over the n gathered tokens, the first k of the order among them.
+TMAC_DEV void draw_from_list(const SampleArgs& a, Shared* sh, int b, int n, int k, float p, float m)
 {
     constexpr int kPer = kList / kThreads;
-    List& list = sh->list;
-    int size = 64;
-    while (size < n) size <<= 1;
-    for (int i = threadIdx.x; i < size; i += kThreads) list.sorted[i] = i < n ? list.key[i] : ~0ull;
+    unsigned long long* key = sh->key;
     if (threadIdx.x == 0) sh->n_keep = 1;
-    __syncthreads();
-    sort_keys(list.sorted, size);
-    const int n_k = k > 0 ? min(k, n) : n;
-
+    sort_keys(key, n);
+    const int n_k = min(k, n);
     float e[kPer];
     unsigned long long w[kPer], sum = 0, all;
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
         const int at = threadIdx.x * kPer + i;
-        e[i] = at < n_k ? weight_exp(__uint_as_float((uint32_t)(list.sorted[at] >> 32))) : 0.0f;
+        e[i] = at < n_k ? weight_exp(__uint_as_float((uint32_t)(key[at] >> 32))) : 0.0f;
         w[i] = at < n_k ? weight_of(e[i]) : 0;
         sum += w[i];
     }
     unsigned long long before = block_scan(sum, sh->red_w, &all);
-    if (k > 0) total = all;
-    const double t = __dmul_rn((double)p, (double)total);
-    if (p < 1.0f && (double)all < t) return false;
+    const double t = __dmul_rn((double)p, (double)all);
     uint32_t keep = 0;  // the longest kept first part that ends with one of this thread's
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
@@ -418,45 +521,47 @@ TMAC_DEV bool draw_from_list(const SampleArgs& a, Shared* sh, int b, int n, int 
     keep = __reduce_max_sync(0xffffffffu, keep);
     if ((threadIdx.x & 31) == 0 && keep) atomicMax(&sh->n_keep, keep);
     __syncthreads();
-    const unsigned long long last = list.sorted[sh->n_keep - 1];
+    const int kept = (int)sh->n_keep;
 
+    // the kept ones in the order of their indexes
+    for (int i = threadIdx.x; i < kept; i += kThreads) key[i] = key[i] << 32 | key[i] >> 32;
+    sort_keys(key, kept);
     sum = 0;
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
         const int at = threadIdx.x * kPer + i;
-        const unsigned long long key = at < n ? list.key[at] : ~0ull;
-        w[i] = key <= last ? weight_of(weight_exp(__uint_as_float((uint32_t)(key >> 32)))) : 0;
+        w[i] = at < kept ? weight_of(weight_exp(__uint_as_float((uint32_t)key[at]))) : 0;
         sum += w[i];
     }
     before = block_scan(sum, sh->red_w, &all);
     const unsigned long long pick = pick_of(a.u[b], all);
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
-        if (w[i] && before <= pick && pick < before + w[i]) {
-            a.tokens[b] = (int)(uint32_t)list.key[threadIdx.x * kPer + i];
+        if (before <= pick && pick < before + w[i]) {
+            a.tokens[b] = (int)(key[threadIdx.x * kPer + i] >> 32);
             a.probs[b] = (float)__ddiv_rn((double)w[i], (double)all);
         }
         before += w[i];
     }
-    return true;
 }
 
-// x = l * inv of the CTA's n logits into d, NaN as -inf; the largest of the thread's.
+// l * inv of the CTA's n logits into x, NaN as -inf, and `pad` (and up to 3 more
+// behind) -inf around them; the largest of the thread's.  x + head is 16-byte aligned.
 template <typename T>
-TMAC_DEV float load_scaled(const T* l, int n, float inv, float* d)
+TMAC_DEV float load_scaled(const T* l, int n, int head, float inv, float* x, int pad)
 {
     float mx = -INFINITY;
-    auto put = [&](int i, float v) {
-        float x = __fmul_rn(v, inv);
-        if (isnan(x)) x = -INFINITY;
-        d[i] = x;
-        mx = fmaxf(mx, x);
+    auto put = [&](int i) {
+        x[i] = fmaxf(__fmul_rn(Elem<T>::load(l + i), inv), -INFINITY);  // fmaxf leaves a NaN out
+        mx = fmaxf(mx, x[i]);
     };
-    constexpr int kVec = 16 / sizeof(T), kFlight = 4;
-    const int head = min(n, (int)((16 - (uintptr_t)l % 16) % 16 / sizeof(T))), vecs = (n - head) / kVec;
-    if ((int)threadIdx.x < head) put(threadIdx.x, Elem<T>::load(l + threadIdx.x));
-    const int tail = head + vecs * kVec;
-    if ((int)threadIdx.x < n - tail) put(tail + threadIdx.x, Elem<T>::load(l + tail + threadIdx.x));
+    constexpr int kVec = 16 / sizeof(T), kFlight = KFLIGHT;
+    head = min(n, head);
+    const int vecs = (n - head) / kVec, tail = head + vecs * kVec;
+    if ((int)threadIdx.x < head) put(threadIdx.x);
+    if ((int)threadIdx.x < n - tail) put(tail + threadIdx.x);
+    if ((int)threadIdx.x < pad) x[-1 - (int)threadIdx.x] = -INFINITY;
+    if ((int)threadIdx.x < 3) x[n + threadIdx.x] = -INFINITY;
     const uint4* v = reinterpret_cast<const uint4*>(l + head);
     for (int i0 = threadIdx.x; i0 < vecs; i0 += kThreads * kFlight) {
         uint4 r[kFlight];
@@ -466,20 +571,18 @@ TMAC_DEV float load_scaled(const T* l, int n, float inv, float* d)
 #pragma unroll
         for (int f = 0; f < kFlight; f++) {
             if (i0 + f * kThreads >= vecs) break;
-            T x[kVec];
-            *reinterpret_cast<uint4*>(x) = r[f];
+            T in[kVec];
+            *reinterpret_cast<uint4*>(in) = r[f];
             float4 y[kVec / 4];
             float* yf = reinterpret_cast<float*>(y);
 #pragma unroll
             for (int c = 0; c < kVec; c++) {
-                yf[c] = __fmul_rn(Elem<T>::load(x + c), inv);
-                if (isnan(yf[c])) yf[c] = -INFINITY;
+                yf[c] = fmaxf(__fmul_rn(Elem<T>::load(in + c), inv), -INFINITY);
                 mx = fmaxf(mx, yf[c]);
             }
-            // d is laid so that element `head` is 16-byte aligned
 #pragma unroll
             for (int c = 0; c < kVec / 4; c++)
-                *reinterpret_cast<float4*>(d + head + (i0 + f * kThreads) * kVec + 4 * c) = y[c];
+                *reinterpret_cast<float4*>(x + head + (i0 + f * kThreads) * kVec + 4 * c) = y[c];
         }
     }
     return mx;
@@ -500,7 +603,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     const T* l = (const T*)a.logits + b * a.stride + row.begin;
     // the first logit on a 16-byte boundary goes to one of shared memory
     const int head = (int)((16 - (uintptr_t)l % 16) % 16 / sizeof(T));
-    row.d = reinterpret_cast<float*>(smem + (sizeof(Shared) + 15) / 16 * 16) + (4 - head % 4) % 4;
+    row.pad = (4 - head % 4) % 4;
+    row.x = reinterpret_cast<float*>(smem + (sizeof(Shared) + 15) / 16 * 16) + row.pad;
 
     const float temperature = a.temperature ? a.temperature[b] : 1.0f;
     float inv = __frcp_rn(temperature);
@@ -517,9 +621,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     m = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
 
     // scaled logits, and the largest of the row
-    float mx = load_scaled<T>(l, row.n, inv, row.d);
+    const float own_max = load_scaled<T>(l, row.n, head, inv, row.x, row.pad);
+    float mx = own_max;
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (lane == 0) sh->red_f[warp] = mx;
+    if (threadIdx.x < kSteps) sh->maxima[threadIdx.x] = 0;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < kWarps; i++) mx = fmaxf(mx, sh->red_f[i]);
@@ -528,7 +634,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     row.cl.sync();
     mx = lane < row.ranks ? row.cl.map_shared_rank(sh, lane)->cta_max : -INFINITY;
     for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    mx = __shfl_sync(0xffffffffu, mx, 0);
+    mx = row.mx = __fadd_rn(__shfl_sync(0xffffffffu, mx, 0), 0.0f);  // -0 as 0: no d is -0
+    if (mx == INFINITY) {  // the infinite ones share the weight, at d = 0
+        for (int i = threadIdx.x; i < row.n; i += kThreads) row.x[i] = row.x[i] == INFINITY ? 0.0f : -INFINITY;
+        mx = row.mx = 0.0f;
+        __syncthreads();
+    }
     if (mx == -INFINITY) {  // nothing to choose from
         row.cl.sync();
         if (row.rank == 0 && threadIdx.x == 0) {
@@ -541,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     if (greedy || k == 1) {  // the lowest index of the largest
         int first = 0x7FFFFFFF;
         for (int i = threadIdx.x; i < row.n; i += kThreads)
-            if (row.d[i] == mx) first = min(first, row.begin + i);
+            if (row.x[i] == mx) first = min(first, row.begin + i);
         first = __reduce_min_sync(0xffffffffu, first);
         if (lane == 0) sh->red_c[warp] = (uint32_t)first;
         __syncthreads();
@@ -559,134 +670,71 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
         return;
     }
 
-    // d, the tokens in each window, and the row's weight where the cut or the draw needs it
-    const bool cuts = k > 0 || p < 1.0f, weigh = k <= 0;
-    unsigned long long mine = 0;
-    uint32_t counts = 0;  // of d < 1, [1, 2), [2, 4), [4, 8), a byte each
-    row.walk([&](float x, int j, bool in) {
-        if (!in) return;
-        const float d = x == mx ? 0.0f : __fsub_rn(mx, x);
-        row.d[j] = d;
-        if (cuts && d < 8.0f) counts += 1u << (8 * max((int)(__float_as_uint(d) >> 23) - 126, 0));
-        if (weigh) {
-            const float e = weight_exp(d);
-            // a cut by top-p is measured before min_p applies
-            if (cuts || e >= m) mine += weight_of(e);
+    Cut cut;
+    if (k > 0) {
+        // the least bound on d below which k threads have their maximum
+        const float own_d = own_max == INFINITY ? 0.0f : row.d_of(own_max);
+        const int step = (int)(__float_as_uint(own_d) >> 20) - kFirstStep;
+        if (step < kSteps) atomicAdd(&sh->maxima[max(step, 0)], 1u);
+        row.cl.sync();
+        uint32_t c0 = 0, c1 = 0;
+        for (int r = 0; r < row.ranks; r++) {
+            const uint2 c = reinterpret_cast<const uint2*>(row.cl.map_shared_rank(sh, r)->maxima)[lane];
+            c0 += c.x;
+            c1 += c.y;
         }
-    });
-    mine = warp_sum(mine);
-    if (lane == 0) sh->red_w[warp] = mine;
-    if (cuts) {
-        uint32_t c = 0;
-#pragma unroll
-        for (int i = 0; i < kWindows; i++) {
-            c += (counts >> (8 * i)) & 0xFF;
-            const uint32_t s = __reduce_add_sync(0xffffffffu, c);
-            if (lane == 0) sh->warp_count[warp][i] = s;
-        }
-    }
-    __syncthreads();
-    if (warp == 0) {
-        unsigned long long s = lane < kWarps ? sh->red_w[lane] : 0;
-        s = warp_sum(s);
-        if (lane == 0) sh->kept = s;
-        if (cuts)
-#pragma unroll
-            for (int i = 0; i < kWindows; i++) {
-                const uint32_t c = __reduce_add_sync(0xffffffffu, lane < kWarps ? sh->warp_count[lane][i] : 0);
-                if (lane == 0) sh->count[i] = c;
+        const uint32_t up = warp_scan(c0 + c1);
+        const uint32_t hit = __ballot_sync(0xffffffffu, up >= (uint32_t)k);
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            const int bound = 2 * at + (__shfl_sync(0xffffffffu, up - c1, at) < (uint32_t)k);
+            row.list(0.0f, __uint_as_float((uint32_t)(kFirstStep + bound + 1) << 20), [](float) { return true; });
+            uint32_t offset;
+            const int n = row.listed(&offset);
+            if (n >= 0) {
+                Shared* first = row.cl.map_shared_rank(sh, 0);
+                for (uint32_t i = threadIdx.x; i < sh->n_local; i += kThreads) first->key[offset + i] = sh->local[i];
+                row.cl.sync();
+                if (row.rank == 0) draw_from_list(a, sh, b, n, k, p, m);
+                return;  // nobody reads another CTA's shared memory any more
             }
+            row.cl.sync();  // the others have read this CTA's count
+        }
+        cut = row.select((uint32_t)k, 0.0f, 0);
     }
+    if (p < 1.0f) {
+        __syncthreads();
+        cut = row.select(0, p, cut.weight);
+    }
+
+    // the draw, in the order of the indexes
+    auto kept_weight = [&](float v, int j) -> unsigned long long {
+        if (!kept_by(cut, v, row.begin + j)) return 0;
+        const float e = weight_exp(v);
+        return e >= m ? weight_of(e) : 0;
+    };
+    unsigned long long mine = 0, total = 0, all;
+    if (cut.bin == kBins && m == 0.0f)
+        row.each([&](float v, int) { mine += weight_of(weight_exp(v)); });
+    else
+        row.each([&](float v, int j) { mine += kept_weight(v, j); });
+    unsigned long long before = block_scan(mine, sh->red_w, &all);
+    if (threadIdx.x == 0) sh->kept = all;
     row.cl.sync();
-    unsigned long long total = 0, before = 0;
     for (int r = 0; r < row.ranks; r++) {
         const unsigned long long w = row.cl.map_shared_rank(sh, r)->kept;
         total += w;
         if (r < row.rank) before += w;
     }
-
-    Cut cut = {kBins, 0xFFFFFFFFu, 0x7FFFFFFF, 0};
-    if (cuts) {
-        // the smallest window that holds top-k's cut, the largest that fits for top-p's alone
-        int window = -1;
-        uint32_t n = 0, offset = 0;
-#pragma unroll
-        for (int i = 0; i < kWindows; i++) {
-            uint32_t c = lane < row.ranks ? row.cl.map_shared_rank(sh, lane)->count[i] : 0;
-            const uint32_t up = warp_scan(c), all = __shfl_sync(0xffffffffu, up, 31);
-            if (all <= kList && (k > 0 ? window < 0 && all >= (uint32_t)k : true)) {
-                window = i;
-                n = all;
-                offset = __shfl_sync(0xffffffffu, up - c, row.rank);
-            }
-        }
-        if (window >= 0) {
-            for (int i = 0; i < warp; i++) offset += sh->warp_count[i][window];
-            Shared* first = row.cl.map_shared_rank(sh, 0);
-            const float limit = (float)(1 << window);
-            row.walk([&](float d, int j, bool) {  // d past the slice is infinite
-                const uint32_t hits = __ballot_sync(0xffffffffu, d < limit);
-                if (d < limit)
-                    first->list.key[offset + __popc(hits & ((1u << lane) - 1))] =
-                        (unsigned long long)__float_as_uint(d) << 32 | (uint32_t)(row.begin + j);
-                offset += __popc(hits);
-            });
-            row.cl.sync();
-            bool done = true;
-            if (row.rank == 0) done = draw_from_list(a, sh, b, (int)n, k, p, m, total);
-            if (k > 0) return;  // the list holds the cut
-            if (row.rank == 0 && threadIdx.x == 0) sh->n_keep = done;
-            row.cl.sync();
-            done = row.cl.map_shared_rank(sh, 0)->n_keep != 0;
-            row.cl.sync();
-            if (done) return;
-        }
-        if (k > 0) {
-            cut = row.select((uint32_t)k, 0.0);
-            total = cut.weight;
-        }
-        if (p < 1.0f) {
-            __syncthreads();
-            cut = row.select(0, __dmul_rn((double)p, (double)total));
-        }
-    }
-
-    // the draw, in the order of the indexes
-    auto kept_weight = [&](float v, int j, bool in) -> unsigned long long {
-        if (!in || !kept_by(cut, v, row.begin + j)) return 0;
-        const float e = weight_exp(v);
-        return e >= m ? weight_of(e) : 0;
-    };
-    if (cuts) {
-        mine = 0;
-        row.walk([&](float v, int j, bool in) { mine += kept_weight(v, j, in); });
-        mine = warp_sum(mine);
-        __syncthreads();
-        if (lane == 0) sh->red_w[warp] = mine;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned long long s = 0;
-            for (int i = 0; i < kWarps; i++) s += sh->red_w[i];
-            sh->kept = s;
-        }
-        row.cl.sync();
-        total = before = 0;
-        for (int r = 0; r < row.ranks; r++) {
-            const unsigned long long w = row.cl.map_shared_rank(sh, r)->kept;
-            total += w;
-            if (r < row.rank) before += w;
-        }
-    }
-    for (int i = 0; i < warp; i++) before += sh->red_w[i];
     const unsigned long long pick = pick_of(a.u[b], total);
     if (before <= pick && pick < before + mine)
-        row.walk([&](float v, int j, bool in) {
-            const unsigned long long w = kept_weight(v, j, in), up_to = before + warp_scan(w);
-            if (w && up_to > pick && up_to - w <= pick) {
+        row.each([&](float v, int j) {
+            const unsigned long long w = kept_weight(v, j);
+            if (before <= pick && pick < before + w) {
                 a.tokens[b] = row.begin + j;
                 a.probs[b] = (float)__ddiv_rn((double)w, (double)total);
             }
-            before = __shfl_sync(0xffffffffu, up_to, 31);
+            before += w;
         });
     row.cl.sync();  // no CTA leaves while another reads its shared memory
 }
@@ -694,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
 template <typename T>
 int launch_sample(const SampleArgs& a, int batch, int ranks, cudaStream_t s)
 {
-    const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + ((size_t)a.slice + 3) * sizeof(float);
+    const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + ((size_t)a.slice + 6) * sizeof(float);
     auto fn = sample_kernel<T>;
     TMAC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     TMAC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
@@ -741,7 +789,7 @@ extern "C" int tmac_sample(const void* logits, int type, int64_t row_stride, int
     a.min_p = min_p;
     a.tokens = tokens;
     a.probs = probs;
-    const int ranks = vocab <= 4096 ? 1 : vocab <= 8 * kMaxSlice ? 8 : 16;
+    const char* er = getenv("TS_RANKS"); const int ranks = er ? atoi(er) : vocab <= 4096 ? 1 : vocab <= 8 * kMaxSlice ? 8 : 16;
     a.slice = ((vocab + ranks - 1) / ranks + 7) & ~7;  // every rank's first logit is as aligned as the row's
     DeviceGuard dg(device);
     if (!dg.ok) return fail(TMAC_ERR_NODEV, "no such CUDA device");
