@@ -13,8 +13,11 @@
 // the token is the first kept index whose running weight passes u times the
 // kept weight.
 //
-// One cluster of CTAs per row holds the row's x in shared memory, so the logits
-// are read from HBM once.  Three ways to the cut:
+// A row belongs to one cluster of CTAs.  With few rows eight CTAs hold its x in
+// shared memory, so the logits are read once.  With many rows (more than the SMs
+// hold that way) fewer CTAs read the logits again for each pass, mostly from L2:
+// then every row is in flight at once, instead of waiting for others' clusters.
+// Three ways to the cut:
 //  * top-k: the k-th largest of the threads' own maxima bounds the k-th largest
 //    logit from below, and closely, since a thread holds a few dozen logits.  The
 //    tokens above the bound are gathered in one CTA, sorted, and the draw ends there.
@@ -36,16 +39,20 @@ namespace cg = cooperative_groups;
 namespace tmac {
 namespace {
 
-#ifndef KFLIGHT
-#define KFLIGHT 4
-#endif
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 512;
 constexpr float kBinScale = 22.5f;  // bins per unit of d in the first round; d < 22.2 where w > 0
-constexpr int kMaxCluster = 16, kMaxSlice = 45000;
-constexpr int kList = 2048, kLocal = 512;  // tokens gathered in one CTA, listed by each
-constexpr int kSteps = 64, kFirstStep = (127 - 4) << 3;  // bounds on d, eight to an octave from 1/16 to 16
+constexpr int kCluster = 8, kMaxCluster = 16, kMaxSlice = 45000, kMaxVocab = kMaxCluster * kMaxSlice;
+constexpr int kList = 2048;                                    // tokens gathered in one CTA
+constexpr int kSteps = 64, kFirstStep = (127 - 4) << 3;        // bounds on d, eight to an octave from 1/16 to 16
 static_assert(kThreads >= kBins && kThreads * kMaxCluster / kBins <= 32, "the threads of a bin are lanes of a warp");
 static_assert(kBins / kMaxCluster % 32 == 0, "a share's bins go to the lanes of a warp");
+// Resident rows list up to 512 tokens per CTA and keep their x; others have the room for more.
+template <bool kResident>
+struct Layout {
+    static constexpr int kLocal = kResident ? 512 : kList;
+    static constexpr int kChunkVecs = kResident ? 64 : 256;  // float4 of a chunk of the draw
+    static constexpr int kChunks = ((kResident ? kMaxSlice : kMaxVocab) + 6) / (4 * kChunkVecs) + 1;
+};
 
 struct SampleArgs {
     const void* logits;
@@ -59,23 +66,32 @@ struct SampleArgs {
 };
 
 struct Shared {
-    uint32_t cnt[kBins], hi[kBins], lo[kBins];  // this CTA's histogram: counts, weights in two halves
+    uint32_t cnt[kBins], hi[kBins], lo[kBins];  // this CTA's histogram: counts, weights in two words
     uint32_t mcnt[kBins];                       // this CTA's share of the bins, summed over the cluster
     unsigned long long mw[kBins];
-    unsigned long long key[kList], local[kLocal];  // bits(d) << 32 | index
+    unsigned long long key[kList];  // gathered tokens: bits(d) << 32 | index
     unsigned long long share_w, red_w[kWarps];
     uint32_t share_c, red_c[kWarps];
     float red_f[kWarps], cta_max;
     int cta_min_index;
     alignas(8) uint32_t maxima[kSteps];  // the threads' maxima by their distance from the row's
-    uint32_t n_local;         // listed tokens; more than kLocal: not all of them
-    uint32_t tie_count, n_keep;
+    uint32_t n_local;                    // listed tokens; more than kLocal: not all of them
+    uint32_t n_keep;
     unsigned long long kept, cut_weight, cut_key;
+    int chunk;  // the draw's
+    unsigned long long chunk_before;
     // broadcast of a search
     int found_bin, tie_index;
     uint32_t found_c, before_c;
     unsigned long long found_w, before_w;
 };
+
+constexpr size_t kSharedBytes = (sizeof(Shared) + 15) / 16 * 16;
+template <bool kResident>
+constexpr size_t list_bytes()  // up to where x starts
+{
+    return (kSharedBytes + sizeof(unsigned long long) * (Layout<kResident>::kLocal + Layout<kResident>::kChunks) + 15) / 16 * 16;
+}
 
 TMAC_DEV float weight_exp(float d) { return expf(-d); }
 TMAC_DEV unsigned long long weight_of(float e)
@@ -181,33 +197,84 @@ TMAC_DEV unsigned long long block_scan(unsigned long long v, unsigned long long*
     return before + up - v;
 }
 
+template <typename T, bool kResident>
 struct Row {
+    using L = Layout<kResident>;
     cg::cluster_group cl;
     Shared* sh;
-    float* x;        // this CTA's scaled logits
-    int n, begin;    // their number and first index
-    int pad;         // -inf before x (and after it), so that whole float4 are read
+    unsigned long long *local, *chunks;  // listed tokens; the draw's sums
+    float* x;                            // resident: this CTA's scaled logits
+    const T* l;                          // its logits
+    float inv;
+    int n, begin;  // their number and first index
+    int pad;       // so many before the first make whole vectors of 4; -inf there and behind
     int ranks, rank;
-    float mx;        // the row's largest
+    float mx;      // the row's largest
+    bool infinite; // it is infinite: those share the weight, at d = 0
 
-    TMAC_DEV float d_of(float v) const { return __fsub_rn(mx, v); }
-
-    // Calls f(d, local index) over the thread's own contiguous part, in order.
-    // An odd number each: a warp's accesses fall on different banks.
-    template <typename F>
-    TMAC_DEV void each(F&& f) const
+    TMAC_DEV float scaled(T v) const { return fmaxf(__fmul_rn(Elem<T>::load(&v), inv), -INFINITY); }  // NaN: -inf
+    TMAC_DEV int vectors() const { return (pad + n + 3) / 4; }
+    // Vector i holds the local indexes from 4 i - pad on.  As it lies in memory, for
+    // one that is whole within the slice:
+    using Raw = std::conditional_t<kResident || sizeof(T) == 4, uint4, uint2>;
+    TMAC_DEV Raw raw4(int i) const
     {
-        const int per = ((n + kThreads - 1) / kThreads) | 1;
-        const int from = threadIdx.x * per, to = min(n, from + per);
-        int i = from;
-        for (; i + 4 <= to; i += 4) {
-            const float v0 = x[i], v1 = x[i + 1], v2 = x[i + 2], v3 = x[i + 3];
-            f(d_of(v0), i);
-            f(d_of(v1), i + 1);
-            f(d_of(v2), i + 2);
-            f(d_of(v3), i + 3);
+        if constexpr (kResident)
+            return reinterpret_cast<const uint4*>(x - pad)[i];
+        else
+            return __ldg(reinterpret_cast<const Raw*>(l + 4 * i - pad));
+    }
+    TMAC_DEV float4 from_raw(const Raw& raw) const
+    {
+        if constexpr (kResident) {
+            return *reinterpret_cast<const float4*>(&raw);
+        } else {
+            const T* r = reinterpret_cast<const T*>(&raw);
+            return make_float4(scaled(r[0]), scaled(r[1]), scaled(r[2]), scaled(r[3]));
         }
-        for (; i < to; i++) f(d_of(x[i]), i);
+    }
+    TMAC_DEV float4 load4(int i) const
+    {
+        const int j = 4 * i - pad;
+        if constexpr (!kResident) {
+            if (j < 0 || j + 4 > n) {
+                float e[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) e[c] = j + c >= 0 && j + c < n ? scaled(l[j + c]) : -INFINITY;
+                return make_float4(e[0], e[1], e[2], e[3]);
+            }
+        }
+        return from_raw(raw4(i));
+    }
+    TMAC_DEV float d_of(float v) const
+    {
+        if (infinite) return v == INFINITY ? 0.0f : INFINITY;
+        return __fsub_rn(mx, v);
+    }
+    // Calls f(d of four, local index of the first) for every `stride`-th vector from
+    // `from` to `to`; indexes outside the slice have d = inf.
+    template <typename F>
+    TMAC_DEV void vectors(int from, int to, int stride, F&& f) const
+    {
+        constexpr int kFlight = 4;  // 2 costs 5-10% where rows are read anew, 8 the same in 16 bits
+        const auto use = [&](const float4& q, int i) {
+            const float e[4] = {d_of(q.x), d_of(q.y), d_of(q.z), d_of(q.w)};
+            f(e, 4 * i - pad);
+        };
+        int i = from;
+        if (!kResident && 4 * i < pad && i < to) {  // starts before the slice
+            use(load4(i), i);
+            i += stride;
+        }
+        const int whole = kResident ? to : min(to, (pad + n) / 4);
+        for (; i + (kFlight - 1) * stride < whole; i += kFlight * stride) {  // several loads in flight
+            Raw raw[kFlight];
+#pragma unroll
+            for (int u = 0; u < kFlight; u++) raw[u] = raw4(i + u * stride);
+#pragma unroll
+            for (int u = 0; u < kFlight; u++) use(from_raw(raw[u]), i + u * stride);
+        }
+        for (; i < to; i += stride) use(load4(i), i);
     }
 
     // Lists the tokens with from <= d < to for which `which` holds too, as long as
@@ -217,25 +284,89 @@ struct Row {
     {
         if (threadIdx.x == 0) sh->n_local = 0;
         __syncthreads();
-        const float4* v = reinterpret_cast<const float4*>(x - pad);
-        const int vecs = (pad + n + 3) / 4;
         const volatile uint32_t* listed = &sh->n_local;
-        for (int i = threadIdx.x; i < vecs; i += kThreads) {
-            const float4 q = v[i];
-            const float e[4] = {d_of(q.x), d_of(q.y), d_of(q.z), d_of(q.w)};
+        vectors(threadIdx.x, vectors(), kThreads, [&](const float (&e)[4], int j) {
             bool any = false;
 #pragma unroll
             for (int c = 0; c < 4; c++) any |= e[c] < to && e[c] >= from;
-            if (any && *listed <= kLocal)
+            if (any && *listed <= L::kLocal)
 #pragma unroll
                 for (int c = 0; c < 4; c++)
                     if (e[c] >= from && e[c] < to && which(e[c])) {
                         const uint32_t at = atomicAdd(&sh->n_local, 1u);
-                        if (at < kLocal) sh->local[at] = order_key(e[c], begin + 4 * i + c - pad);
+                        if (at < L::kLocal) local[at] = order_key(e[c], begin + j + c);
                     }
-        }
+        });
         cl.sync();
     }
+
+    // The token at which the running sum of f(d, index), over the cluster in the order
+    // of the indexes, passes pick_of_total(total); the thread that holds it calls
+    // found(index, f of it, total).
+    template <typename F, typename P, typename G>
+    TMAC_DEV void draw(F&& f, P&& pick_of_total, G&& found)
+    {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        const int n_chunks = (vectors() + L::kChunkVecs - 1) / L::kChunkVecs;
+        unsigned long long mine = 0, all, total = 0, before = 0;
+        for (int c = warp; c < n_chunks; c += kWarps) {
+            unsigned long long s = 0;
+            vectors(c * L::kChunkVecs + lane, min(vectors(), (c + 1) * L::kChunkVecs), 32, [&](const float (&e)[4], int j) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) s += f(e[i], begin + j + i);
+            });
+            s = warp_sum(s);
+            if (lane == 0) chunks[c] = s;
+            mine += s;
+        }
+        block_scan(lane == 0 ? mine : 0, sh->red_w, &all);
+        if (threadIdx.x == 0) sh->kept = all;
+        cl.sync();
+        for (int r = 0; r < ranks; r++) {
+            const unsigned long long w = cl.map_shared_rank(sh, r)->kept;
+            total += w;
+            if (r < rank) before += w;
+        }
+        const unsigned long long pick = pick_of_total(total);
+        if (before <= pick && pick < before + all) {  // the whole CTA
+            unsigned long long sum;
+            for (int c0 = 0; c0 < n_chunks; c0 += kThreads) {
+                const int c = c0 + threadIdx.x;
+                const unsigned long long s = c < n_chunks ? chunks[c] : 0, at = before + block_scan(s, sh->red_w, &sum);
+                if (at <= pick && pick < at + s) {
+                    sh->chunk = c;
+                    sh->chunk_before = at;
+                }
+                before += sum;
+            }
+            __syncthreads();
+            const int v = sh->chunk * L::kChunkVecs + threadIdx.x;
+            unsigned long long w[4] = {};
+            if (threadIdx.x < L::kChunkVecs && v < vectors()) {
+                const float4 q = load4(v);
+                const float e[4] = {d_of(q.x), d_of(q.y), d_of(q.z), d_of(q.w)};
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = f(e[i], begin + 4 * v - pad + i);
+            }
+            unsigned long long at = sh->chunk_before + block_scan(w[0] + w[1] + w[2] + w[3], sh->red_w, &sum);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (at <= pick && pick < at + w[i]) found(begin + 4 * v - pad + i, w[i], total);
+                at += w[i];
+            }
+        }
+        cl.sync();  // no CTA goes on while another reads its shared memory
+    }
+    // The index of the m-th element (from 1) with bits(d) == key, over the cluster.
+    TMAC_DEV int tie(uint32_t key, uint32_t m)
+    {
+        draw([&](float v, int) -> unsigned long long { return __float_as_uint(v) == key; }, [&](unsigned long long) { return m - 1; },
+             [&](int index, unsigned long long, unsigned long long) {
+                 for (int r = 0; r < ranks; r++) cl.map_shared_rank(sh, r)->tie_index = index;
+             });
+        return sh->tie_index;
+    }
+
     // The number of the cluster's listed tokens, or -1 if they do not fit in one CTA;
     // this rank's come after `offset`.
     TMAC_DEV int listed(uint32_t* offset) const
@@ -244,16 +375,16 @@ struct Row {
         const uint32_t c = lane < ranks ? cl.map_shared_rank(sh, lane)->n_local : 0, up = warp_scan(c);
         const uint32_t all = __shfl_sync(0xffffffffu, up, 31);
         *offset = __shfl_sync(0xffffffffu, up - c, rank);
-        return __any_sync(0xffffffffu, c > kLocal) || all > kList ? -1 : (int)all;
+        return __any_sync(0xffffffffu, c > (uint32_t)L::kLocal) || all > kList ? -1 : (int)all;
     }
     // Copies every rank's listed tokens into this CTA's keys.
     TMAC_DEV void gather() const
     {
         uint32_t at = 0;
         for (int r = 0; r < ranks; r++) {
-            const Shared* o = cl.map_shared_rank(sh, r);
-            const uint32_t c = o->n_local;
-            for (uint32_t i = threadIdx.x; i < c; i += kThreads) sh->key[at + i] = o->local[i];
+            const uint32_t c = cl.map_shared_rank(sh, r)->n_local;
+            const unsigned long long* from = cl.map_shared_rank(local, r);
+            for (uint32_t i = threadIdx.x; i < c; i += kThreads) sh->key[at + i] = from[i];
             at += c;
         }
         __syncthreads();
@@ -265,15 +396,17 @@ struct Row {
     {
         for (int i = threadIdx.x; i < kBins; i += kThreads) sh->cnt[i] = sh->hi[i] = sh->lo[i] = 0;
         __syncthreads();
-        each([&](float v, int) {
-            const int b = bin_of(v);
-            if (b < 0) return;
-            const unsigned long long w = weight_of(weight_exp(v));
-            if (!w) return;
-            // a slice has at most kMaxSlice elements of at most 2^16 in either half: no overflow
-            if (kCounts) atomicAdd(&sh->cnt[b], 1u);
-            atomicAdd(&sh->hi[b], (uint32_t)(w >> 16));
-            atomicAdd(&sh->lo[b], (uint32_t)(w & 0xFFFF));
+        vectors(threadIdx.x, vectors(), kThreads, [&](const float (&e)[4], int) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int b = bin_of(e[i]);
+                if (b < 0) continue;
+                const unsigned long long w = weight_of(weight_exp(e[i]));
+                if (!w) continue;
+                if (kCounts) atomicAdd(&sh->cnt[b], 1u);
+                const uint32_t low = (uint32_t)w, carry = atomicAdd(&sh->lo[b], low) > 0xFFFFFFFFu - low;
+                if (carry + (w >> 32)) atomicAdd(&sh->hi[b], carry + (uint32_t)(w >> 32));
+            }
         });
         cl.sync();
         // this rank's share of the bins, over all ranks: `each` threads to a bin
@@ -284,7 +417,7 @@ struct Row {
         for (int r = part; r < ranks; r += each) {
             const Shared* o = cl.map_shared_rank(sh, r);
             c_sum += o->cnt[rank * share + bin];
-            w_sum += ((unsigned long long)o->hi[rank * share + bin] << 16) + o->lo[rank * share + bin];
+            w_sum += ((unsigned long long)o->hi[rank * share + bin] << 32) + o->lo[rank * share + bin];
         }
         for (int o = each / 2; o > 0; o >>= 1) {
             c_sum += __shfl_xor_sync(0xffffffffu, c_sum, o);
@@ -369,25 +502,6 @@ struct Row {
         }
         __syncthreads();
         return sh->found_bin >= 0;
-    }
-
-    // The index of the m-th element (from 1) with bits(d) == key, over the cluster.
-    TMAC_DEV int tie(uint32_t key, uint32_t m)
-    {
-        uint32_t c = 0;
-        each([&](float v, int) { c += __float_as_uint(v) == key; });
-        unsigned long long all;
-        uint32_t before = (uint32_t)block_scan(c, sh->red_w, &all);
-        if (threadIdx.x == 0) sh->tie_count = (uint32_t)all;
-        cl.sync();
-        for (int r = 0; r < rank; r++) before += cl.map_shared_rank(sh, r)->tie_count;
-        if (before < m && m <= before + c)
-            each([&](float v, int j) {
-                if (__float_as_uint(v) == key && ++before == m)
-                    for (int r = 0; r < ranks; r++) cl.map_shared_rank(sh, r)->tie_index = begin + j;
-            });
-        cl.sync();
-        return sh->tie_index;
     }
 
     // Cuts the order after its first k elements (k > 0), or after the element at which
@@ -546,17 +660,17 @@ TMAC_DEV void draw_from_list(const SampleArgs& a, Shared* sh, int b, int n, int 
 }
 
 // l * inv of the CTA's n logits into x, NaN as -inf, and `pad` (and up to 3 more
-// behind) -inf around them; the largest of the thread's.  x + head is 16-byte aligned.
+// behind) -inf around them; the largest of the thread's.
 template <typename T>
-TMAC_DEV float load_scaled(const T* l, int n, int head, float inv, float* x, int pad)
+TMAC_DEV float load_scaled(const T* l, int n, float inv, float* x, int pad)
 {
     float mx = -INFINITY;
     auto put = [&](int i) {
         x[i] = fmaxf(__fmul_rn(Elem<T>::load(l + i), inv), -INFINITY);  // fmaxf leaves a NaN out
         mx = fmaxf(mx, x[i]);
     };
-    constexpr int kVec = 16 / sizeof(T), kFlight = KFLIGHT;
-    head = min(n, head);
+    constexpr int kVec = 16 / sizeof(T), kFlight = 4;
+    const int head = min(n, (int)((16 - (uintptr_t)l % 16) % 16 / sizeof(T)));
     const int vecs = (n - head) / kVec, tail = head + vecs * kVec;
     if ((int)threadIdx.x < head) put(threadIdx.x);
     if ((int)threadIdx.x < n - tail) put(tail + threadIdx.x);
@@ -588,28 +702,30 @@ TMAC_DEV float load_scaled(const T* l, int n, int head, float inv, float* x, int
     return mx;
 }
 
-template <typename T>
+template <typename T, bool kResident>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
 {
     extern __shared__ __align__(16) uint8_t smem[];
-    Row row = {cg::this_cluster()};
-    row.sh = reinterpret_cast<Shared*>(smem);
+    using R = Row<T, kResident>;
+    R row = {cg::this_cluster()};
+    Shared* sh = row.sh = reinterpret_cast<Shared*>(smem);
+    row.local = reinterpret_cast<unsigned long long*>(smem + kSharedBytes);
+    row.chunks = row.local + R::L::kLocal;
     row.ranks = (int)row.cl.num_blocks();
     row.rank = (int)row.cl.block_rank();
-    Shared* sh = row.sh;
     const int b = blockIdx.x / row.ranks, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     row.begin = row.rank * a.slice;
     row.n = max(0, min(a.slice, a.vocab - row.begin));
-    const T* l = (const T*)a.logits + b * a.stride + row.begin;
-    // the first logit on a 16-byte boundary goes to one of shared memory
-    const int head = (int)((16 - (uintptr_t)l % 16) % 16 / sizeof(T));
-    row.pad = (4 - head % 4) % 4;
-    row.x = reinterpret_cast<float*>(smem + (sizeof(Shared) + 15) / 16 * 16) + row.pad;
+    row.l = (const T*)a.logits + b * a.stride + row.begin;
+    // vectors of 4 logits start on a multiple of their size; so do those of x
+    row.pad = (int)((uintptr_t)row.l % (4 * sizeof(T)) / sizeof(T));
+    row.x = reinterpret_cast<float*>(smem + list_bytes<kResident>()) + row.pad;
+    row.infinite = false;
 
     const float temperature = a.temperature ? a.temperature[b] : 1.0f;
-    float inv = __frcp_rn(temperature);
+    const float inv = __frcp_rn(temperature);
     const bool greedy = !(temperature > 0.0f) || isinf(inv);
-    if (greedy) inv = 1.0f;
+    row.inv = greedy ? 1.0f : inv;
     int k = a.top_k ? a.top_k[b] : 0;
     if (k < 0 || k >= a.vocab) k = 0;
     float p = a.top_p ? a.top_p[b] : 1.0f;
@@ -621,7 +737,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     m = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
 
     // scaled logits, and the largest of the row
-    const float own_max = load_scaled<T>(l, row.n, head, inv, row.x, row.pad);
+    float own_max = -INFINITY;
+    if (kResident) {
+        own_max = load_scaled<T>(row.l, row.n, row.inv, row.x, row.pad);
+    } else {
+        row.mx = 0.0f;
+        row.vectors(threadIdx.x, row.vectors(), kThreads, [&](const float (&e)[4], int) {  // here -x
+            own_max = fmaxf(own_max, -fminf(fminf(e[0], e[1]), fminf(e[2], e[3])));
+        });
+    }
     float mx = own_max;
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (lane == 0) sh->red_f[warp] = mx;
@@ -635,11 +759,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     mx = lane < row.ranks ? row.cl.map_shared_rank(sh, lane)->cta_max : -INFINITY;
     for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     mx = row.mx = __fadd_rn(__shfl_sync(0xffffffffu, mx, 0), 0.0f);  // -0 as 0: no d is -0
-    if (mx == INFINITY) {  // the infinite ones share the weight, at d = 0
-        for (int i = threadIdx.x; i < row.n; i += kThreads) row.x[i] = row.x[i] == INFINITY ? 0.0f : -INFINITY;
-        mx = row.mx = 0.0f;
-        __syncthreads();
-    }
+    row.infinite = mx == INFINITY;
     if (mx == -INFINITY) {  // nothing to choose from
         row.cl.sync();
         if (row.rank == 0 && threadIdx.x == 0) {
@@ -651,8 +771,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
 
     if (greedy || k == 1) {  // the lowest index of the largest
         int first = 0x7FFFFFFF;
-        for (int i = threadIdx.x; i < row.n; i += kThreads)
-            if (row.x[i] == mx) first = min(first, row.begin + i);
+        row.vectors(threadIdx.x, row.vectors(), kThreads, [&](const float (&e)[4], int j) {
+#pragma unroll
+            for (int c = 3; c >= 0; c--)
+                if (e[c] == 0.0f) first = min(first, row.begin + j + c);
+        });
         first = __reduce_min_sync(0xffffffffu, first);
         if (lane == 0) sh->red_c[warp] = (uint32_t)first;
         __syncthreads();
@@ -673,8 +796,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     Cut cut;
     if (k > 0) {
         // the least bound on d below which k threads have their maximum
-        const float own_d = own_max == INFINITY ? 0.0f : row.d_of(own_max);
-        const int step = (int)(__float_as_uint(own_d) >> 20) - kFirstStep;
+        const int step = (int)(__float_as_uint(row.d_of(own_max)) >> 20) - kFirstStep;
         if (step < kSteps) atomicAdd(&sh->maxima[max(step, 0)], 1u);
         row.cl.sync();
         uint32_t c0 = 0, c1 = 0;
@@ -693,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
             const int n = row.listed(&offset);
             if (n >= 0) {
                 Shared* first = row.cl.map_shared_rank(sh, 0);
-                for (uint32_t i = threadIdx.x; i < sh->n_local; i += kThreads) first->key[offset + i] = sh->local[i];
+                for (uint32_t i = threadIdx.x; i < sh->n_local; i += kThreads) first->key[offset + i] = row.local[i];
                 row.cl.sync();
                 if (row.rank == 0) draw_from_list(a, sh, b, n, k, p, m);
                 return;  // nobody reads another CTA's shared memory any more
@@ -708,42 +830,28 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     }
 
     // the draw, in the order of the indexes
-    auto kept_weight = [&](float v, int j) -> unsigned long long {
-        if (!kept_by(cut, v, row.begin + j)) return 0;
-        const float e = weight_exp(v);
-        return e >= m ? weight_of(e) : 0;
+    const auto pick = [&](unsigned long long total) { return pick_of(a.u[b], total); };
+    const auto found = [&](int index, unsigned long long w, unsigned long long total) {
+        a.tokens[b] = index;
+        a.probs[b] = (float)__ddiv_rn((double)w, (double)total);
     };
-    unsigned long long mine = 0, total = 0, all;
     if (cut.bin == kBins && m == 0.0f)
-        row.each([&](float v, int) { mine += weight_of(weight_exp(v)); });
+        row.draw([](float d, int) { return weight_of(weight_exp(d)); }, pick, found);
     else
-        row.each([&](float v, int j) { mine += kept_weight(v, j); });
-    unsigned long long before = block_scan(mine, sh->red_w, &all);
-    if (threadIdx.x == 0) sh->kept = all;
-    row.cl.sync();
-    for (int r = 0; r < row.ranks; r++) {
-        const unsigned long long w = row.cl.map_shared_rank(sh, r)->kept;
-        total += w;
-        if (r < row.rank) before += w;
-    }
-    const unsigned long long pick = pick_of(a.u[b], total);
-    if (before <= pick && pick < before + mine)
-        row.each([&](float v, int j) {
-            const unsigned long long w = kept_weight(v, j);
-            if (before <= pick && pick < before + w) {
-                a.tokens[b] = row.begin + j;
-                a.probs[b] = (float)__ddiv_rn((double)w, (double)total);
-            }
-            before += w;
-        });
-    row.cl.sync();  // no CTA leaves while another reads its shared memory
+        row.draw(
+            [&](float d, int index) -> unsigned long long {
+                if (!kept_by(cut, d, index)) return 0;
+                const float e = weight_exp(d);
+                return e >= m ? weight_of(e) : 0;
+            },
+            pick, found);
 }
 
-template <typename T>
+template <typename T, bool kResident>
 int launch_sample(const SampleArgs& a, int batch, int ranks, cudaStream_t s)
 {
-    const size_t smem = (sizeof(Shared) + 15) / 16 * 16 + ((size_t)a.slice + 6) * sizeof(float);
-    auto fn = sample_kernel<T>;
+    const size_t smem = list_bytes<kResident>() + (kResident ? ((size_t)a.slice + 6) * sizeof(float) : 0);
+    auto fn = sample_kernel<T, kResident>;
     TMAC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     TMAC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
@@ -773,7 +881,7 @@ extern "C" int tmac_sample(const void* logits, int type, int64_t row_stride, int
     const int bytes = type_bytes(type);
     if (!bytes) return fail(TMAC_ERR_TYPE, "logits must be F32, F16 or BF16");
     if (batch < 0 || batch > 0x7FFFFFF) return fail(TMAC_ERR_SHAPE, "batch out of range");
-    if (vocab <= 0 || vocab > kMaxCluster * kMaxSlice) return fail(TMAC_ERR_SHAPE, "vocab must be 1 to 720000");
+    if (vocab <= 0 || vocab > kMaxVocab) return fail(TMAC_ERR_SHAPE, "vocab must be 1 to 720000");
     if (batch > 1 && row_stride < vocab) return fail(TMAC_ERR_SHAPE, "row_stride must cover a row");
     if (batch == 0) return TMAC_OK;
     if (!logits || !u || !tokens || !probs) return fail(TMAC_ERR_INVALID, "NULL argument");
@@ -789,11 +897,19 @@ extern "C" int tmac_sample(const void* logits, int type, int64_t row_stride, int
     a.min_p = min_p;
     a.tokens = tokens;
     a.probs = probs;
-    const char* er = getenv("TS_RANKS"); const int ranks = er ? atoi(er) : vocab <= 4096 ? 1 : vocab <= 8 * kMaxSlice ? 8 : 16;
+    // Up to two CTAs per SM hold their rows; more rows than that are read anew for
+    // each pass by as few CTAs as fill the SMs twice.  Top-k 40 of 151936 logits, held
+    // against read anew: 21.7 / 25.0 us for 32 rows, 36.2 / 23.5 for 64, 126 / 62 for 256.
+    const int room = 2 * num_sms(device);
+    int ranks = vocab <= 4096 ? 1 : vocab <= kCluster * kMaxSlice ? kCluster : kMaxCluster;
+    const bool resident = (int64_t)batch * ranks <= room;
+    while (!resident && ranks > 1 && (int64_t)batch * ranks > room) ranks /= 2;
     a.slice = ((vocab + ranks - 1) / ranks + 7) & ~7;  // every rank's first logit is as aligned as the row's
     DeviceGuard dg(device);
     if (!dg.ok) return fail(TMAC_ERR_NODEV, "no such CUDA device");
     return with_type(type, [&](auto* t) {
-        return launch_sample<std::remove_pointer_t<decltype(t)>>(a, batch, ranks, (cudaStream_t)stream);
+        using T = std::remove_pointer_t<decltype(t)>;
+        return resident ? launch_sample<T, true>(a, batch, ranks, (cudaStream_t)stream)
+                        : launch_sample<T, false>(a, batch, ranks, (cudaStream_t)stream);
     });
 }
