@@ -9,8 +9,13 @@
 // The prefix's keys are read once for all sequences: its scores are one matrix
 // product of all tokens' query rows, the own part one product per sequence.
 // Both run as jobs of one grid, each a tile of rows (token, head of a key/value
-// head's group) against a range of keys with a running maximum and sum; a job
-// leaves (maximum, sum, unnormalised o), and attn_join_kernel joins a row's jobs.
+// head's group) against a range of 64-key tiles with a running maximum and sum; a
+// job leaves (maximum, sum, unnormalised o), and attn_join_kernel joins a row's
+// jobs.  Where that is less work than a second launch, every sequence reads the
+// prefix itself, and one job holds all of a row's keys and writes its result.
+//
+// Two kernels share this frame: 32-bit elements on the FMA units, 16-bit ones on
+// mma.sync.  Tiles come through cp.async, several in flight.
 #include "serving.cuh"
 
 #include <algorithm>
@@ -31,11 +36,13 @@ struct AttnArgs {
     const int *tables, *own_lens;
     int table_width, max_own;
     float scale;
-    // jobs: prefix tiles x key ranges x kv heads, then (sequence, tile) x key ranges x kv heads
-    int p_tiles, p_splits, p_chunk;
-    int o_tiles, o_splits, o_chunk;
+    // Jobs: prefix row tiles x kv heads x key ranges, then (sequence, row tile) x kv
+    // heads x key ranges.  Key ranges are counted in tiles of kTile keys.
+    bool alone;      // no prefix jobs: each sequence's keys are the prefix's and its own
+    int p_tiles, p_splits, p_range;
+    int o_tiles, o_splits, o_range;
     int64_t p_jobs;
-    int parts;       // per row: p_splits + o_splits
+    int parts;       // per row: p_splits + o_splits; 1: jobs write the result
     float* part_o;   // [tokens][heads][parts][dim]
     float2* part_ml; // [tokens][heads][parts]
     int* err;
@@ -80,33 +87,20 @@ TMAC_DEV int sequence_of(const AttnArgs& a, int token)
     return lo;
 }
 
-// ---------------------------------------------------- 32-bit arithmetic ----
-// Tiles of 8 rows per warp.  A warp takes 16 keys at a time: lane = (key, half
-// of the rows) for the scores, lane = dims for the output.  With up to 8 rows
-// in the job the four warps take different keys of a 64-key tile and join at
-// the end; with more they take different rows and share the tile.
-constexpr int kRows = 8, kTile = 64, kStep = 16, kSimtWarps = 4;
-
-template <typename T, int D>
-struct SimtSmem {
-    float q[kSimtWarps * kRows][D];
-    float p[kSimtWarps][kStep][kRows];
-    float alpha[kSimtWarps][kRows];
-    T k[kTile][D + 16 / sizeof(T)];
-    T v[kTile][D];
-    int limit[kSimtWarps * kRows], least_limit;
-    int token[kSimtWarps * kRows], head[kSimtWarps * kRows];
-};
+// Up to so many key tiles (prefix and own) every sequence reads the prefix itself, in one job.
+constexpr int kAloneTiles = 8;
+constexpr int kTile = 64, kWarps = 4, kThreads = kWarps * 32;
 
 // A job's rows and keys, the same for every kernel.
 struct Job {
-    int kvh, seq;             // seq < 0: prefix
-    int row0, rows;           // of the sequence's (or all) tokens x group
-    int key0, key1;           // key range
+    int kvh, seq;          // seq < 0: rows of all sequences, the prefix's keys
+    int row0, rows, token0;
+    int tile0, tile1;      // key tiles: first those of the prefix, then the own ones
+    int p_tiles;           // of the prefix within them
+    int p_keys, o_keys;    // keys in reach of the job
     int part;
-    const int* pages;
-    int token0;
 };
+TMAC_DEV int tiles_of(int keys) { return (keys + kTile - 1) / kTile; }
 template <int kJobRows>
 TMAC_DEV bool find_job(const AttnArgs& a, Job* j)
 {
@@ -115,15 +109,16 @@ TMAC_DEV bool find_job(const AttnArgs& a, Job* j)
         const int tile = (int)(id % a.p_tiles);
         id /= a.p_tiles;
         j->kvh = (int)(id % a.cache.kv_heads);
-        const int split = (int)(id / a.cache.kv_heads);
+        j->part = (int)(id / a.cache.kv_heads);
         j->seq = -1;
+        j->token0 = 0;
         j->row0 = tile * kJobRows;
         j->rows = min(kJobRows, a.tokens * a.group - j->row0);
-        j->key0 = split * a.p_chunk;
-        j->key1 = min(a.prefix_len, j->key0 + a.p_chunk);
-        j->part = split;
-        j->pages = a.prefix_pages;
-        j->token0 = 0;
+        j->p_keys = a.prefix_len;
+        j->o_keys = 0;
+        j->p_tiles = tiles_of(j->p_keys);
+        j->tile0 = j->part * a.p_range;
+        j->tile1 = min(j->p_tiles, j->tile0 + a.p_range);
         return true;
     }
     id -= a.p_jobs;
@@ -133,63 +128,178 @@ TMAC_DEV bool find_job(const AttnArgs& a, Job* j)
     id /= a.cache.kv_heads;
     const int split = (int)(id % a.o_splits);
     j->seq = (int)(id / a.o_splits);
+    j->part = a.p_splits + split;
+    j->token0 = first_token(a, j->seq);
     j->row0 = tile * kJobRows;
     j->rows = min(kJobRows, token_count(a, j->seq) * a.group - j->row0);
-    j->key0 = split * a.o_chunk;
-    j->key1 = min(own_len(a, j->seq), j->key0 + a.o_chunk);
-    j->part = a.p_splits + split;
-    j->pages = a.tables + (int64_t)j->seq * a.table_width;
-    j->token0 = first_token(a, j->seq);
-    return j->rows > 0 && j->key1 > j->key0;  // the join leaves other parts out
+    j->p_keys = a.alone ? prefix_seen(a, j->seq) : 0;
+    j->o_keys = a.max_own ? own_len(a, j->seq) : 0;
+    j->p_tiles = tiles_of(j->p_keys);
+    j->tile0 = split * a.o_range;
+    j->tile1 = min(j->p_tiles + tiles_of(j->o_keys), j->tile0 + a.o_range);
+    // without keys: the join leaves other parts out, but a lone part is the result
+    return j->rows > 0 && (j->tile1 > j->tile0 || a.parts == 1);
 }
-// The row's token and head, and how many keys of the job's kind it sees.
-TMAC_DEV void find_row(const AttnArgs& a, const Job& j, int r, int* token, int* head, int* limit)
+// The row's token and head, and how many keys of the prefix and of its own it sees.
+struct RowOf {
+    int token, head, p_limit, o_limit;
+};
+TMAC_DEV RowOf find_row(const AttnArgs& a, const Job& j, int r)
 {
     const int row = j.row0 + r, i = row / a.group;
-    *token = j.token0 + i;
-    *head = j.kvh * a.group + row % a.group;
-    *limit = j.seq < 0 ? prefix_seen(a, sequence_of(a, *token)) : own_len(a, j.seq) - token_count(a, j.seq) + 1 + i;
-}
-// First element of key `key`'s row in a pool; -1 for a page outside the pool
-// (its rows count as zeros, and the error word says so).
-TMAC_DEV int64_t key_row(const AttnArgs& a, const Job& j, int key)
-{
-    const int shift = a.cache.page_shift;
-    const int64_t page = j.pages[key >> shift];
-    if (page < 0 || page >= a.cache.n_pages) {
-        record_error(a.err, TMAC_ERR_BOUNDS);
-        return -1;
+    RowOf o;
+    o.token = j.token0 + i;
+    o.head = j.kvh * a.group + row % a.group;
+    if (j.seq < 0) {
+        o.p_limit = a.prefix_lens ? prefix_seen(a, sequence_of(a, o.token)) : a.prefix_len;
+        o.o_limit = 0;
+    } else {
+        o.p_limit = j.p_keys;
+        o.o_limit = max(0, j.o_keys - token_count(a, j.seq) + 1 + i);
     }
-    return (((page * a.cache.kv_heads + j.kvh) << shift) + (key & ((1 << shift) - 1))) * a.cache.dim;
+    return o;
+}
+// Rows of a job as the kernels keep them in shared memory.
+template <int kJobRows>
+struct Rows {
+    int token[kJobRows], head[kJobRows], p_limit[kJobRows], o_limit[kJobRows];
+    int p_least, o_least;  // smallest limits: tiles below them need no mask
+    TMAC_DEV void find(const AttnArgs& a, const Job& j)
+    {
+        if (threadIdx.x == 0) p_least = o_least = 0x7FFFFFFF;
+        __syncthreads();
+        for (int r = threadIdx.x; r < kJobRows; r += blockDim.x) {
+            RowOf o = {0, 0, 0, 0};
+            if (r < j.rows) {
+                o = find_row(a, j, r);
+                atomicMin(&p_least, o.p_limit);
+                atomicMin(&o_least, o.o_limit);
+            }
+            token[r] = o.token;
+            head[r] = o.head;
+            p_limit[r] = o.p_limit;
+            o_limit[r] = o.o_limit;
+        }
+        __syncthreads();
+    }
+};
+// Where tile t's keys lie: the page list, the first key's number in it, the keys in reach.
+struct TileOf {
+    const int* pages;
+    int key0, keys;
+    bool prefix;
+};
+TMAC_DEV TileOf find_tile(const AttnArgs& a, const Job& j, int t)
+{
+    TileOf o;
+    o.prefix = t < j.p_tiles;
+    o.pages = o.prefix ? a.prefix_pages : a.tables + (int64_t)j.seq * a.table_width;
+    o.key0 = (o.prefix ? t : t - j.p_tiles) * kTile;
+    o.keys = o.prefix ? j.p_keys : j.o_keys;
+    return o;
+}
+TMAC_DEV void cp_async16(void* dst, const void* src, bool valid)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+TMAC_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+TMAC_DEV void cp_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+// Starts the copies of tile t's keys and values; k_at(key, value) and v_at say where
+// 16 bytes from that value on go.  Keys out of reach, and rows of a page outside
+// the pool (the error word says so), become zeros.
+template <typename T, int D, typename FK, typename FV>
+TMAC_DEV void copy_tile(const AttnArgs& a, const Job& j, int t, FK&& k_at, FV&& v_at)
+{
+    constexpr int kVec = 16 / sizeof(T), kPer = D / kVec, kCopies = kTile * kPer / kThreads;
+    const TileOf tile = find_tile(a, j, t);
+    const int shift = a.cache.page_shift;
+#pragma unroll
+    for (int i = 0; i < kCopies; i++) {
+        const int at = threadIdx.x + i * kThreads, key = at / kPer, c = at % kPer * kVec;
+        const int g = tile.key0 + key;
+        bool valid = g < tile.keys;
+        const int64_t page = valid ? tile.pages[g >> shift] : 0;
+        if (page < 0 || page >= a.cache.n_pages) {
+            record_error(a.err, TMAC_ERR_BOUNDS);
+            valid = false;
+        }
+        const int64_t from = valid ? (((page * a.cache.kv_heads + j.kvh) << shift) + (g & ((1 << shift) - 1))) * D + c : 0;
+        cp_async16(k_at(key, c), (const T*)a.cache.k + from, valid);
+        cp_async16(v_at(key, c), (const T*)a.cache.v + from, valid);
+    }
+}
+// Row r's result, value d: the part's, or the rounded quotient when there is no other.
+template <typename T, int D>
+TMAC_DEV void put_result(const AttnArgs& a, const Job& j, int token, int head, int d, float m, float l, float o)
+{
+    if (a.parts == 1) {
+        Elem<T>::store((T*)a.out + token * a.out_stride + head * D + d, l == 0.0f ? 0.0f : __fdiv_rn(o, l));
+        return;
+    }
+    const int64_t at = ((int64_t)token * a.heads + head) * a.parts + j.part;
+    a.part_o[at * D + d] = o;
+    if (d == 0) a.part_ml[at] = make_float2(m, l);
+}
+// Maxima are in units of the exponential's base: e in 32 bits, where the difference
+// of two scores is formed before it is scaled; 2 in 16 bits, one multiplication less.
+TMAC_DEV float exp2_fast(float x)  // within 2^-22 relatively, tiny ones as 0
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <typename T>
+TMAC_DEV float power(float x)
+{
+    return sizeof(T) == 4 ? expf(x) : exp2_fast(x);
 }
 
+// ---------------------------------------------------- 32-bit arithmetic ----
+// Tiles of 8 rows per warp.  A warp takes 16 keys at a time: lane = (key, half
+// of the rows) for the scores, lane = dims for the output.  With up to 8 rows
+// in the job the four warps take different keys of a tile and join at the end;
+// with more they take different rows and share the tile.
+constexpr int kRows = 8, kStep = 16, kSimtStages = 2;
+
+template <int D>
+struct SimtSmem {
+    float q[kWarps * kRows][D];
+    float p[kWarps][kStep][kRows];
+    float alpha[kWarps][kRows];
+    float ml[kWarps][kRows][2];
+    struct {
+        float k[kTile][D + 4];
+        float v[kTile][D];
+    } stage[kSimtStages];
+    Rows<kWarps * kRows> rows;
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kSimtWarps * 32) attn_simt_kernel(AttnArgs a)
+__global__ void __launch_bounds__(kThreads) attn_simt_kernel(AttnArgs a)
 {
     extern __shared__ __align__(16) uint8_t smem[];
-    SimtSmem<T, D>& sh = *reinterpret_cast<SimtSmem<T, D>*>(smem);
-    constexpr int kJobRows = kSimtWarps * kRows, kDims = D / 32, kVec = 16 / sizeof(T);
+    SimtSmem<D>& sh = *reinterpret_cast<SimtSmem<D>*>(smem);
+    constexpr int kJobRows = kWarps * kRows, kDims = D / 32;
     Job j;
     if (!find_job<kJobRows>(a, &j)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool split_keys = j.rows <= kRows;
-    if (threadIdx.x == 0) sh.least_limit = 0x7FFFFFFF;
-    __syncthreads();
-    for (int r = threadIdx.x; r < kJobRows; r += blockDim.x) {
-        int token = 0, head = 0, limit = 0;
-        if (r < j.rows) {
-            find_row(a, j, r, &token, &head, &limit);
-            atomicMin(&sh.least_limit, limit);
+    const auto start = [&](int t) {
+        if (t < j.tile1) {
+            auto& st = sh.stage[(t - j.tile0) % kSimtStages];
+            copy_tile<T, D>(a, j, t, [&](int key, int c) { return &st.k[key][c]; }, [&](int key, int c) { return &st.v[key][c]; });
         }
-        sh.token[r] = token;
-        sh.head[r] = head;
-        sh.limit[r] = limit;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kJobRows * D; i += blockDim.x) {
+        cp_async_commit();
+    };
+    start(j.tile0);
+    sh.rows.find(a, j);
+    for (int i = threadIdx.x; i < kJobRows * D; i += kThreads) {
         const int r = i / D, d = i % D;
-        sh.q[r][d] = r < j.rows ? __fmul_rn(a.scale, Elem<T>::load((const T*)a.q + sh.token[r] * a.q_stride + sh.head[r] * D + d))
-                                : 0.0f;
+        sh.q[r][d] = r < j.rows ? __fmul_rn(a.scale, ((const T*)a.q)[sh.rows.token[r] * a.q_stride + sh.rows.head[r] * D + d]) : 0.0f;
     }
 
     const int r0 = split_keys ? 0 : warp * kRows;  // the warp's rows
@@ -202,47 +312,35 @@ __global__ void __launch_bounds__(kSimtWarps * 32) attn_simt_kernel(AttnArgs a)
 #pragma unroll
         for (int c = 0; c < kDims; c++) o[r][c] = 0.0f;
 
-    for (int tile = j.key0; tile < j.key1; tile += kTile) {
+    for (int t = j.tile0; t < j.tile1; t++) {
+        start(t + 1);
+        cp_async_wait<1>();
         __syncthreads();
-        for (int i = threadIdx.x; i < kTile * (D / kVec); i += blockDim.x) {
-            const int key = i / (D / kVec), c = i % (D / kVec) * kVec;
-            uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-            if (tile + key < j.key1) {
-                const int64_t at = key_row(a, j, tile + key);
-                if (at >= 0) {
-                    kx = *reinterpret_cast<const uint4*>((const T*)a.cache.k + at + c);
-                    vx = *reinterpret_cast<const uint4*>((const T*)a.cache.v + at + c);
-                }
-            }
-            *reinterpret_cast<uint4*>(&sh.k[key][c]) = kx;
-            *reinterpret_cast<uint4*>(&sh.v[key][c]) = vx;
-        }
-        __syncthreads();
+        auto& st = sh.stage[(t - j.tile0) % kSimtStages];
+        const TileOf tile = find_tile(a, j, t);
+        const int* limits = tile.prefix ? sh.rows.p_limit : sh.rows.o_limit;
+        const int least = tile.prefix ? sh.rows.p_least : sh.rows.o_least;
         for (int step = split_keys ? warp * kStep : 0; step < (split_keys ? (warp + 1) * kStep : kTile); step += kStep) {
-            if (tile + step >= j.key1) break;
-            const int kk = step + (lane & 15), key = tile + kk;
+            if (tile.key0 + step >= tile.keys || r0 >= j.rows) break;
+            const int kk = step + (lane & 15), key = tile.key0 + kk;
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-            for (int d = 0; d < D; d += kVec) {
-                T kx[kVec];
-                *reinterpret_cast<uint4*>(kx) = *reinterpret_cast<const uint4*>(&sh.k[kk][d]);
+            for (int d = 0; d < D; d += 4) {
+                const float4 kx = *reinterpret_cast<const float4*>(&st.k[kk][d]);
 #pragma unroll
-                for (int e = 0; e < kVec; e += 4) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float4 qv = *reinterpret_cast<const float4*>(&sh.q[r0 + half * 4 + i][d + e]);
-                        s[i] = __fmaf_rn(qv.x, Elem<T>::load(kx + e), s[i]);
-                        s[i] = __fmaf_rn(qv.y, Elem<T>::load(kx + e + 1), s[i]);
-                        s[i] = __fmaf_rn(qv.z, Elem<T>::load(kx + e + 2), s[i]);
-                        s[i] = __fmaf_rn(qv.w, Elem<T>::load(kx + e + 3), s[i]);
-                    }
+                for (int i = 0; i < 4; i++) {
+                    const float4 qv = *reinterpret_cast<const float4*>(&sh.q[r0 + half * 4 + i][d]);
+                    s[i] = __fmaf_rn(qv.x, kx.x, s[i]);
+                    s[i] = __fmaf_rn(qv.y, kx.y, s[i]);
+                    s[i] = __fmaf_rn(qv.z, kx.z, s[i]);
+                    s[i] = __fmaf_rn(qv.w, kx.w, s[i]);
                 }
             }
             float p[4], al[4];
             bool moved = false;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (key >= j.key1 || key >= sh.limit[r0 + half * 4 + i]) s[i] = -INFINITY;
+                if (key >= limits[r0 + half * 4 + i]) s[i] = -INFINITY;
                 float mx = s[i];
 #pragma unroll
                 for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
@@ -265,14 +363,14 @@ __global__ void __launch_bounds__(kSimtWarps * 32) attn_simt_kernel(AttnArgs a)
                     for (int c = 0; c < kDims; c++) o[r][c] = __fmul_rn(o[r][c], sh.alpha[warp][r]);
             }
             __syncwarp();
-            const bool some_masked = tile + step + kStep > sh.least_limit;
+            const bool some_masked = tile.key0 + step + kStep > least;
 #pragma unroll 4
             for (int i = 0; i < kStep; i++) {
                 float pr[kRows], vx[kDims];
 #pragma unroll
                 for (int r = 0; r < kRows; r++) pr[r] = sh.p[warp][i][r];
 #pragma unroll
-                for (int c = 0; c < kDims; c++) vx[c] = Elem<T>::load(&sh.v[step + i][lane * kDims + c]);
+                for (int c = 0; c < kDims; c++) vx[c] = st.v[step + i][lane * kDims + c];
                 // a row must not take 0 * inf from a key it does not see
 #pragma unroll
                 for (int r = 0; r < kRows; r++)
@@ -281,6 +379,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) attn_simt_kernel(AttnArgs a)
                         for (int c = 0; c < kDims; c++) o[r][c] = __fmaf_rn(pr[r], vx[c], o[r][c]);
             }
         }
+        __syncthreads();
     }
     // row sums over the 16 key lanes
 #pragma unroll
@@ -289,46 +388,293 @@ __global__ void __launch_bounds__(kSimtWarps * 32) attn_simt_kernel(AttnArgs a)
         for (int w = 8; w > 0; w >>= 1) l[i] = __fadd_rn(l[i], __shfl_xor_sync(0xffffffffu, l[i], w));
 
     // the warps' results, joined over the warps when they split the keys
+    cp_async_wait<0>();
     __syncthreads();
-    float* ml = reinterpret_cast<float*>(&sh.q[0][0]);        // [warps][8][2]
-    float* ow = reinterpret_cast<float*>(&sh.k[0][0]);        // [warps][8][D]
-    static_assert(sizeof(float) * kSimtWarps * kRows * D <= sizeof(sh.k) + sizeof(sh.v), "join space");
+    float* ow = reinterpret_cast<float*>(&sh.stage[0]);  // [warps][8][D]
+    static_assert(sizeof(float) * kWarps * kRows * D <= sizeof(sh.stage), "join space");
     if ((lane & 15) == 0)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            ml[(warp * kRows + half * 4 + i) * 2] = m[i];
-            ml[(warp * kRows + half * 4 + i) * 2 + 1] = l[i];
+            sh.ml[warp][half * 4 + i][0] = m[i];
+            sh.ml[warp][half * 4 + i][1] = l[i];
         }
 #pragma unroll
     for (int r = 0; r < kRows; r++)
 #pragma unroll
         for (int c = 0; c < kDims; c++) ow[(warp * kRows + r) * D + lane * kDims + c] = o[r][c];
     __syncthreads();
-    for (int i = threadIdx.x; i < j.rows * D; i += blockDim.x) {
+    for (int i = threadIdx.x; i < j.rows * D; i += kThreads) {
         const int r = i / D, d = i % D;
         float mx, sum, val;
         if (split_keys) {
             mx = -INFINITY;
-            for (int w = 0; w < kSimtWarps; w++) mx = fmaxf(mx, ml[(w * kRows + r) * 2]);
+            for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, sh.ml[w][r][0]);
             sum = val = 0.0f;
-            for (int w = 0; w < kSimtWarps; w++) {
-                const float mw = ml[(w * kRows + r) * 2], lw = ml[(w * kRows + r) * 2 + 1];
+            for (int w = 0; w < kWarps; w++) {
+                const float lw = sh.ml[w][r][1];
                 if (lw == 0.0f) continue;  // saw no key
-                const float f = expf(__fsub_rn(mw, mx));
+                const float f = expf(__fsub_rn(sh.ml[w][r][0], mx));
                 sum = __fmaf_rn(f, lw, sum);
                 val = __fmaf_rn(f, ow[(w * kRows + r) * D + d], val);
             }
         } else {
-            mx = ml[r * 2];
-            sum = ml[r * 2 + 1];
+            mx = sh.ml[r / kRows][r % kRows][0];
+            sum = sh.ml[r / kRows][r % kRows][1];
             val = ow[r * D + d];
         }
-        const int64_t at = ((int64_t)sh.token[r] * a.heads + sh.head[r]) * a.parts + j.part;
-        a.part_o[at * D + d] = val;
-        if (d == 0) a.part_ml[at] = make_float2(mx, sum);
+        put_result<T, D>(a, j, sh.rows.token[r], sh.rows.head[r], d, mx, sum, val);
     }
 }
 
+// ------------------------------------------------- 16-bit tensor arithmetic ----
+// Tiles of 16 rows per warp, 16 keys at a time, mma.sync m16n8k16 for both
+// products with 32-bit sums; the weights are rounded to the elements' type for
+// the second, as the values are.  Keys split over the warps as above.
+constexpr int kMmaRows = 16;
+template <typename T, int D>
+struct MmaConf {
+    static constexpr int kStages = D == 64 ? 4 : 3;
+};
+template <typename T, int D>
+struct MmaSmem {
+    struct {
+        T k[kTile * D], v[kTile * D];
+    } stage[MmaConf<T, D>::kStages];
+    float ml[kWarps][kMmaRows][2];
+    Rows<kWarps * kMmaRows> rows;
+};
+// 16-byte pieces of a row lie turned by the row's number: eight rows of one column
+// fall on different banks.
+template <int D>
+TMAC_DEV int turned(int row, int c)
+{
+    return row * D + ((c / 8 ^ (row & 7)) * 8 | c % 8);
+}
+TMAC_DEV void ldmatrix4(uint32_t (&r)[4], const void* p)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_addr(p))
+                 : "memory");
+}
+TMAC_DEV void ldmatrix4_trans(uint32_t (&r)[4], const void* p)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_addr(p))
+                 : "memory");
+}
+template <typename T>
+TMAC_DEV void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (std::is_same_v<T, __half>)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T>
+TMAC_DEV uint32_t pack2(float lo, float hi)
+{
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+TMAC_DEV bool finite16(uint32_t pair, uint32_t exponent)  // both values of a pair
+{
+    return (pair & exponent) != exponent && ((pair >> 16) & exponent) != exponent;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
+{
+    extern __shared__ __align__(16) uint8_t smem[];
+    using Smem = MmaSmem<T, D>;
+    Smem& sh = *reinterpret_cast<Smem*>(smem);
+    constexpr int kJobRows = kWarps * kMmaRows, kStages = MmaConf<T, D>::kStages, kN = D / 8;
+    Job j;
+    if (!find_job<kJobRows>(a, &j)) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
+    const bool split_keys = j.rows <= kMmaRows;
+    const auto start = [&](int t) {
+        if (t < j.tile1) {
+            auto& st = sh.stage[(t - j.tile0) % kStages];
+            copy_tile<T, D>(a, j, t, [&](int key, int c) { return &st.k[turned<D>(key, c)]; },
+                            [&](int key, int c) { return &st.v[turned<D>(key, c)]; });
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) start(j.tile0 + i);
+    sh.rows.find(a, j);
+
+    // this thread's rows g and g + 8 of the warp's, as the product's first operand
+    const int r0 = split_keys ? 0 : warp * kMmaRows;
+    uint32_t q[D / 16][4];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int r = r0 + g + 8 * h;
+        const T* src = (const T*)a.q + sh.rows.token[r] * a.q_stride + sh.rows.head[r] * D + c2;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++)
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                T pair[2] = {};
+                if (r < j.rows) {
+                    pair[0] = src[16 * i + 8 * w];
+                    pair[1] = src[16 * i + 8 * w + 1];
+                }
+                q[i][2 * w + h] = *reinterpret_cast<const uint32_t*>(pair);
+            }
+    }
+    const float scale = __fmul_rn(a.scale, 1.44269504f);  // log2 e: exponentials are powers of 2
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[kN][4];
+#pragma unroll
+    for (int n = 0; n < kN; n++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[n][c] = 0.0f;
+
+    for (int t = j.tile0; t < j.tile1; t++) {
+        cp_async_wait<kStages - 2>();
+        __syncthreads();
+        start(t + kStages - 1);
+        const auto& st = sh.stage[(t - j.tile0) % kStages];
+        const TileOf tile = find_tile(a, j, t);
+        const int* limits = tile.prefix ? sh.rows.p_limit : sh.rows.o_limit;
+        const int least = min(tile.prefix ? sh.rows.p_least : sh.rows.o_least, tile.keys);
+        for (int step = split_keys ? warp * kStep : 0; step < (split_keys ? (warp + 1) * kStep : kTile); step += kStep) {
+            if (tile.key0 + step >= tile.keys || r0 >= j.rows) break;
+            float s[2][4] = {};
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                uint32_t kx[4];  // keys 0-7 and 8-15, two halves of 16 dims each
+                ldmatrix4(kx, &st.k[turned<D>(step + (lane & 7) + (lane >> 4) * 8, 16 * i + (lane >> 3 & 1) * 8)]);
+                mma16816<T>(s[0], q[i], kx[0], kx[1]);
+                mma16816<T>(s[1], q[i], kx[2], kx[3]);
+            }
+            const bool some_masked = tile.key0 + step + kStep > least;
+            float al[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int limit = limits[r0 + g + 8 * h];
+                float mx = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float& x = s[n][2 * h + c];
+                        x = __fmul_rn(x, scale);
+                        if (some_masked && tile.key0 + step + 8 * n + c2 + c >= limit) x = -INFINITY;
+                        mx = fmaxf(mx, x);
+                    }
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                mx = fmaxf(mx, m[h]);
+                al[h] = mx == m[h] ? 1.0f : exp2_fast(__fsub_rn(m[h], mx));
+                float sum = 0.0f;
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float& x = s[n][2 * h + c];
+                        x = x == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(x, mx));
+                        sum = __fadd_rn(sum, x);
+                    }
+                m[h] = mx;
+                l[h] = __fmaf_rn(l[h], al[h], sum);
+            }
+            if (__any_sync(0xffffffffu, al[0] != 1.0f || al[1] != 1.0f))
+#pragma unroll
+                for (int n = 0; n < kN; n++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[n][c] = __fmul_rn(o[n][c], al[c >> 1]);
+            bool sound = true;  // no value that times 0 is not 0, where some row has 0 for a key it does not see
+            if (some_masked) {
+                const uint32_t exponent = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+                for (int i = lane; i < kStep * D / 2; i += 32)
+                    sound &= finite16(*reinterpret_cast<const uint32_t*>(&st.v[(step + i / (D / 2)) * D + i % (D / 2) * 2]), exponent);
+                sound = __all_sync(0xffffffffu, sound);
+            }
+            if (sound) {
+                const uint32_t p[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
+                                       pack2<T>(s[1][2], s[1][3])};
+#pragma unroll
+                for (int n = 0; n < kN; n += 2) {
+                    uint32_t vx[4];  // keys 0-7 and 8-15 of dims 8n.., then of the next eight
+                    ldmatrix4_trans(vx, &st.v[turned<D>(step + (lane & 15), 8 * n + (lane >> 4) * 8)]);
+                    mma16816<T>(o[n], p, vx[0], vx[1]);
+                    mma16816<T>(o[n + 1], p, vx[2], vx[3]);
+                }
+            } else {
+                // key by key, each row with those it sees
+#pragma unroll
+                for (int kk = 0; kk < kStep; kk++) {
+                    const float p0 = __shfl_sync(0xffffffffu, s[kk / 8][kk & 1], g * 4 + (kk % 8) / 2);
+                    const float p1 = __shfl_sync(0xffffffffu, s[kk / 8][2 + (kk & 1)], g * 4 + (kk % 8) / 2);
+#pragma unroll
+                    for (int n = 0; n < kN; n++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            const float v = Elem<T>::load(&st.v[turned<D>(step + kk, 8 * n + c2 + c)]);
+                            if (p0 != 0.0f) o[n][c] = __fmaf_rn(p0, v, o[n][c]);
+                            if (p1 != 0.0f) o[n][2 + c] = __fmaf_rn(p1, v, o[n][2 + c]);
+                        }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 1));
+        l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 2));
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    float* ow = reinterpret_cast<float*>(&sh.stage[0]);  // [warps][16][D]
+    static_assert(sizeof(float) * kWarps * kMmaRows * D <= sizeof(sh.stage), "join space");
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const int r = g + 8 * h;
+        if (c2 == 0) {
+            sh.ml[warp][r][0] = m[h];
+            sh.ml[warp][r][1] = l[h];
+        }
+#pragma unroll
+        for (int n = 0; n < kN; n++)
+            *reinterpret_cast<float2*>(&ow[(warp * kMmaRows + r) * D + 8 * n + c2]) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < j.rows * D; i += kThreads) {
+        const int r = i / D, d = i % D;
+        float mx, sum, val;
+        if (split_keys) {
+            mx = -INFINITY;
+            for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, sh.ml[w][r][0]);
+            sum = val = 0.0f;
+            for (int w = 0; w < kWarps; w++) {
+                const float lw = sh.ml[w][r][1];
+                if (lw == 0.0f) continue;  // saw no key
+                const float f = exp2_fast(__fsub_rn(sh.ml[w][r][0], mx));
+                sum = __fmaf_rn(f, lw, sum);
+                val = __fmaf_rn(f, ow[(w * kMmaRows + r) * D + d], val);
+            }
+        } else {
+            mx = sh.ml[r / kMmaRows][r % kMmaRows][0];
+            sum = sh.ml[r / kMmaRows][r % kMmaRows][1];
+            val = ow[r * D + d];
+        }
+        put_result<T, D>(a, j, sh.rows.token[r], sh.rows.head[r], d, mx, sum, val);
+    }
+}
+
+// ------------------------------------------------------------------- join ----
 // Joins the parts of one (token, head) per warp.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a)
@@ -338,8 +684,11 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a)
     if (row >= (int64_t)a.tokens * a.heads) return;
     const int token = (int)(row / a.heads), head = (int)(row % a.heads), lane = threadIdx.x & 31;
     const int b = sequence_of(a, token);
-    const int own = a.o_splits ? (own_len(a, b) + a.o_chunk - 1) / a.o_chunk : 0;
-    const int n = a.p_splits + (token_count(a, b) > token - first_token(a, b) ? own : 0);
+    int own = 0;
+    if (a.o_splits && token_count(a, b) > token - first_token(a, b)) {
+        own = (tiles_of(own_len(a, b)) + a.o_range - 1) / a.o_range;
+    }
+    const int n = a.p_splits + own;
     const float2* ml = a.part_ml + row * a.parts;
     const float* po = a.part_o + row * a.parts * D + lane * kDims;
     float mx = -INFINITY;
@@ -352,7 +701,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a)
     for (int s = 0; s < n; s++) {
         const float2 p = ml[s];
         if (p.y == 0.0f) continue;  // saw no key
-        const float f = expf(__fsub_rn(p.x, mx));
+        const float f = power<T>(__fsub_rn(p.x, mx));
         sum = __fmaf_rn(f, p.y, sum);
 #pragma unroll
         for (int c = 0; c < kDims; c++) o[c] = __fmaf_rn(f, po[(int64_t)s * D + c], o[c]);
@@ -362,26 +711,34 @@ __global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a)
     for (int c = 0; c < kDims; c++) Elem<T>::store(out + c, sum == 0.0f ? 0.0f : __fdiv_rn(o[c], sum));
 }
 
-// How the work is cut: key ranges so that the grid has about two jobs per SM, of
-// a tile at least.
-int plan(AttnArgs* a, int sms)
+// How the work is cut.
+int plan(AttnArgs* a, int job_rows, int sms)
 {
-    constexpr int kJobRows = kSimtWarps * kRows;
     const int hk = a->cache.kv_heads;
-    auto ranges = [&](int64_t jobs, int keys, int* splits, int* chunk) {
-        if (!jobs || !keys) {
-            *splits = *chunk = 0;
+    const auto tiles = [](int keys) { return (keys + kTile - 1) / kTile; };
+    // key ranges so that there are about `per_sm` jobs per SM, of a tile at least
+    const auto ranges = [&](int64_t jobs, int n_tiles, int per_sm, int* splits, int* range) {
+        if (!jobs || !n_tiles) {
+            *splits = *range = 0;
             return;
         }
-        const int tiles = (keys + kTile - 1) / kTile;
-        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(tiles, 2 * sms / jobs));
-        *chunk = (int)((tiles + want - 1) / want) * kTile;
-        *splits = (keys + *chunk - 1) / *chunk;
+        const int64_t want = std::max<int64_t>(1, std::min<int64_t>(n_tiles, (int64_t)per_sm * sms / jobs));
+        *range = (int)((n_tiles + want - 1) / want);
+        *splits = (n_tiles + *range - 1) / *range;
     };
-    a->p_tiles = (int)(((int64_t)a->tokens * a->group + kJobRows - 1) / kJobRows);
-    a->o_tiles = (int)(((int64_t)a->max_q * a->group + kJobRows - 1) / kJobRows);
-    ranges((int64_t)a->p_tiles * hk, a->prefix_len, &a->p_splits, &a->p_chunk);
-    ranges((int64_t)a->batch * a->o_tiles * hk, a->max_own, &a->o_splits, &a->o_chunk);
+    a->o_tiles = (int)(((int64_t)a->max_q * a->group + job_rows - 1) / job_rows);
+    const int64_t o_jobs = (int64_t)a->batch * a->o_tiles * hk;
+    const int all_tiles = tiles(a->prefix_len) + tiles(a->max_own);
+    a->alone = all_tiles <= kAloneTiles;
+    if (a->alone) {
+        a->p_tiles = a->p_splits = 0;
+        a->o_splits = 1;
+        a->o_range = std::max(1, all_tiles);
+    } else {
+        a->p_tiles = (int)(((int64_t)a->tokens * a->group + job_rows - 1) / job_rows);
+        ranges((int64_t)a->p_tiles * hk, tiles(a->prefix_len), 2, &a->p_splits, &a->p_range);
+        ranges(o_jobs, tiles(a->max_own), 2, &a->o_splits, &a->o_range);
+    }
     a->p_jobs = (int64_t)a->p_tiles * hk * a->p_splits;
     a->parts = a->p_splits + a->o_splits;
     return TMAC_OK;
@@ -389,6 +746,7 @@ int plan(AttnArgs* a, int sms)
 
 size_t workspace_bytes_of(const AttnArgs& a)
 {
+    if (a.parts == 1) return 0;
     const size_t rows = (size_t)a.tokens * a.heads * a.parts;
     return rows * (size_t)a.cache.dim * sizeof(float) + rows * sizeof(float2);
 }
@@ -399,11 +757,20 @@ int launch_attention(const AttnArgs& a, cudaStream_t s)
     const int64_t jobs = a.p_jobs + (int64_t)a.batch * a.o_tiles * a.cache.kv_heads * a.o_splits;
     if (jobs > 0x7FFFFFFF) return fail(TMAC_ERR_SHAPE, "too many jobs for one grid");
     if (jobs) {
-        auto fn = attn_simt_kernel<T, D>;
-        TMAC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SimtSmem<T, D>)));
-        fn<<<(unsigned)jobs, kSimtWarps * 32, sizeof(SimtSmem<T, D>), s>>>(a);
+        size_t smem;
+        void (*fn)(AttnArgs);
+        if constexpr (sizeof(T) == 4) {
+            fn = attn_simt_kernel<T, D>;
+            smem = sizeof(SimtSmem<D>);
+        } else {
+            fn = attn_mma_kernel<T, D>;
+            smem = sizeof(MmaSmem<T, D>);
+        }
+        TMAC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        fn<<<(unsigned)jobs, kThreads, smem, s>>>(a);
         TMAC_CUDA_TRY(cudaGetLastError());
     }
+    if (a.parts == 1) return TMAC_OK;
     attn_join_kernel<T, D><<<(unsigned)(((int64_t)a.tokens * a.heads + 3) / 4), 128, 0, s>>>(a);
     TMAC_CUDA_TRY(cudaGetLastError());
     return TMAC_OK;
@@ -432,7 +799,7 @@ int prepare(const tmac_paged_cache* cache, int heads, int tokens, int batch, int
     a->max_own = max_own;
     a->table_width = table_width;
     if (tokens == 0) return TMAC_OK;
-    return plan(a, num_sms(cache->device));
+    return plan(a, cache->type == TMAC_TYPE_F32 ? kWarps * kRows : kWarps * kMmaRows, num_sms(cache->device));
 }
 
 }  // namespace
