@@ -208,30 +208,51 @@ TMAC_DEV void cp_async_wait()
 {
     asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
-// Starts the copies of tile t's keys and values; k_at(key, value) and v_at say where
-// 16 bytes from that value on go.  Keys out of reach, and rows of a page outside
-// the pool (the error word says so), become zeros.
-template <typename T, int D, typename FK, typename FV>
-TMAC_DEV void copy_tile(const AttnArgs& a, const Job& j, int t, FK&& k_at, FV&& v_at)
-{
-    constexpr int kVec = 16 / sizeof(T), kPer = D / kVec, kCopies = kTile * kPer / kThreads;
-    const TileOf tile = find_tile(a, j, t);
-    const int shift = a.cache.page_shift;
-#pragma unroll
-    for (int i = 0; i < kCopies; i++) {
-        const int at = threadIdx.x + i * kThreads, key = at / kPer, c = at % kPer * kVec;
-        const int g = tile.key0 + key;
-        bool valid = g < tile.keys;
-        const int64_t page = valid ? tile.pages[g >> shift] : 0;
-        if (page < 0 || page >= a.cache.n_pages) {
-            record_error(a.err, TMAC_ERR_BOUNDS);
-            valid = false;
-        }
-        const int64_t from = valid ? (((page * a.cache.kv_heads + j.kvh) << shift) + (g & ((1 << shift) - 1))) * D + c : 0;
-        cp_async16(k_at(key, c), (const T*)a.cache.k + from, valid);
-        cp_async16(v_at(key, c), (const T*)a.cache.v + from, valid);
+// Copies tiles of keys and values into shared memory, 16 bytes a thread.  A warp
+// touches 16 keys of a tile; its lanes look their pages up one tile ahead of the
+// copies, so a copy does not wait for a table.
+template <typename T, int D>
+struct Copier {
+    static constexpr int kVec = 16 / sizeof(T), kPer = D / kVec;          // copies to a key
+    static constexpr int kCopies = kTile * kPer / kThreads;               // of a thread
+    static constexpr int kAtOnce = 32 / kPer < 1 ? 1 : 32 / kPer;         // keys of a warp's one copy
+    static constexpr int kKeys = kTile / kWarps;                          // keys of the warp
+    static_assert(kPer <= 32 && kKeys <= 32 && kKeys == kCopies * kAtOnce, "a lane to a key");
+    int page;  // of this lane's key, for the tile to copy next
+
+    // The tile's key that copy i of lane `lane` belongs to
+    static TMAC_DEV int key_of(int i, int lane) { return (threadIdx.x >> 5) * kAtOnce + i * (kWarps * kAtOnce) + lane / kPer; }
+    TMAC_DEV void look_up(const AttnArgs& a, const Job& j, int t)
+    {
+        const int lane = threadIdx.x & 31;
+        if (t >= j.tile1 || lane >= kKeys) return;
+        const TileOf tile = find_tile(a, j, t);
+        const int g = tile.key0 + key_of(lane / kAtOnce, lane % kAtOnce * kPer);
+        page = g < tile.keys ? __ldg(tile.pages + (g >> a.cache.page_shift)) : 0;
     }
-}
+    // Starts tile t's copies, after its look_up; k_at(key, value) and v_at say where 16
+    // bytes from that value on go.  Keys out of reach, and rows of a page outside the
+    // pool (the error word says so), become zeros.
+    template <typename FK, typename FV>
+    TMAC_DEV void start(const AttnArgs& a, const Job& j, int t, FK&& k_at, FV&& v_at) const
+    {
+        const int lane = threadIdx.x & 31, shift = a.cache.page_shift;
+        const TileOf tile = find_tile(a, j, t);
+        const bool known = page >= 0 && page < a.cache.n_pages;
+        if (!known && lane < kKeys && tile.key0 + key_of(lane / kAtOnce, lane % kAtOnce * kPer) < tile.keys)
+            record_error(a.err, TMAC_ERR_BOUNDS);
+        const int safe = known ? page : -1;
+#pragma unroll
+        for (int i = 0; i < kCopies; i++) {
+            const int key = key_of(i, lane), c = lane % kPer * kVec, g = tile.key0 + key;
+            const int64_t pg = __shfl_sync(0xffffffffu, safe, i * kAtOnce + lane / kPer);
+            const bool valid = pg >= 0 && g < tile.keys;
+            const int64_t from = valid ? (((pg * a.cache.kv_heads + j.kvh) << shift) + (g & ((1 << shift) - 1))) * D + c : 0;
+            cp_async16(k_at(key, c), (const T*)a.cache.k + from, valid);
+            cp_async16(v_at(key, c), (const T*)a.cache.v + from, valid);
+        }
+    }
+};
 // Row r's result, value d: the part's, or the rounded quotient when there is no other.
 template <typename T, int D>
 TMAC_DEV void put_result(const AttnArgs& a, const Job& j, int token, int head, int d, float m, float l, float o)
@@ -288,13 +309,16 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(AttnArgs a)
     if (!find_job<kJobRows>(a, &j)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool split_keys = j.rows <= kRows;
+    Copier<T, D> copier;
     const auto start = [&](int t) {
         if (t < j.tile1) {
             auto& st = sh.stage[(t - j.tile0) % kSimtStages];
-            copy_tile<T, D>(a, j, t, [&](int key, int c) { return &st.k[key][c]; }, [&](int key, int c) { return &st.v[key][c]; });
+            copier.start(a, j, t, [&](int key, int c) { return &st.k[key][c]; }, [&](int key, int c) { return &st.v[key][c]; });
+            copier.look_up(a, j, t + 1);
         }
         cp_async_commit();
     };
+    copier.look_up(a, j, j.tile0);
     start(j.tile0);
     sh.rows.find(a, j);
     for (int i = threadIdx.x; i < kJobRows * D; i += kThreads) {
@@ -427,13 +451,13 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(AttnArgs a)
 }
 
 // ------------------------------------------------- 16-bit tensor arithmetic ----
-// Tiles of 16 rows per warp, 16 keys at a time, mma.sync m16n8k16 for both
-// products with 32-bit sums; the weights are rounded to the elements' type for
+// Tiles of 16 rows per warp, mma.sync m16n8k16 for both products with 32-bit sums; the weights are rounded to the elements' type for
 // the second, as the values are.  Keys split over the warps as above.
 constexpr int kMmaRows = 16;
 template <typename T, int D>
 struct MmaConf {
     static constexpr int kStages = D == 64 ? 4 : 3;
+    static constexpr int kWide = D == 64 ? 64 : 32;  // keys at a time where warps hold different rows
 };
 template <typename T, int D>
 struct MmaSmem {
@@ -487,30 +511,28 @@ TMAC_DEV uint32_t pack2(float lo, float hi)
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 }
-TMAC_DEV bool finite16(uint32_t pair, uint32_t exponent)  // both values of a pair
-{
-    return (pair & exponent) != exponent && ((pair >> 16) & exponent) != exponent;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
 {
     extern __shared__ __align__(16) uint8_t smem[];
     using Smem = MmaSmem<T, D>;
     Smem& sh = *reinterpret_cast<Smem*>(smem);
-    constexpr int kJobRows = kWarps * kMmaRows, kStages = MmaConf<T, D>::kStages, kN = D / 8;
+    constexpr int kJobRows = kWarps * kMmaRows, kStages = MmaConf<T, D>::kStages, kWide = MmaConf<T, D>::kWide, kN = D / 8;
     Job j;
     if (!find_job<kJobRows>(a, &j)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
     const bool split_keys = j.rows <= kMmaRows;
+    Copier<T, D> copier;
     const auto start = [&](int t) {
         if (t < j.tile1) {
             auto& st = sh.stage[(t - j.tile0) % kStages];
-            copy_tile<T, D>(a, j, t, [&](int key, int c) { return &st.k[turned<D>(key, c)]; },
-                            [&](int key, int c) { return &st.v[turned<D>(key, c)]; });
+            copier.start(a, j, t, [&](int key, int c) { return &st.k[turned<D>(key, c)]; },
+                         [&](int key, int c) { return &st.v[turned<D>(key, c)]; });
+            copier.look_up(a, j, t + 1);
         }
         cp_async_commit();
     };
+    copier.look_up(a, j, j.tile0);
 #pragma unroll
     for (int i = 0; i < kStages - 1; i++) start(j.tile0 + i);
     sh.rows.find(a, j);
@@ -535,7 +557,11 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
             }
     }
     const float scale = __fmul_rn(a.scale, 1.44269504f);  // log2 e: exponentials are powers of 2
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[kN][4];
+    float m[2], l[2], o[kN][4];
+    bool careful = false;
+again:
+#pragma unroll
+    for (int h = 0; h < 2; h++) m[h] = -INFINITY, l[h] = 0.0f;
 #pragma unroll
     for (int n = 0; n < kN; n++)
 #pragma unroll
@@ -549,24 +575,27 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
         const TileOf tile = find_tile(a, j, t);
         const int* limits = tile.prefix ? sh.rows.p_limit : sh.rows.o_limit;
         const int least = min(tile.prefix ? sh.rows.p_least : sh.rows.o_least, tile.keys);
-        for (int step = split_keys ? warp * kStep : 0; step < (split_keys ? (warp + 1) * kStep : kTile); step += kStep) {
-            if (tile.key0 + step >= tile.keys || r0 >= j.rows) break;
-            float s[2][4] = {};
+        // kN8 * 8 keys from `step` on
+        const auto keys = [&](auto n8, int step) {
+            constexpr int kN8 = decltype(n8)::value;
+            float s[kN8][4] = {};
 #pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                uint32_t kx[4];  // keys 0-7 and 8-15, two halves of 16 dims each
-                ldmatrix4(kx, &st.k[turned<D>(step + (lane & 7) + (lane >> 4) * 8, 16 * i + (lane >> 3 & 1) * 8)]);
-                mma16816<T>(s[0], q[i], kx[0], kx[1]);
-                mma16816<T>(s[1], q[i], kx[2], kx[3]);
-            }
-            const bool some_masked = tile.key0 + step + kStep > least;
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int n = 0; n < kN8; n += 2) {
+                    uint32_t kx[4];  // keys 0-7 and 8-15, two halves of 16 dims each
+                    ldmatrix4(kx, &st.k[turned<D>(step + 8 * n + (lane & 7) + (lane >> 4) * 8, 16 * i + (lane >> 3 & 1) * 8)]);
+                    mma16816<T>(s[n], q[i], kx[0], kx[1]);
+                    mma16816<T>(s[n + 1], q[i], kx[2], kx[3]);
+                }
+            const bool some_masked = tile.key0 + step + 8 * kN8 > least;
             float al[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const int limit = limits[r0 + g + 8 * h];
                 float mx = -INFINITY;
 #pragma unroll
-                for (int n = 0; n < 2; n++)
+                for (int n = 0; n < kN8; n++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         float& x = s[n][2 * h + c];
@@ -578,13 +607,14 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 mx = fmaxf(mx, m[h]);
                 al[h] = mx == m[h] ? 1.0f : exp2_fast(__fsub_rn(m[h], mx));
+                const float base = mx == -INFINITY ? 0.0f : mx;  // sees nothing yet: all 0
                 float sum = 0.0f;
 #pragma unroll
-                for (int n = 0; n < 2; n++)
+                for (int n = 0; n < kN8; n++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         float& x = s[n][2 * h + c];
-                        x = x == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(x, mx));
+                        x = exp2_fast(__fsub_rn(x, base));
                         sum = __fadd_rn(sum, x);
                     }
                 m[h] = mx;
@@ -595,39 +625,61 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
                 for (int n = 0; n < kN; n++)
 #pragma unroll
                     for (int c = 0; c < 4; c++) o[n][c] = __fmul_rn(o[n][c], al[c >> 1]);
-            bool sound = true;  // no value that times 0 is not 0, where some row has 0 for a key it does not see
-            if (some_masked) {
-                const uint32_t exponent = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
-                for (int i = lane; i < kStep * D / 2; i += 32)
-                    sound &= finite16(*reinterpret_cast<const uint32_t*>(&st.v[(step + i / (D / 2)) * D + i % (D / 2) * 2]), exponent);
-                sound = __all_sync(0xffffffffu, sound);
-            }
-            if (sound) {
-                const uint32_t p[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
-                                       pack2<T>(s[1][2], s[1][3])};
+            if (!careful) {
 #pragma unroll
-                for (int n = 0; n < kN; n += 2) {
-                    uint32_t vx[4];  // keys 0-7 and 8-15 of dims 8n.., then of the next eight
-                    ldmatrix4_trans(vx, &st.v[turned<D>(step + (lane & 15), 8 * n + (lane >> 4) * 8)]);
-                    mma16816<T>(o[n], p, vx[0], vx[1]);
-                    mma16816<T>(o[n + 1], p, vx[2], vx[3]);
+                for (int k = 0; k < kN8; k += 2) {
+                    const uint32_t p[4] = {pack2<T>(s[k][0], s[k][1]), pack2<T>(s[k][2], s[k][3]), pack2<T>(s[k + 1][0], s[k + 1][1]),
+                                           pack2<T>(s[k + 1][2], s[k + 1][3])};
+#pragma unroll
+                    for (int n = 0; n < kN; n += 2) {
+                        uint32_t vx[4];  // keys 0-7 and 8-15 of dims 8n.., then of the next eight
+                        ldmatrix4_trans(vx, &st.v[turned<D>(step + 8 * k + (lane & 15), 8 * n + (lane >> 4) * 8)]);
+                        mma16816<T>(o[n], p, vx[0], vx[1]);
+                        mma16816<T>(o[n + 1], p, vx[2], vx[3]);
+                    }
                 }
             } else {
-                // key by key, each row with those it sees
 #pragma unroll
-                for (int kk = 0; kk < kStep; kk++) {
-                    const float p0 = __shfl_sync(0xffffffffu, s[kk / 8][kk & 1], g * 4 + (kk % 8) / 2);
-                    const float p1 = __shfl_sync(0xffffffffu, s[kk / 8][2 + (kk & 1)], g * 4 + (kk % 8) / 2);
+                for (int k = 0; k < kN8; k++)
 #pragma unroll
-                    for (int n = 0; n < kN; n++)
+                    for (int c8 = 0; c8 < 2; c8++)
+#pragma unroll 1
+                        for (int u = 0; u < 4; u++) {  // key 8 k + 2 u + c8, whose weights lane u of each row holds
+                            const float p0 = __shfl_sync(0xffffffffu, s[k][c8], g * 4 + u), p1 = __shfl_sync(0xffffffffu, s[k][2 + c8], g * 4 + u);
 #pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            const float v = Elem<T>::load(&st.v[turned<D>(step + kk, 8 * n + c2 + c)]);
-                            if (p0 != 0.0f) o[n][c] = __fmaf_rn(p0, v, o[n][c]);
-                            if (p1 != 0.0f) o[n][2 + c] = __fmaf_rn(p1, v, o[n][2 + c]);
+                            for (int n = 0; n < kN; n++)
+#pragma unroll
+                                for (int c = 0; c < 2; c++) {
+                                    const float v = Elem<T>::load(&st.v[turned<D>(step + 8 * k + 2 * u + c8, 8 * n + c2 + c)]);
+                                    if (p0 != 0.0f) o[n][c] = __fmaf_rn(p0, v, o[n][c]);
+                                    if (p1 != 0.0f) o[n][2 + c] = __fmaf_rn(p1, v, o[n][2 + c]);
+                                }
                         }
-                }
             }
+        };
+        if (split_keys) {
+            if (tile.key0 + warp * kStep < tile.keys) keys(std::integral_constant<int, 2>(), warp * kStep);
+        } else if (r0 < j.rows) {
+            for (int step = 0; step < kTile && tile.key0 + step < tile.keys; step += kWide)
+                keys(std::integral_constant<int, kWide / 8>(), step);
+        }
+    }
+    cp_async_wait<0>();
+    // The product adds 0 * v for a key that a row does not see, which an infinite or NaN
+    // v turns into NaN.  Where any sum is not finite the job runs again key by key,
+    // each row with those it sees.
+    if (!careful) {
+        bool finite = true;
+#pragma unroll
+        for (int n = 0; n < kN; n++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) finite &= fabsf(o[n][c]) < INFINITY;
+        if (__syncthreads_or(!finite)) {
+            careful = true;
+            copier.look_up(a, j, j.tile0);
+#pragma unroll
+            for (int i = 0; i < kStages - 1; i++) start(j.tile0 + i);
+            goto again;
         }
     }
 #pragma unroll
@@ -635,7 +687,6 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
         l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 1));
         l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 2));
     }
-    cp_async_wait<0>();
     __syncthreads();
     float* ow = reinterpret_cast<float*>(&sh.stage[0]);  // [warps][16][D]
     static_assert(sizeof(float) * kWarps * kMmaRows * D <= sizeof(sh.stage), "join space");
@@ -675,40 +726,78 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
 }
 
 // ------------------------------------------------------------------- join ----
-// Joins the parts of one (token, head) per warp.
+// Joins the parts of one (token, head) per CTA: groups of D / 4 threads take every
+// kGroups-th part, four values a thread, several loads in flight.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attn_join_kernel(AttnArgs a)
+__global__ void __launch_bounds__(kThreads) attn_join_kernel(AttnArgs a)
 {
-    constexpr int kDims = D / 32;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= (int64_t)a.tokens * a.heads) return;
-    const int token = (int)(row / a.heads), head = (int)(row % a.heads), lane = threadIdx.x & 31;
+    constexpr int kLanes = D / 4, kGroups = kThreads / kLanes, kFlight = 4;
+    __shared__ float weight[kThreads], red[kWarps][2];
+    __shared__ float4 sums[kGroups][kLanes];
+    const int64_t row = blockIdx.x;
+    const int token = (int)(row / a.heads), head = (int)(row % a.heads);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = threadIdx.x / kLanes, d4 = threadIdx.x % kLanes;
     const int b = sequence_of(a, token);
     int own = 0;
-    if (a.o_splits && token_count(a, b) > token - first_token(a, b)) {
-        own = (tiles_of(own_len(a, b)) + a.o_range - 1) / a.o_range;
-    }
+    if (a.o_splits && token_count(a, b) > token - first_token(a, b)) own = (tiles_of(own_len(a, b)) + a.o_range - 1) / a.o_range;
     const int n = a.p_splits + own;
     const float2* ml = a.part_ml + row * a.parts;
-    const float* po = a.part_o + row * a.parts * D + lane * kDims;
-    float mx = -INFINITY;
-    for (int s = lane; s < n; s += 32) mx = fmaxf(mx, ml[s].x);
+    const float4* po = reinterpret_cast<const float4*>(a.part_o + row * a.parts * D) + d4;
+    pdl_wait();
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < n; s0 += kThreads) {
+        const int count = min(kThreads, n - s0);
+        const float2 p = (int)threadIdx.x < count ? ml[s0 + threadIdx.x] : make_float2(-INFINITY, 0.0f);
+        float mx = p.x;
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-    float sum = 0.0f, o[kDims];
+        for (int w = 16; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+        if (lane == 0) red[warp][0] = mx;
+        __syncthreads();
+        mx = m;
 #pragma unroll
-    for (int c = 0; c < kDims; c++) o[c] = 0.0f;
-    for (int s = 0; s < n; s++) {
-        const float2 p = ml[s];
-        if (p.y == 0.0f) continue;  // saw no key
-        const float f = power<T>(__fsub_rn(p.x, mx));
-        sum = __fmaf_rn(f, p.y, sum);
+        for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, red[w][0]);
+        const float f = p.y == 0.0f ? 0.0f : power<T>(__fsub_rn(p.x, mx));  // 0: saw no key
+        weight[threadIdx.x] = f;
+        float sum = f == 0.0f ? 0.0f : __fmul_rn(f, p.y);
 #pragma unroll
-        for (int c = 0; c < kDims; c++) o[c] = __fmaf_rn(f, po[(int64_t)s * D + c], o[c]);
+        for (int w = 16; w > 0; w >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, w));
+        if (lane == 0) red[warp][1] = sum;
+        __syncthreads();
+        const float al = m == mx ? 1.0f : power<T>(__fsub_rn(m, mx));
+        m = mx;
+        l = __fmul_rn(l, al);
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) l = __fadd_rn(l, red[w][1]);
+        o = make_float4(__fmul_rn(o.x, al), __fmul_rn(o.y, al), __fmul_rn(o.z, al), __fmul_rn(o.w, al));
+        for (int s = group; s < count; s += kGroups * kFlight) {
+            float4 v[kFlight];
+            float g[kFlight];
+#pragma unroll
+            for (int u = 0; u < kFlight; u++) {
+                const int at = s + u * kGroups;
+                g[u] = at < count ? weight[at] : 0.0f;
+                v[u] = at < count ? __ldg(po + (int64_t)(s0 + at) * kLanes) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int u = 0; u < kFlight; u++) {
+                if (g[u] == 0.0f) continue;
+                o.x = __fmaf_rn(g[u], v[u].x, o.x);
+                o.y = __fmaf_rn(g[u], v[u].y, o.y);
+                o.z = __fmaf_rn(g[u], v[u].z, o.z);
+                o.w = __fmaf_rn(g[u], v[u].w, o.w);
+            }
+        }
+        __syncthreads();
     }
-    T* out = (T*)a.out + token * a.out_stride + head * D + lane * kDims;
+    sums[group][d4] = o;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        float v = 0.0f;
 #pragma unroll
-    for (int c = 0; c < kDims; c++) Elem<T>::store(out + c, sum == 0.0f ? 0.0f : __fdiv_rn(o[c], sum));
+        for (int g = 0; g < kGroups; g++) v = __fadd_rn(v, reinterpret_cast<const float*>(sums[g])[threadIdx.x]);
+        Elem<T>::store((T*)a.out + token * a.out_stride + head * D + threadIdx.x, l == 0.0f ? 0.0f : __fdiv_rn(v, l));
+    }
 }
 
 // How the work is cut.
@@ -729,15 +818,15 @@ int plan(AttnArgs* a, int job_rows, int sms)
     a->o_tiles = (int)(((int64_t)a->max_q * a->group + job_rows - 1) / job_rows);
     const int64_t o_jobs = (int64_t)a->batch * a->o_tiles * hk;
     const int all_tiles = tiles(a->prefix_len) + tiles(a->max_own);
-    a->alone = all_tiles <= kAloneTiles;
+    a->alone = all_tiles <= (getenv("AL")?atoi(getenv("AL")):kAloneTiles);
     if (a->alone) {
         a->p_tiles = a->p_splits = 0;
         a->o_splits = 1;
         a->o_range = std::max(1, all_tiles);
     } else {
         a->p_tiles = (int)(((int64_t)a->tokens * a->group + job_rows - 1) / job_rows);
-        ranges((int64_t)a->p_tiles * hk, tiles(a->prefix_len), 2, &a->p_splits, &a->p_range);
-        ranges(o_jobs, tiles(a->max_own), 2, &a->o_splits, &a->o_range);
+        ranges((int64_t)a->p_tiles * hk, tiles(a->prefix_len), getenv("PS")?atoi(getenv("PS")):2, &a->p_splits, &a->p_range);
+        ranges(o_jobs, tiles(a->max_own), getenv("OS")?atoi(getenv("OS")):2, &a->o_splits, &a->o_range);
     }
     a->p_jobs = (int64_t)a->p_tiles * hk * a->p_splits;
     a->parts = a->p_splits + a->o_splits;
@@ -771,8 +860,8 @@ int launch_attention(const AttnArgs& a, cudaStream_t s)
         TMAC_CUDA_TRY(cudaGetLastError());
     }
     if (a.parts == 1) return TMAC_OK;
-    attn_join_kernel<T, D><<<(unsigned)(((int64_t)a.tokens * a.heads + 3) / 4), 128, 0, s>>>(a);
-    TMAC_CUDA_TRY(cudaGetLastError());
+    PdlScope overlap;  // the join's start overlaps the jobs' end; it waits for them before it reads
+    TMAC_CUDA_TRY(launch_k(attn_join_kernel<T, D>, dim3((unsigned)(a.tokens * a.heads)), dim3(kThreads), 0, s, a));
     return TMAC_OK;
 }
 
