@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import tmac_zynq_fpga_b200 as tm
-from tmac_zynq_fpga_b200.serving import _CacheStruct
+from tmac_zynq_fpga_b200.serving import PagedCacheStruct
 
 torch = pytest.importorskip("torch")
 
@@ -16,7 +16,7 @@ A = 0x10000  # stands for an aligned device address that is never read
 
 
 def cache(k=A, v=A, n_pages=8, type=0, kv_heads=2, page_size=16, head_dim=64, device=0):
-    return _CacheStruct(k, v, n_pages, type, kv_heads, page_size, head_dim, device)
+    return PagedCacheStruct(k, v, n_pages, type, kv_heads, page_size, head_dim, device)
 
 
 def append(c=None, **kw):
@@ -69,7 +69,8 @@ def test_append_of_no_token_is_ok():
 
 @pytest.mark.parametrize("what,code", [
     (dict(q=None), INVALID), (dict(out=None), INVALID), (dict(pages=None), INVALID), (dict(tables=None), INVALID),
-    (dict(lens=None), INVALID), (dict(work=None), INVALID), (dict(work_bytes=8), INVALID), (dict(work=A + 8), INVALID),
+    (dict(lens=None), INVALID), (dict(prefix=40000, work=None), INVALID), (dict(prefix=40000, work_bytes=8), INVALID),
+    (dict(prefix=40000, work=A + 8), INVALID),
     (dict(heads=13), SHAPE), (dict(heads=0), SHAPE), (dict(tokens=-1), SHAPE), (dict(batch=2), SHAPE), (dict(max_q=0), SHAPE),
     (dict(max_q=2), SHAPE), (dict(prefix=-1), SHAPE), (dict(max_own=-1), SHAPE), (dict(max_own=65), SHAPE), (dict(qs=64), SHAPE),
     (dict(os=64), SHAPE), (dict(batch=0, q_start=A), SHAPE), (dict(q=A + 2), INVALID)])

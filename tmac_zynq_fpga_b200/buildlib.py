@@ -1,14 +1,19 @@
 """Builds libtmac_cuda.so in-tree: every .cu under csrc/ compiled for sm_100a
 (B200) with nvcc, FMA contraction off (-fmad=false) because results must match
-the reference's fp32/fp64 roundings bit for bit."""
+the reference's fp32/fp64 roundings bit for bit.  Then _serving.so, the CPython
+module that takes torch tensors to the batched decode operators."""
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libtmac_cuda.so")
+BINDING = os.path.join(HERE, "host", "serving_binding.cpp")
+BINDING_OUT = os.path.join(HERE, "_serving.so")
+CXX = os.environ.get("CXX", "g++")
 NVCC = os.environ.get("NVCC", shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-fmad=false", "-Xcompiler", "-fPIC,-O2,-ffp-contract=off",
@@ -31,7 +36,32 @@ def up_to_date():
     return all(os.path.getmtime(d) <= t for d in deps())
 
 
+def build_binding(force=False, verbose=False):
+    """Compiles _serving.so against the installed torch (host code only)."""
+    sources = (BINDING, os.path.join(HERE, "..", "include", "tmac_cuda.h"), os.path.abspath(__file__))
+    if not force and os.path.exists(BINDING_OUT) and all(os.path.getmtime(s) <= os.path.getmtime(BINDING_OUT) for s in sources):
+        return BINDING_OUT
+    import torch
+    t = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(NVCC))), "include")
+    tmp = BINDING_OUT + ".tmp"
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", BINDING, "-o", tmp, f"-I{t}/include", f"-I{t}/include/torch/csrc/api/include",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{cuda}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f"-L{t}/lib", "-lc10", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda", f"-L{HERE}", "-l:libtmac_cuda.so", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING_OUT)
+    return BINDING_OUT
+
+
 def build(force=False, verbose=False, jobs=8):
+    out = build_library(force, verbose, jobs)
+    build_binding(force, verbose)
+    return out
+
+
+def build_library(force=False, verbose=False, jobs=8):
     if not force and up_to_date():
         return OUT
     objdir = os.path.join(HERE, "_build")

@@ -16,188 +16,11 @@
 //
 // Two kernels share this frame: 32-bit elements on the FMA units, 16-bit ones on
 // mma.sync.  Tiles come through cp.async, several in flight.
-#include "serving.cuh"
-
-#include <algorithm>
+#include "prefix_attention.cuh"
 
 namespace tmac {
 namespace {
 
-struct AttnArgs {
-    CacheDev cache;
-    const void* q;
-    int64_t q_stride;
-    void* out;
-    int64_t out_stride;
-    int heads, group, tokens, batch, max_q;
-    const int* q_start;
-    const int *prefix_pages, *prefix_lens;
-    int prefix_len;
-    const int *tables, *own_lens;
-    int table_width, max_own;
-    float scale;
-    // Jobs: prefix row tiles x kv heads x key ranges, then (sequence, row tile) x kv
-    // heads x key ranges.  Key ranges are counted in tiles of kTile keys.
-    bool alone;      // no prefix jobs: each sequence's keys are the prefix's and its own
-    int p_tiles, p_splits, p_range;
-    int o_tiles, o_splits, o_range;
-    int64_t p_jobs;
-    int parts;       // per row: p_splits + o_splits; 1: jobs write the result
-    float* part_o;   // [tokens][heads][parts][dim]
-    float2* part_ml; // [tokens][heads][parts]
-    int* err;
-};
-
-TMAC_DEV int first_token(const AttnArgs& a, int b)
-{
-    const int t = a.q_start ? a.q_start[b] : b;
-    return max(0, min(t, a.tokens));
-}
-// Query tokens of sequence b: at most max_q are computed, more is an error.
-TMAC_DEV int token_count(const AttnArgs& a, int b)
-{
-    const int n = first_token(a, b + 1) - first_token(a, b);
-    if (n > a.max_q) record_error(a.err, TMAC_ERR_BOUNDS);
-    return max(0, min(n, a.max_q));
-}
-TMAC_DEV int own_len(const AttnArgs& a, int b)
-{
-    const int n = a.own_lens[b];
-    if (n > a.max_own) record_error(a.err, TMAC_ERR_BOUNDS);
-    return max(0, min(n, a.max_own));
-}
-TMAC_DEV int prefix_seen(const AttnArgs& a, int b)
-{
-    if (!a.prefix_lens) return a.prefix_len;
-    const int n = a.prefix_lens[b];
-    if (n > a.prefix_len) record_error(a.err, TMAC_ERR_BOUNDS);
-    return max(0, min(n, a.prefix_len));
-}
-TMAC_DEV int sequence_of(const AttnArgs& a, int token)
-{
-    if (!a.q_start) return token;
-    int lo = 0, hi = a.batch - 1;  // the last sequence that starts at or before the token
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (a.q_start[mid] <= token)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    return lo;
-}
-
-// Up to so many key tiles (prefix and own) every sequence reads the prefix itself, in one job.
-constexpr int kAloneTiles = 8;
-constexpr int kTile = 64, kWarps = 4, kThreads = kWarps * 32;
-
-// A job's rows and keys, the same for every kernel.
-struct Job {
-    int kvh, seq;          // seq < 0: rows of all sequences, the prefix's keys
-    int row0, rows, token0;
-    int tile0, tile1;      // key tiles: first those of the prefix, then the own ones
-    int p_tiles;           // of the prefix within them
-    int p_keys, o_keys;    // keys in reach of the job
-    int part;
-};
-TMAC_DEV int tiles_of(int keys) { return (keys + kTile - 1) / kTile; }
-template <int kJobRows>
-TMAC_DEV bool find_job(const AttnArgs& a, Job* j)
-{
-    int64_t id = blockIdx.x;
-    if (id < a.p_jobs) {
-        const int tile = (int)(id % a.p_tiles);
-        id /= a.p_tiles;
-        j->kvh = (int)(id % a.cache.kv_heads);
-        j->part = (int)(id / a.cache.kv_heads);
-        j->seq = -1;
-        j->token0 = 0;
-        j->row0 = tile * kJobRows;
-        j->rows = min(kJobRows, a.tokens * a.group - j->row0);
-        j->p_keys = a.prefix_len;
-        j->o_keys = 0;
-        j->p_tiles = tiles_of(j->p_keys);
-        j->tile0 = j->part * a.p_range;
-        j->tile1 = min(j->p_tiles, j->tile0 + a.p_range);
-        return true;
-    }
-    id -= a.p_jobs;
-    const int tile = (int)(id % a.o_tiles);
-    id /= a.o_tiles;
-    j->kvh = (int)(id % a.cache.kv_heads);
-    id /= a.cache.kv_heads;
-    const int split = (int)(id % a.o_splits);
-    j->seq = (int)(id / a.o_splits);
-    j->part = a.p_splits + split;
-    j->token0 = first_token(a, j->seq);
-    j->row0 = tile * kJobRows;
-    j->rows = min(kJobRows, token_count(a, j->seq) * a.group - j->row0);
-    j->p_keys = a.alone ? prefix_seen(a, j->seq) : 0;
-    j->o_keys = a.max_own ? own_len(a, j->seq) : 0;
-    j->p_tiles = tiles_of(j->p_keys);
-    j->tile0 = split * a.o_range;
-    j->tile1 = min(j->p_tiles + tiles_of(j->o_keys), j->tile0 + a.o_range);
-    // without keys: the join leaves other parts out, but a lone part is the result
-    return j->rows > 0 && (j->tile1 > j->tile0 || a.parts == 1);
-}
-// The row's token and head, and how many keys of the prefix and of its own it sees.
-struct RowOf {
-    int token, head, p_limit, o_limit;
-};
-TMAC_DEV RowOf find_row(const AttnArgs& a, const Job& j, int r)
-{
-    const int row = j.row0 + r, i = row / a.group;
-    RowOf o;
-    o.token = j.token0 + i;
-    o.head = j.kvh * a.group + row % a.group;
-    if (j.seq < 0) {
-        o.p_limit = a.prefix_lens ? prefix_seen(a, sequence_of(a, o.token)) : a.prefix_len;
-        o.o_limit = 0;
-    } else {
-        o.p_limit = j.p_keys;
-        o.o_limit = max(0, j.o_keys - token_count(a, j.seq) + 1 + i);
-    }
-    return o;
-}
-// Rows of a job as the kernels keep them in shared memory.
-template <int kJobRows>
-struct Rows {
-    int token[kJobRows], head[kJobRows], p_limit[kJobRows], o_limit[kJobRows];
-    int p_least, o_least;  // smallest limits: tiles below them need no mask
-    TMAC_DEV void find(const AttnArgs& a, const Job& j)
-    {
-        if (threadIdx.x == 0) p_least = o_least = 0x7FFFFFFF;
-        __syncthreads();
-        for (int r = threadIdx.x; r < kJobRows; r += blockDim.x) {
-            RowOf o = {0, 0, 0, 0};
-            if (r < j.rows) {
-                o = find_row(a, j, r);
-                atomicMin(&p_least, o.p_limit);
-                atomicMin(&o_least, o.o_limit);
-            }
-            token[r] = o.token;
-            head[r] = o.head;
-            p_limit[r] = o.p_limit;
-            o_limit[r] = o.o_limit;
-        }
-        __syncthreads();
-    }
-};
-// Where tile t's keys lie: the page list, the first key's number in it, the keys in reach.
-struct TileOf {
-    const int* pages;
-    int key0, keys;
-    bool prefix;
-};
-TMAC_DEV TileOf find_tile(const AttnArgs& a, const Job& j, int t)
-{
-    TileOf o;
-    o.prefix = t < j.p_tiles;
-    o.pages = o.prefix ? a.prefix_pages : a.tables + (int64_t)j.seq * a.table_width;
-    o.key0 = (o.prefix ? t : t - j.p_tiles) * kTile;
-    o.keys = o.prefix ? j.p_keys : j.o_keys;
-    return o;
-}
 TMAC_DEV void cp_async16(void* dst, const void* src, bool valid)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -253,32 +76,6 @@ struct Copier {
         }
     }
 };
-// Row r's result, value d: the part's, or the rounded quotient when there is no other.
-template <typename T, int D>
-TMAC_DEV void put_result(const AttnArgs& a, const Job& j, int token, int head, int d, float m, float l, float o)
-{
-    if (a.parts == 1) {
-        Elem<T>::store((T*)a.out + token * a.out_stride + head * D + d, l == 0.0f ? 0.0f : __fdiv_rn(o, l));
-        return;
-    }
-    const int64_t at = ((int64_t)token * a.heads + head) * a.parts + j.part;
-    a.part_o[at * D + d] = o;
-    if (d == 0) a.part_ml[at] = make_float2(m, l);
-}
-// Maxima are in units of the exponential's base: e in 32 bits, where the difference
-// of two scores is formed before it is scaled; 2 in 16 bits, one multiplication less.
-TMAC_DEV float exp2_fast(float x)  // within 2^-22 relatively, tiny ones as 0
-{
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-template <typename T>
-TMAC_DEV float power(float x)
-{
-    return sizeof(T) == 4 ? expf(x) : exp2_fast(x);
-}
-
 // ---------------------------------------------------- 32-bit arithmetic ----
 // Tiles of 8 rows per warp.  A warp takes 16 keys at a time: lane = (key, half
 // of the rows) for the scores, lane = dims for the output.  With up to 8 rows
@@ -500,19 +297,8 @@ TMAC_DEV void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint3
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T>
-TMAC_DEV uint32_t pack2(float lo, float hi)
-{
-    if constexpr (std::is_same_v<T, __half>) {
-        const __half2 h = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-}
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
+TMAC_DEV void attn_mma(const AttnArgs& a)
 {
     extern __shared__ __align__(16) uint8_t smem[];
     using Smem = MmaSmem<T, D>;
@@ -725,6 +511,15 @@ again:
     }
 }
 
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
+{
+    attn_mma<T, D>(a);
+    // Where the tcgen05 kernel runs beside this one, this grid ends after it, so the
+    // join, which waits for this grid, has waited for both.
+    if (blockIdx.x == 0) pdl_wait();
+}
+
 // ------------------------------------------------------------------- join ----
 // Joins the parts of one (token, head) per CTA: groups of D / 4 threads take every
 // kGroups-th part, four values a thread, several loads in flight.
@@ -801,8 +596,9 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(AttnArgs a)
 }
 
 // How the work is cut.
-int plan(AttnArgs* a, int job_rows, int sms)
+int plan(AttnArgs* a, int type, int sms)
 {
+    const int job_rows = type == TMAC_TYPE_F32 ? kWarps * kRows : kWarps * kMmaRows;
     const int hk = a->cache.kv_heads;
     const auto tiles = [](int keys) { return (keys + kTile - 1) / kTile; };
     // key ranges so that there are about `per_sm` jobs per SM, of a tile at least
@@ -818,15 +614,24 @@ int plan(AttnArgs* a, int job_rows, int sms)
     a->o_tiles = (int)(((int64_t)a->max_q * a->group + job_rows - 1) / job_rows);
     const int64_t o_jobs = (int64_t)a->batch * a->o_tiles * hk;
     const int all_tiles = tiles(a->prefix_len) + tiles(a->max_own);
-    a->alone = all_tiles <= (getenv("AL")?atoi(getenv("AL")):kAloneTiles);
+    a->alone = all_tiles <= kAloneTiles;
     if (a->alone) {
         a->p_tiles = a->p_splits = 0;
         a->o_splits = 1;
         a->o_range = std::max(1, all_tiles);
     } else {
-        a->p_tiles = (int)(((int64_t)a->tokens * a->group + job_rows - 1) / job_rows);
-        ranges((int64_t)a->p_tiles * hk, tiles(a->prefix_len), getenv("PS")?atoi(getenv("PS")):2, &a->p_splits, &a->p_range);
-        ranges(o_jobs, tiles(a->max_own), getenv("OS")?atoi(getenv("OS")):2, &a->o_splits, &a->o_range);
+        const int64_t rows = (int64_t)a->tokens * a->group;
+        a->tc = type != TMAC_TYPE_F32 && rows >= kTcLeast && a->cache.page_shift >= 3;
+        const int p_rows = a->tc ? kTcRows : job_rows;
+        a->p_tiles = (int)((rows + p_rows - 1) / p_rows);
+        if (a->tc) {  // tiles of 128 keys
+            ranges((int64_t)a->p_tiles * hk, (a->prefix_len + 2 * kTile - 1) / (2 * kTile), a->cache.dim == 64 ? 2 : 1, &a->p_splits,
+                   &a->p_range);
+            a->p_range *= 2;
+        } else {
+            ranges((int64_t)a->p_tiles * hk, tiles(a->prefix_len), 2, &a->p_splits, &a->p_range);
+        }
+        ranges(o_jobs, tiles(a->max_own), 2, &a->o_splits, &a->o_range);
     }
     a->p_jobs = (int64_t)a->p_tiles * hk * a->p_splits;
     a->parts = a->p_splits + a->o_splits;
@@ -843,8 +648,15 @@ size_t workspace_bytes_of(const AttnArgs& a)
 template <typename T, int D>
 int launch_attention(const AttnArgs& a, cudaStream_t s)
 {
-    const int64_t jobs = a.p_jobs + (int64_t)a.batch * a.o_tiles * a.cache.kv_heads * a.o_splits;
-    if (jobs > 0x7FFFFFFF) return fail(TMAC_ERR_SHAPE, "too many jobs for one grid");
+    const int64_t o_jobs = (int64_t)a.batch * a.o_tiles * a.cache.kv_heads * a.o_splits;
+    if (a.p_jobs + o_jobs > 0x7FFFFFFF) return fail(TMAC_ERR_SHAPE, "too many jobs for one grid");
+    AttnArgs rest = a;  // without the prefix's jobs, where the tcgen05 kernel takes them
+    if (a.tc) {
+        const int rc = launch_prefix_tc(a, std::is_same_v<T, __half> ? TMAC_TYPE_F16 : TMAC_TYPE_BF16, s);
+        if (rc) return rc;
+        rest.p_jobs = 0;
+    }
+    const int64_t jobs = rest.p_jobs + o_jobs;
     if (jobs) {
         size_t smem;
         void (*fn)(AttnArgs);
@@ -855,9 +667,18 @@ int launch_attention(const AttnArgs& a, cudaStream_t s)
             fn = attn_mma_kernel<T, D>;
             smem = sizeof(MmaSmem<T, D>);
         }
-        TMAC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        fn<<<(unsigned)jobs, kThreads, smem, s>>>(a);
-        TMAC_CUDA_TRY(cudaGetLastError());
+        static std::atomic<uint64_t> done{0};
+        const int rc = set_once(done, a.device, [&] {
+            return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        });
+        if (rc) return rc;
+        if (a.tc) {  // beside the prefix's jobs
+            PdlScope beside;
+            TMAC_CUDA_TRY(launch_k(fn, dim3((unsigned)jobs), dim3(kThreads), smem, s, rest));
+        } else {
+            fn<<<(unsigned)jobs, kThreads, smem, s>>>(rest);
+            TMAC_CUDA_TRY(cudaGetLastError());
+        }
     }
     if (a.parts == 1) return TMAC_OK;
     PdlScope overlap;  // the join's start overlaps the jobs' end; it waits for them before it reads
@@ -888,7 +709,7 @@ int prepare(const tmac_paged_cache* cache, int heads, int tokens, int batch, int
     a->max_own = max_own;
     a->table_width = table_width;
     if (tokens == 0) return TMAC_OK;
-    return plan(a, cache->type == TMAC_TYPE_F32 ? kWarps * kRows : kWarps * kMmaRows, num_sms(cache->device));
+    return plan(a, cache->type, num_sms(cache->device));
 }
 
 }  // namespace
@@ -941,6 +762,7 @@ extern "C" int tmac_prefix_attention(const tmac_paged_cache* cache, const void* 
     a.tables = tables;
     a.own_lens = own_lens;
     a.scale = scale;
+    a.device = cache->device;
     a.part_o = (float*)workspace;
     a.part_ml = (float2*)(a.part_o + (size_t)tokens * heads * a.parts * cache->head_dim);
     DeviceGuard dg(cache->device);

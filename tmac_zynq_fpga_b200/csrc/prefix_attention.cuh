@@ -1,0 +1,234 @@
+// prefix_attention.cuh -- what the kernels of prefix_attention share: the arguments,
+// how the grid's jobs, rows and key tiles are found, and where results go.
+#pragma once
+
+#include "serving.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace tmac {
+
+struct AttnArgs {
+    CacheDev cache;
+    const void* q;
+    int64_t q_stride;
+    void* out;
+    int64_t out_stride;
+    int heads, group, tokens, batch, max_q;
+    const int* q_start;
+    const int *prefix_pages, *prefix_lens;
+    int prefix_len;
+    const int *tables, *own_lens;
+    int table_width, max_own;
+    float scale;
+    // Jobs: prefix row tiles x kv heads x key ranges, then (sequence, row tile) x kv
+    // heads x key ranges.  Key ranges are counted in tiles of kTile keys.
+    bool alone;      // no prefix jobs: each sequence's keys are the prefix's and its own
+    bool tc;         // the prefix jobs are the tcgen05 kernel's
+    int p_tiles, p_splits, p_range;
+    int o_tiles, o_splits, o_range;
+    int64_t p_jobs;
+    int parts;       // per row: p_splits + o_splits; 1: jobs write the result
+    float* part_o;   // [tokens][heads][parts][dim]
+    float2* part_ml; // [tokens][heads][parts]
+    int* err;
+    int device;
+};
+
+TMAC_DEV int first_token(const AttnArgs& a, int b)
+{
+    const int t = a.q_start ? a.q_start[b] : b;
+    return max(0, min(t, a.tokens));
+}
+// Query tokens of sequence b: at most max_q are computed, more is an error.
+TMAC_DEV int token_count(const AttnArgs& a, int b)
+{
+    const int n = first_token(a, b + 1) - first_token(a, b);
+    if (n > a.max_q) record_error(a.err, TMAC_ERR_BOUNDS);
+    return max(0, min(n, a.max_q));
+}
+TMAC_DEV int own_len(const AttnArgs& a, int b)
+{
+    const int n = a.own_lens[b];
+    if (n > a.max_own) record_error(a.err, TMAC_ERR_BOUNDS);
+    return max(0, min(n, a.max_own));
+}
+TMAC_DEV int prefix_seen(const AttnArgs& a, int b)
+{
+    if (!a.prefix_lens) return a.prefix_len;
+    const int n = a.prefix_lens[b];
+    if (n > a.prefix_len) record_error(a.err, TMAC_ERR_BOUNDS);
+    return max(0, min(n, a.prefix_len));
+}
+TMAC_DEV int sequence_of(const AttnArgs& a, int token)
+{
+    if (!a.q_start) return token;
+    int lo = 0, hi = a.batch - 1;  // the last sequence that starts at or before the token
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (a.q_start[mid] <= token)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
+// Up to so many key tiles (prefix and own) every sequence reads the prefix itself, in one job.
+constexpr int kAloneTiles = 8;
+// From so many query rows on the prefix goes to the tcgen05 kernel.
+constexpr int kTcLeast = 48;
+constexpr int kTile = 64, kWarps = 4, kThreads = kWarps * 32;
+
+// A job's rows and keys, the same for every kernel.
+struct Job {
+    int kvh, seq;          // seq < 0: rows of all sequences, the prefix's keys
+    int row0, rows, token0;
+    int tile0, tile1;      // key tiles: first those of the prefix, then the own ones
+    int p_tiles;           // of the prefix within them
+    int p_keys, o_keys;    // keys in reach of the job
+    int part;
+};
+TMAC_DEV int tiles_of(int keys) { return (keys + kTile - 1) / kTile; }
+template <int kJobRows>
+TMAC_DEV bool find_job(const AttnArgs& a, Job* j)
+{
+    int64_t id = blockIdx.x;
+    if (id < a.p_jobs) {
+        const int tile = (int)(id % a.p_tiles);
+        id /= a.p_tiles;
+        j->kvh = (int)(id % a.cache.kv_heads);
+        j->part = (int)(id / a.cache.kv_heads);
+        j->seq = -1;
+        j->token0 = 0;
+        j->row0 = tile * kJobRows;
+        j->rows = min(kJobRows, a.tokens * a.group - j->row0);
+        j->p_keys = a.prefix_len;
+        j->o_keys = 0;
+        j->p_tiles = tiles_of(j->p_keys);
+        j->tile0 = j->part * a.p_range;
+        j->tile1 = min(j->p_tiles, j->tile0 + a.p_range);
+        return true;
+    }
+    id -= a.p_jobs;
+    const int tile = (int)(id % a.o_tiles);
+    id /= a.o_tiles;
+    j->kvh = (int)(id % a.cache.kv_heads);
+    id /= a.cache.kv_heads;
+    const int split = (int)(id % a.o_splits);
+    j->seq = (int)(id / a.o_splits);
+    j->part = a.p_splits + split;
+    j->token0 = first_token(a, j->seq);
+    j->row0 = tile * kJobRows;
+    j->rows = min(kJobRows, token_count(a, j->seq) * a.group - j->row0);
+    j->p_keys = a.alone ? prefix_seen(a, j->seq) : 0;
+    j->o_keys = a.max_own ? own_len(a, j->seq) : 0;
+    j->p_tiles = tiles_of(j->p_keys);
+    j->tile0 = split * a.o_range;
+    j->tile1 = min(j->p_tiles + tiles_of(j->o_keys), j->tile0 + a.o_range);
+    // without keys: the join leaves other parts out, but a lone part is the result
+    return j->rows > 0 && (j->tile1 > j->tile0 || a.parts == 1);
+}
+// The row's token and head, and how many keys of the prefix and of its own it sees.
+struct RowOf {
+    int token, head, p_limit, o_limit;
+};
+TMAC_DEV RowOf find_row(const AttnArgs& a, const Job& j, int r)
+{
+    const int row = j.row0 + r, i = row / a.group;
+    RowOf o;
+    o.token = j.token0 + i;
+    o.head = j.kvh * a.group + row % a.group;
+    if (j.seq < 0) {
+        o.p_limit = a.prefix_lens ? prefix_seen(a, sequence_of(a, o.token)) : a.prefix_len;
+        o.o_limit = 0;
+    } else {
+        o.p_limit = j.p_keys;
+        o.o_limit = max(0, j.o_keys - token_count(a, j.seq) + 1 + i);
+    }
+    return o;
+}
+// Rows of a job as the kernels keep them in shared memory.
+template <int kJobRows>
+struct Rows {
+    int token[kJobRows], head[kJobRows], p_limit[kJobRows], o_limit[kJobRows];
+    int p_least, o_least;  // smallest limits: tiles below them need no mask
+    TMAC_DEV void find(const AttnArgs& a, const Job& j)
+    {
+        if (threadIdx.x == 0) p_least = o_least = 0x7FFFFFFF;
+        __syncthreads();
+        for (int r = threadIdx.x; r < kJobRows; r += blockDim.x) {
+            RowOf o = {0, 0, 0, 0};
+            if (r < j.rows) {
+                o = find_row(a, j, r);
+                atomicMin(&p_least, o.p_limit);
+                atomicMin(&o_least, o.o_limit);
+            }
+            token[r] = o.token;
+            head[r] = o.head;
+            p_limit[r] = o.p_limit;
+            o_limit[r] = o.o_limit;
+        }
+        __syncthreads();
+    }
+};
+// Where tile t's keys lie: the page list, the first key's number in it, the keys in reach.
+struct TileOf {
+    const int* pages;
+    int key0, keys;
+    bool prefix;
+};
+TMAC_DEV TileOf find_tile(const AttnArgs& a, const Job& j, int t)
+{
+    TileOf o;
+    o.prefix = t < j.p_tiles;
+    o.pages = o.prefix ? a.prefix_pages : a.tables + (int64_t)j.seq * a.table_width;
+    o.key0 = (o.prefix ? t : t - j.p_tiles) * kTile;
+    o.keys = o.prefix ? j.p_keys : j.o_keys;
+    return o;
+}
+// Row r's result, value d: the part's, or the rounded quotient when there is no other.
+template <typename T, int D>
+TMAC_DEV void put_result(const AttnArgs& a, const Job& j, int token, int head, int d, float m, float l, float o)
+{
+    if (a.parts == 1) {
+        Elem<T>::store((T*)a.out + token * a.out_stride + head * D + d, l == 0.0f ? 0.0f : __fdiv_rn(o, l));
+        return;
+    }
+    const int64_t at = ((int64_t)token * a.heads + head) * a.parts + j.part;
+    a.part_o[at * D + d] = o;
+    if (d == 0) a.part_ml[at] = make_float2(m, l);
+}
+// Maxima are in units of the exponential's base: e in 32 bits, where the difference
+// of two scores is formed before it is scaled; 2 in 16 bits, one multiplication less.
+TMAC_DEV float exp2_fast(float x)  // within 2^-22 relatively, tiny ones as 0
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <typename T>
+TMAC_DEV float power(float x)
+{
+    return sizeof(T) == 4 ? expf(x) : exp2_fast(x);
+}
+
+// 16-bit elements as pairs, the first in the low half.
+template <typename T>
+TMAC_DEV uint32_t pack2(float lo, float hi)
+{
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+// prefix_attention_tc.cu: the prefix's jobs of 16-bit elements on tcgen05.
+constexpr int kTcRows = 128;  // rows of a job
+int launch_prefix_tc(const AttnArgs& a, int type, cudaStream_t s);
+
+}  // namespace tmac

@@ -1,0 +1,439 @@
+// prefix_attention_tc.cu -- the shared prefix's part of prefix_attention on the
+// 5th-generation tensor cores, for 16-bit elements and many query rows.
+//
+// A job is 128 rows (token, head of a key/value head's group) against a range of
+// key tiles of 128.  Scores S = Q K^T are one tcgen05.mma chain per tile, both
+// operands in shared memory; four softmax warps (a thread per row) read S from
+// TMEM, keep the running maximum and sum, and store the weights P as 16-bit
+// pairs into TMEM, where they are the first operand of O += P V; V's tile is the
+// second as it lies ([keys][dims], the dims contiguous).  O stays in TMEM; it is
+// rescaled only when a row's maximum has grown by 2^8 and more, so the weights stay
+// below 2^8 and the sums keep their precision.  One thread issues the products, one
+// warp the TMA copies of the pages (a box per page, 128-byte swizzle).
+//
+// Bound: the exponentials, 128 x 128 per tile at 16 a clock against 256 clocks of
+// products at 64 dims; so two CTAs share an SM at 64 dims, and S has two buffers
+// at 128 dims, where the operands leave room for one CTA.
+#include "prefix_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace tmac {
+namespace {
+
+constexpr int kTcTile = 128, kTcThreads = 6 * 32;  // warp 0 copies, warp 1 products, warps 2-5 softmax
+constexpr int kSlab = 128 * 128;                   // bytes of 128 rows of 64 values
+constexpr float kGrow = 8.0f;                      // log2 of the growth that rescales O
+
+template <int D>
+struct Conf {
+    static constexpr int kSlabs = D / 64, kStages = 2;
+    static constexpr int kSBufs = D == 64 ? 1 : 2;
+    static constexpr int kCols = D == 64 ? 256 : 512;  // TMEM: S buffers, P, O
+    static constexpr int kP = kSBufs * 128, kO = kP + 64;
+    static constexpr int kBytes = kSlabs * kSlab;      // of a tile's keys or values, and of Q
+    static constexpr size_t kSmem = 1024 + (size_t)kBytes * (1 + 2 * kStages) + 256;
+    static_assert(kO + D <= kCols, "TMEM columns");
+};
+struct Bars {
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full, pv_done, drain;
+    uint32_t tmem;
+    int failed;
+};
+
+// Second operand of O += P V: dims contiguous, 64-dim slabs of [keys][128 bytes]
+// with the 128-byte swizzle; 8 keys (1024 bytes) apart along the product's depth.
+TMAC_DEV uint64_t desc_v(uint32_t saddr)
+{
+    uint64_t d = (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(kSlab >> 4) << 16;  // leading: the next 64 dims
+    d |= (uint64_t)(1024 >> 4) << 32;   // stride: the next 8 keys
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// kind::f16, 32-bit sums, both operands f16 (0) or bf16 (1), 128 x n; v_dims: the
+// second operand lies with its n contiguous.
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t bf16, uint32_t n, uint32_t v_dims)
+{
+    return (1u << 4) | (bf16 << 7) | (bf16 << 10) | (v_dims << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+TMAC_DEV void mma_f16(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u));
+}
+TMAC_DEV void mma_f16_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u));
+}
+#define TMAC_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define TMAC_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+TMAC_DEV void tmem_ld32(uint32_t addr, uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : TMAC_R8(r, 0), TMAC_R8(r, 8), TMAC_R8(r, 16), TMAC_R8(r, 24)
+        : "r"(addr));
+}
+TMAC_DEV void tmem_st32(uint32_t addr, const uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::TMAC_I8(r, 0),
+        TMAC_I8(r, 8), TMAC_I8(r, 16), TMAC_I8(r, 24), "r"(addr)
+        : "memory");
+}
+TMAC_DEV void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::TMAC_I8(r, 0),
+        TMAC_I8(r, 8), "r"(addr)
+        : "memory");
+}
+TMAC_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// The row's result key by key from the pools, only over the keys that it sees: for
+// jobs whose products met an infinite or NaN value, which 0 times is not 0.
+template <typename T, int D>
+TMAC_DEV void row_by_keys(const AttnArgs& a, const Job& j, const RowOf& row, int key0, int key1, float scale, float* m_out,
+                          float* l_out, float (&o)[D])
+{
+    const T* q = (const T*)a.q + row.token * a.q_stride + row.head * D;
+    float m = -INFINITY, l = 0.0f;
+    for (int d = 0; d < D; d++) o[d] = 0.0f;
+    const int shift = a.cache.page_shift;
+    for (int key = key0; key < min(key1, row.p_limit); key++) {
+        const int64_t page = a.prefix_pages[key >> shift];
+        const bool known = page >= 0 && page < a.cache.n_pages;
+        const int64_t at = (((page * a.cache.kv_heads + j.kvh) << shift) + (key & ((1 << shift) - 1))) * D;
+        float s = 0.0f;
+        for (int d = 0; d < D; d++) s = __fmaf_rn(Elem<T>::load(q + d), known ? Elem<T>::load((const T*)a.cache.k + at + d) : 0.0f, s);
+        s = __fmul_rn(s, scale);
+        const float mx = fmaxf(m, s), al = m == mx ? 1.0f : exp2_fast(__fsub_rn(m, mx));
+        const float p = s == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(s, mx));
+        l = __fmaf_rn(l, al, p);
+        for (int d = 0; d < D; d++) {
+            o[d] = __fmul_rn(o[d], al);
+            if (p != 0.0f) o[d] = __fmaf_rn(p, known ? Elem<T>::load((const T*)a.cache.v + at + d) : 0.0f, o[d]);
+        }
+        m = mx;
+    }
+    *m_out = m;
+    *l_out = l;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTcThreads, D == 64 ? 2 : 1)
+    attn_tc_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map)
+{
+    using C = Conf<D>;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + (1024 - (smem_addr(smem_raw) & 1023)) % 1024;
+    uint8_t *q_s = smem, *k_s = q_s + C::kBytes, *v_s = k_s + C::kStages * C::kBytes;
+    Bars& bar = *reinterpret_cast<Bars*>(v_s + C::kStages * C::kBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch();  // the own part may start beside this kernel
+    Job j;
+    find_job<kTcRows>(a, &j);
+    const int key0 = j.tile0 * kTile, key1 = min(j.p_keys, j.tile1 * kTile);
+    const int n_tiles = (key1 - key0 + kTcTile - 1) / kTcTile;
+
+    if (threadIdx.x == 0) {
+        mbar_init(&bar.q_full, 128);
+        for (int i = 0; i < C::kStages; i++) {
+            mbar_init(&bar.k_full[i], 1);
+            mbar_init(&bar.k_empty[i], 1);
+            mbar_init(&bar.v_full[i], 1);
+            mbar_init(&bar.v_empty[i], 1);
+        }
+        for (int i = 0; i < C::kSBufs; i++) {
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.s_empty[i], 128);
+        }
+        mbar_init(&bar.p_full, 128);
+        mbar_init(&bar.pv_done, 1);
+        mbar_init(&bar.drain, 1);
+        bar.failed = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc(&bar.tmem, C::kCols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar.tmem;
+    const auto wait = [&](uint64_t* b, int use) {  // the use-th completion (from 0) of a barrier
+        if (mbar_wait_bounded(b, (uint32_t)(use & 1), a.err)) return true;
+        *(volatile int*)&bar.failed = 1;
+        return false;
+    };
+
+    if (warp == 0) {
+        // ---- copies: a lane to a page
+        const int shift = a.cache.page_shift, page_rows = min(1 << shift, kTcTile), boxes = kTcTile / page_rows;
+        const int rows_all = (int)((a.cache.n_pages * a.cache.kv_heads) << shift);  // past the pool: reads zeros
+        int issued = 0;
+        bool ok = true;
+        for (int t = 0; t < n_tiles; t++) {
+            const int st = t % C::kStages, key = key0 + t * kTcTile;
+            const int here = min(boxes, (key1 - key + page_rows - 1) / page_rows);
+            int row = rows_all;
+            if (lane < here) {
+                const int g = key + lane * page_rows;
+                const int64_t page = a.prefix_pages[g >> shift];
+                if (page >= 0 && page < a.cache.n_pages)
+                    row = (int)((page * a.cache.kv_heads + j.kvh) << shift) + (g & ((1 << shift) - 1));
+                else
+                    record_error(a.err, TMAC_ERR_BOUNDS);
+            }
+            const auto copy = [&](uint64_t* full, uint64_t* empty, uint8_t* to, const CUtensorMap* map) {
+                if (ok && t >= C::kStages) ok = wait(empty, t / C::kStages - 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(here * page_rows * 128 * C::kSlabs));
+                __syncwarp();
+                if (lane < here)
+                    for (int h = 0; h < C::kSlabs; h++) tma_load_2d(to + h * kSlab + lane * page_rows * 128, map, h * 64, row, full);
+            };
+            copy(&bar.k_full[st], &bar.k_empty[st], k_s + st * C::kBytes, &k_map);
+            if (!ok) break;
+            issued = 2 * t + 1;
+            copy(&bar.v_full[st], &bar.v_empty[st], v_s + st * C::kBytes, &v_map);
+            if (!ok) break;
+            issued = 2 * t + 2;
+        }
+        if (*(volatile int*)&bar.failed)  // wait for the copies in flight, within the limit again
+            for (int i = max(0, issued - 2 * C::kStages); i < issued; i++)
+                mbar_wait_bounded(i & 1 ? &bar.v_full[i / 2 % C::kStages] : &bar.k_full[i / 2 % C::kStages],
+                                  (uint32_t)(i / 2 / C::kStages & 1), a.err);
+    } else if (warp == 1) {
+        // ---- products
+        if (lane == 0) {
+            constexpr uint32_t kBf16 = std::is_same_v<T, __nv_bfloat16>;
+            constexpr uint32_t kIdS = idesc_f16(kBf16, kTcTile, 0), kIdO = idesc_f16(kBf16, D, 1);
+            bool ok = wait(&bar.q_full, 0);
+            const auto scores = [&](int t) {
+                const int st = t % C::kStages, sb = t % C::kSBufs;
+                if (!ok || !(ok = wait(&bar.k_full[st], t / C::kStages))) return;
+                if (t >= C::kSBufs && !(ok = wait(&bar.s_empty[sb], t / C::kSBufs - 1))) return;
+                tc_fence_after();
+                for (int i = 0; i < D / 16; i++) {
+                    const int at = i / 4 * kSlab + i % 4 * 32;
+                    mma_f16(tmem + sb * 128, desc_sw128(smem_addr(q_s) + at), desc_sw128(smem_addr(k_s + st * C::kBytes) + at), kIdS, i > 0);
+                }
+                mma_commit(&bar.k_empty[st]);
+                mma_commit(&bar.s_full[sb]);
+            };
+            scores(0);
+            for (int t = 0; ok && t < n_tiles; t++) {
+                if (t + 1 < n_tiles) scores(t + 1);
+                const int st = t % C::kStages;
+                if (!ok || !(ok = wait(&bar.v_full[st], t / C::kStages)) || !(ok = wait(&bar.p_full, t))) break;
+                tc_fence_after();
+                for (int i = 0; i < kTcTile / 16; i++)
+                    mma_f16_tmem(tmem + C::kO, tmem + C::kP + 8 * i, desc_v(smem_addr(v_s + st * C::kBytes) + i * 16 * 128), kIdO,
+                                 t > 0 || i > 0);
+                mma_commit(&bar.v_empty[st]);
+                mma_commit(&bar.pv_done);
+            }
+            mma_commit(&bar.drain);
+            mbar_wait_bounded(&bar.drain, 0, a.err);  // nothing in flight when TMEM is freed
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: thread = row
+        const int quarter = warp & 3, r = quarter * 32 + lane;
+        const uint32_t mine = tmem + ((uint32_t)quarter << 21);  // lane quarter * 32 of TMEM
+        const bool idle = quarter * 32 >= j.rows;  // no row of this warp: its weights are not read
+        RowOf row = {0, 0, 0x7FFFFFFF, 0};
+        if (r < j.rows) row = find_row(a, j, r);
+        {
+            // a negative scale turns Q's signs, so that the largest score has the largest weight
+            const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0;
+            const T* src = (const T*)a.q + row.token * a.q_stride + row.head * D;
+            const bool aligned = ((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) % 16 == 0;
+            for (int c = 0; c < D / 8; c++) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (r < j.rows) {
+                    if (aligned) {
+                        x = __ldg(reinterpret_cast<const uint4*>(src) + c);
+                    } else {
+                        T e[8];
+                        for (int i = 0; i < 8; i++) e[i] = src[8 * c + i];
+                        x = *reinterpret_cast<const uint4*>(e);
+                    }
+                }
+                x.x ^= sign, x.y ^= sign, x.z ^= sign, x.w ^= sign;
+                *reinterpret_cast<uint4*>(q_s + c / 8 * kSlab + r * 128 + ((c & 7) ^ (r & 7)) * 16) = x;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&bar.q_full);
+        }
+        const float scale = __fmul_rn(fabsf(a.scale), 1.44269504f);  // exponentials are powers of 2
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        // V's rows past the keys hold what the page or an earlier tile holds: zeros instead
+        const auto zero_values = [&](int t) {
+            const int st = t % C::kStages;
+            if (!__all_sync(0xffffffffu, wait(&bar.v_full[st], t / C::kStages))) return false;
+            if (r >= key1 - (key0 + t * kTcTile))
+                for (int h = 0; h < C::kSlabs; h++)
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        *reinterpret_cast<uint4*>(v_s + st * C::kBytes + h * kSlab + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            return true;
+        };
+        for (int t = 0; t < n_tiles; t++) {
+            const int sb = t % C::kSBufs, key = key0 + t * kTcTile, seen = min(row.p_limit, key1) - key;
+            const uint32_t s_at = mine + sb * 128;
+            ok = __all_sync(0xffffffffu, wait(&bar.s_full[sb], t / C::kSBufs));
+            if (!ok) break;
+            tc_fence_after();
+            if (idle) {
+                if (t > 0 && !(ok = __all_sync(0xffffffffu, wait(&bar.pv_done, t - 1)))) break;
+                mbar_arrive(&bar.s_empty[sb]);
+                if (key1 - key < kTcTile && !(ok = zero_values(t))) break;
+                mbar_arrive(&bar.p_full);
+                continue;
+            }
+            const bool masked = __any_sync(0xffffffffu, seen < kTcTile);
+            uint32_t x[32];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                tmem_ld32(s_at + 32 * c, x);
+                tmem_wait_ld();
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (32 * c + i < seen) mx = fmaxf(mx, __uint_as_float(x[i]));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(x[i]));
+                }
+            }
+            mx = __fmul_rn(mx, scale);
+            // the last tile's weights must have been read before they are written anew,
+            // and its sums be complete before they are rescaled
+            if (t > 0) {
+                ok = __all_sync(0xffffffffu, wait(&bar.pv_done, t - 1));
+                if (!ok) break;
+                tc_fence_after();
+            }
+            const bool grown = mx > m + kGrow || (m == -INFINITY && mx > m);
+            if (__any_sync(0xffffffffu, grown)) {
+                const float al = grown ? exp2_fast(__fsub_rn(m, mx)) : 1.0f;
+                if (grown) m = mx;
+                l = __fmul_rn(l, al);
+                if (t > 0) {
+#pragma unroll
+                    for (int c = 0; c < D / 32; c++) {
+                        tmem_ld32(mine + C::kO + 32 * c, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[i] = __float_as_uint(__fmul_rn(__uint_as_float(x[i]), al));
+                        tmem_st32(mine + C::kO + 32 * c, x);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.0f : -m;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                tmem_ld32(s_at + 32 * c, x);
+                tmem_wait_ld();
+                uint32_t p[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float p0 = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * i]), scale, base));
+                    float p1 = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * i + 1]), scale, base));
+                    if (masked) {
+                        if (32 * c + 2 * i >= seen) p0 = 0.0f;
+                        if (32 * c + 2 * i + 1 >= seen) p1 = 0.0f;
+                    }
+                    sum[i & 3] = __fadd_rn(sum[i & 3], __fadd_rn(p0, p1));
+                    p[i] = pack2<T>(p0, p1);
+                }
+                tmem_st16(mine + C::kP + 16 * c, p);
+            }
+            tc_fence_before();
+            mbar_arrive(&bar.s_empty[sb]);
+            l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+            if (key1 - key < kTcTile && !(ok = zero_values(t))) break;
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&bar.p_full);
+        }
+        if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, wait(&bar.pv_done, n_tiles - 1));
+        if (ok && !idle) {
+            tc_fence_after();
+            bool finite = true;
+            float o[D];
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                uint32_t x[32];
+                tmem_ld32(mine + C::kO + 32 * c, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    o[32 * c + i] = __uint_as_float(x[i]);
+                    finite &= fabsf(o[32 * c + i]) < INFINITY;
+                }
+            }
+            if (r < j.rows) {
+                if (!finite && row.p_limit < key1) row_by_keys<T, D>(a, j, row, key0, key1, __fmul_rn(a.scale, 1.44269504f), &m, &l, o);
+                if (l == 0.0f)
+                    for (int d = 0; d < D; d++) o[d] = 0.0f;
+#pragma unroll
+                for (int d = 0; d < D; d++) put_result<T, D>(a, j, row.token, row.head, d, m, l, o[d]);
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, C::kCols);
+}
+
+template <typename T, int D>
+int launch_tc(const AttnArgs& a, cudaStream_t s)
+{
+    using C = Conf<D>;
+    auto encode = encode_fn();
+    if (!encode) return fail(TMAC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const int page_rows = std::min(1 << a.cache.page_shift, kTcTile);
+    CUtensorMap maps[2];
+    for (int i = 0; i < 2; i++) {
+        const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)(a.cache.n_pages * a.cache.kv_heads) << a.cache.page_shift};
+        const cuuint64_t strides[1] = {D * sizeof(T)};
+        const cuuint32_t box[2] = {64, (cuuint32_t)page_rows}, elem[2] = {1, 1};
+        const auto type = std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        if (encode(&maps[i], type, 2, i ? a.cache.v : a.cache.k, dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return fail(TMAC_ERR_CUDA, "cuTensorMapEncodeTiled failed for the cache's pages");
+    }
+    static std::atomic<uint64_t> done{0};
+    const int rc = set_once(done, a.device, [&] {
+        return cudaFuncSetAttribute(attn_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem);
+    });
+    if (rc) return rc;
+    attn_tc_kernel<T, D><<<(unsigned)a.p_jobs, kTcThreads, C::kSmem, s>>>(a, maps[0], maps[1]);
+    TMAC_CUDA_TRY(cudaGetLastError());
+    return TMAC_OK;
+}
+
+}  // namespace
+
+int launch_prefix_tc(const AttnArgs& a, int type, cudaStream_t s)
+{
+    if (type == TMAC_TYPE_F16) return a.cache.dim == 64 ? launch_tc<__half, 64>(a, s) : launch_tc<__half, 128>(a, s);
+    return a.cache.dim == 64 ? launch_tc<__nv_bfloat16, 64>(a, s) : launch_tc<__nv_bfloat16, 128>(a, s);
+}
+
+}  // namespace tmac

@@ -848,12 +848,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
 }
 
 template <typename T, bool kResident>
-int launch_sample(const SampleArgs& a, int batch, int ranks, cudaStream_t s)
+int launch_sample(const SampleArgs& a, int batch, int ranks, int device, cudaStream_t s)
 {
     const size_t smem = list_bytes<kResident>() + (kResident ? ((size_t)a.slice + 6) * sizeof(float) : 0);
     auto fn = sample_kernel<T, kResident>;
-    TMAC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    TMAC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    static std::atomic<uint64_t> done{0};
+    const int rc = set_once(done, device, [&] {
+        const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        return e ? e : cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    });
+    if (rc) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(batch * ranks));
     cfg.blockDim = dim3(kThreads);
@@ -909,7 +913,7 @@ extern "C" int tmac_sample(const void* logits, int type, int64_t row_stride, int
     if (!dg.ok) return fail(TMAC_ERR_NODEV, "no such CUDA device");
     return with_type(type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        return resident ? launch_sample<T, true>(a, batch, ranks, (cudaStream_t)stream)
-                        : launch_sample<T, false>(a, batch, ranks, (cudaStream_t)stream);
+        return resident ? launch_sample<T, true>(a, batch, ranks, device, (cudaStream_t)stream)
+                        : launch_sample<T, false>(a, batch, ranks, device, (cudaStream_t)stream);
     });
 }

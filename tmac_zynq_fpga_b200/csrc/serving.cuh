@@ -10,6 +10,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 namespace tmac {
 
 constexpr int kMaxPage = 256;
@@ -58,6 +60,17 @@ struct CacheDev {
 };
 
 TMAC_DEV void record_error(int* err, int code) { atomicExch(err, code); }
+
+// Kernel attributes are set once per kernel and device: `done` has a bit for each device.
+template <typename F>
+int set_once(std::atomic<uint64_t>& done, int device, F&& set)
+{
+    const uint64_t bit = 1ull << (device & 63);
+    if (done.load(std::memory_order_acquire) & bit) return TMAC_OK;
+    TMAC_CUDA_TRY(set());
+    done.fetch_or(bit, std::memory_order_release);
+    return TMAC_OK;
+}
 
 // Host-side checks, none of which touches a device.
 inline int check_cache(const tmac_paged_cache* c, CacheDev* out)

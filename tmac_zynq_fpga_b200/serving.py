@@ -12,7 +12,6 @@ one given (a torch stream or a raw address), else torch's current stream.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -25,7 +24,7 @@ _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 
 
-class _CacheStruct(ctypes.Structure):
+class PagedCacheStruct(ctypes.Structure):
     """tmac_paged_cache"""
     _fields_ = [("k", _P), ("v", _P), ("n_pages", _I64), ("type", _INT), ("kv_heads", _INT), ("page_size", _INT),
                 ("head_dim", _INT), ("device", _INT)]
@@ -40,26 +39,21 @@ SIGNATURES = {
     "tmac_sample": (_INT, [_P, _INT, _I64, _INT, _INT, _P, _P, _P, _P, _P, _P, _P, _INT, _P]),
 }
 
-_types = None
+_native = None
 
 
-def _type_of(dtype):
-    global _types
-    if _types is None:
-        import torch
-        _types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: BF16}
-    return _types.get(dtype, -1)
+def _ext():
+    """The module that checks tensors and calls the library (host/serving_binding.cpp)."""
+    global _native
+    if _native is None:
+        import torch  # noqa: F401  (the module needs its libraries loaded)
 
-
-def _lib():
-    import tmac_zynq_fpga_b200 as tm
-    return tm.lib()
-
-
-def _check(rc):
-    if rc:
         import tmac_zynq_fpga_b200 as tm
-        tm.check(rc)
+        tm.lib()
+        from . import _serving
+        _serving.set_error_class(tm.TmacError)
+        _native = _serving
+    return _native
 
 
 def _refuse(code, msg):
@@ -67,34 +61,12 @@ def _refuse(code, msg):
     raise tm.TmacError(code, msg)
 
 
-def _stream(stream, device):
-    """(context that makes the stream torch's current one, its address)."""
+def _on(stream, device):
+    """The context in which `stream`, a torch stream or an address, is torch's current one."""
     import torch
-    if stream is None:
-        return None, torch.cuda.current_stream(device).cuda_stream
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
-    return torch.cuda.stream(stream), stream.cuda_stream
-
-
-def _vector(name, t, dtype, shape, device):
-    """The address of a contiguous tensor of that type and shape, or of None."""
-    if t is None:
-        return None
-    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
-        _refuse(-1, f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, "
-                    f"not {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
-
-
-def _heads(name, t, dim, device):
-    """Checks [tokens, heads, head_dim] with adjoining heads; the token stride."""
-    if t.dim() != 3 or t.shape[2] != dim:
-        _refuse(-3, f"{name} must be [tokens, heads, {dim}], not {tuple(t.shape)}")
-    s = t.stride()
-    if t.device != device or (s[2] != 1 and dim > 1) or (s[1] != dim and t.shape[1] > 1):
-        _refuse(-1, f"{name} must lie on {device} with the heads of a token adjoining")
-    return s[0] if t.shape[0] > 1 else t.shape[1] * dim
+    return torch.cuda.stream(stream)
 
 
 class PagedCache:
@@ -103,19 +75,11 @@ class PagedCache:
     power of two up to 256.  The tensors stay the caller's: which pages belong to which
     sequence is in the tables given to each call."""
 
+    __slots__ = ("k", "v")
+
     def __init__(self, k, v):
-        if k.dim() != 4 or k.shape != v.shape:
-            _refuse(-3, f"k and v must both be [n_pages, kv_heads, page_size, head_dim], not {tuple(k.shape)} and {tuple(v.shape)}")
-        code = _type_of(k.dtype)
-        if code < 0 or v.dtype != k.dtype:
-            _refuse(-2, f"k and v must both be float32, float16 or bfloat16, not {k.dtype} and {v.dtype}")
-        if not k.is_cuda or v.device != k.device or not k.is_contiguous() or not v.is_contiguous():
-            _refuse(-1, "k and v must be contiguous tensors on one CUDA device")
-        self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
-        self.n_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
-        self._struct = _CacheStruct(k.data_ptr(), v.data_ptr(), self.n_pages, code, self.kv_heads, self.page_size,
-                                    self.head_dim, k.device.index)
-        self._ref = ctypes.addressof(self._struct)
+        (_native or _ext()).check_cache(k, v)
+        self.k, self.v = k, v
 
 
 def rope_table(max_pos, rot_dim, theta=1e6, factor=1.0, original=None, low=1.0, high=32.0, scale=1.0, device="cuda"):
@@ -150,30 +114,11 @@ def rope_append(cache, q, k, v, pos, tables, cos, sin, *, seq=None, starts=None,
     distance between tokens; pos, seq int32 [tokens]; tables int32 [n_seq, width]; starts
     int32 [n_seq]; cos, sin float32 [max_pos, rot_dim / 2] (`rope_table`); bias float32
     [(heads + 2 kv_heads) * head_dim].  See tmac_rope_append for the places they name."""
-    import torch
-    dev, dim = cache.device, cache.head_dim
-    code = _type_of(q.dtype)
-    if code < 0 or k.dtype != q.dtype or v.dtype != q.dtype:
-        _refuse(-2, "q, k and v must be of one type: float32, float16 or bfloat16")
-    qs, ks, vs = _heads("q", q, dim, dev), _heads("k", k, dim, dev), _heads("v", v, dim, dev)
-    n, heads = q.shape[0], q.shape[1]
-    if k.shape != v.shape or k.shape[0] != n or k.shape[1] != cache.kv_heads:
-        _refuse(-3, f"k and v must be [{n}, {cache.kv_heads}, {dim}], not {tuple(k.shape)} and {tuple(v.shape)}")
-    if tables.dim() != 2 or cos.dim() != 2:
-        _refuse(-3, "tables must be [n_seq, width] and cos [max_pos, rot_dim / 2]")
-    i32, f32 = torch.int32, torch.float32
-    n_seq, width = tables.shape
-    args = (_vector("bias", bias, f32, ((heads + 2 * cache.kv_heads) * dim,), dev), _vector("seq", seq, i32, (n,), dev),
-            _vector("pos", pos, i32, (n,), dev), _vector("starts", starts, i32, (n_seq,), dev),
-            _vector("tables", tables, i32, tables.shape, dev), n_seq, width, _vector("cos", cos, f32, cos.shape, dev),
-            _vector("sin", sin, f32, cos.shape, dev), cos.shape[0], 2 * cos.shape[1], 1 if interleaved else 0)
-    ctx, s = _stream(stream, dev)
-    with ctx or contextlib.nullcontext():
-        if q_out is None:
-            q_out = torch.empty((n, heads, dim), dtype=cache.dtype, device=dev)
-        _check(_lib().tmac_rope_append(cache._ref, code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, heads, n,
-                                       *args, _vector("q_out", q_out, cache.dtype, (n, heads, dim), dev), s))
-    return q_out
+    if stream is not None:
+        with _on(stream, cache.k.device):
+            return rope_append(cache, q, k, v, pos, tables, cos, sin, seq=seq, starts=starts, interleaved=interleaved, bias=bias,
+                               q_out=q_out)
+    return (_native or _ext()).rope_append(cache.k, cache.v, q, k, v, pos, tables, cos, sin, seq, starts, interleaved, bias, q_out)
 
 
 def prefix_attention(q, cache, tables, own_lens, *, prefix_pages=None, prefix_len=0, prefix_lens=None, q_start=None, max_q=1,
@@ -187,39 +132,12 @@ def prefix_attention(q, cache, tables, own_lens, *, prefix_pages=None, prefix_le
     prefix_lens int32 [batch]: how much of them each sequence sees (all).  q_start int32
     [batch + 1] with max_q: several query tokens per sequence, each seeing the keys up to
     its own; without it one per sequence.  See tmac_prefix_attention."""
-    import torch
-    dev, dim = cache.device, cache.head_dim
-    if q.dtype != cache.dtype:
-        _refuse(-2, f"q must have the cache's type {cache.dtype}, not {q.dtype}")
-    qs = _heads("q", q, dim, dev)
-    n, heads = q.shape[0], q.shape[1]
-    if tables.dim() != 2:
-        _refuse(-3, "tables must be [batch, width]")
-    batch, width = tables.shape
-    if max_own is None:
-        max_own = width * cache.page_size
-    if prefix_pages is not None and prefix_len > prefix_pages.numel() * cache.page_size:
-        _refuse(-3, "prefix_pages do not cover prefix_len")
-    i32 = torch.int32
-    own = _vector("own_lens", own_lens, i32, (batch,), dev)
-    table = _vector("tables", tables, i32, tables.shape, dev)
-    pages = None if prefix_pages is None else _vector("prefix_pages", prefix_pages, i32, (prefix_pages.numel(),), dev)
-    shared = _vector("prefix_lens", prefix_lens, i32, (batch,), dev)
-    starts = _vector("q_start", q_start, i32, (batch + 1,), dev)
-    L = _lib()
-    need = ctypes.c_size_t()
-    _check(L.tmac_prefix_attention_workspace(cache._ref, heads, n, batch, max_q, prefix_len, max_own, ctypes.addressof(need)))
-    ctx, s = _stream(stream, dev)
-    with ctx or contextlib.nullcontext():
-        if out is None:
-            out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
-        elif out.dtype != q.dtype or out.shape != q.shape:
-            _refuse(-1, "out must have q's type and shape")
-        work = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        _check(L.tmac_prefix_attention(cache._ref, q.data_ptr(), qs, heads, n, batch, starts, max_q, pages, prefix_len,
-                                       shared, table, width, own, max_own, dim ** -0.5 if scale is None else scale,
-                                       out.data_ptr(), _heads("out", out, dim, dev), work.data_ptr(), need.value, s))
-    return out
+    if stream is not None:
+        with _on(stream, cache.k.device):
+            return prefix_attention(q, cache, tables, own_lens, prefix_pages=prefix_pages, prefix_len=prefix_len,
+                                    prefix_lens=prefix_lens, q_start=q_start, max_q=max_q, max_own=max_own, scale=scale, out=out)
+    return (_native or _ext()).prefix_attention(q, cache.k, cache.v, tables, own_lens, prefix_pages, prefix_len, prefix_lens, q_start,
+                                                max_q, max_own, scale, out)
 
 
 def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
@@ -227,23 +145,7 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, s
     distance between rows) and its probability among the kept tokens: int32 [batch],
     float32 [batch].  u float32 [batch] in [0, 1); temperature, top_p, min_p float32
     [batch], top_k int32 [batch], each optional.  See tmac_sample for the filters."""
-    import torch
-    code = _type_of(logits.dtype)
-    if code < 0:
-        _refuse(-2, f"logits must be float32, float16 or bfloat16, not {logits.dtype}")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        _refuse(-3, "logits must be [batch, vocab] with adjoining values")
-    if not logits.is_cuda:
-        _refuse(-1, "logits must lie on a CUDA device")
-    dev, (n, vocab) = logits.device, logits.shape
-    f32, shape = torch.float32, (n,)
-    args = (_vector("u", u, f32, shape, dev), _vector("temperature", temperature, f32, shape, dev),
-            _vector("top_k", top_k, torch.int32, shape, dev), _vector("top_p", top_p, f32, shape, dev),
-            _vector("min_p", min_p, f32, shape, dev))
-    ctx, s = _stream(stream, dev)
-    with ctx or contextlib.nullcontext():
-        tokens = torch.empty(n, dtype=torch.int32, device=dev)
-        probs = torch.empty(n, dtype=f32, device=dev)
-        _check(_lib().tmac_sample(logits.data_ptr(), code, logits.stride(0) if n > 1 else vocab, n, vocab, *args,
-                                  tokens.data_ptr(), probs.data_ptr(), dev.index, s))
-    return tokens, probs
+    if stream is not None:
+        with _on(stream, logits.device):
+            return sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    return (_native or _ext()).sample(logits, u, temperature, top_k, top_p, min_p)
