@@ -624,13 +624,7 @@ int plan(AttnArgs* a, int type, int sms)
         a->tc = type != TMAC_TYPE_F32 && rows >= kTcLeast && a->cache.page_shift >= 3;
         const int p_rows = a->tc ? kTcRows : job_rows;
         a->p_tiles = (int)((rows + p_rows - 1) / p_rows);
-        if (a->tc) {  // tiles of 128 keys
-            ranges((int64_t)a->p_tiles * hk, (a->prefix_len + 2 * kTile - 1) / (2 * kTile), a->cache.dim == 64 ? 2 : 1, &a->p_splits,
-                   &a->p_range);
-            a->p_range *= 2;
-        } else {
-            ranges((int64_t)a->p_tiles * hk, tiles(a->prefix_len), 2, &a->p_splits, &a->p_range);
-        }
+        ranges((int64_t)a->p_tiles * hk, tiles(a->prefix_len), 2, &a->p_splits, &a->p_range);
         ranges(o_jobs, tiles(a->max_own), 2, &a->o_splits, &a->o_range);
     }
     a->p_jobs = (int64_t)a->p_tiles * hk * a->p_splits;

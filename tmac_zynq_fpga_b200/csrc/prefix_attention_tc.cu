@@ -2,40 +2,39 @@
 // 5th-generation tensor cores, for 16-bit elements and many query rows.
 //
 // A job is 128 rows (token, head of a key/value head's group) against a range of
-// key tiles of 128.  Scores S = Q K^T are one tcgen05.mma chain per tile, both
+// key tiles of 64.  Scores S = Q K^T are one tcgen05.mma chain per tile, both
 // operands in shared memory; four softmax warps (a thread per row) read S from
 // TMEM, keep the running maximum and sum, and store the weights P as 16-bit
-// pairs into TMEM, where they are the first operand of O += P V; V's tile is the
-// second as it lies ([keys][dims], the dims contiguous).  O stays in TMEM; it is
+// pairs over S, where they are the first operand of O += P V; V's tile is the
+// second as it lies ([keys][dims], the dims contiguous).  S has two buffers, so the
+// next tile's scores are ready when a tile's weights are.  O stays in TMEM; it is
 // rescaled only when a row's maximum has grown by 2^8 and more, so the weights stay
 // below 2^8 and the sums keep their precision.  One thread issues the products, one
 // warp the TMA copies of the pages (a box per page, 128-byte swizzle).
 //
-// Bound: the exponentials, 128 x 128 per tile at 16 a clock against 256 clocks of
-// products at 64 dims; so two CTAs share an SM at 64 dims, and S has two buffers
-// at 128 dims, where the operands leave room for one CTA.
+// Bound: the exponentials, 128 x 64 per tile at 16 a clock, 512 clocks against 128
+// of products at 64 dims.  Two CTAs share an SM: one's waits are the other's work.
 #include "prefix_attention.cuh"
 #include "tcgen05.cuh"
 
 namespace tmac {
 namespace {
 
-constexpr int kTcTile = 128, kTcThreads = 6 * 32;  // warp 0 copies, warp 1 products, warps 2-5 softmax
-constexpr int kSlab = 128 * 128;                   // bytes of 128 rows of 64 values
-constexpr float kGrow = 8.0f;                      // log2 of the growth that rescales O
+constexpr int kTcThreads = 6 * 32;  // warp 0 copies, warp 1 products, warps 2-5 softmax
+constexpr int kSlab = kTile * 128;   // bytes of a tile's keys (or values) in 64 dims
+constexpr int kQSlab = kTcRows * 128;
+constexpr float kGrow = 8.0f;        // log2 of the growth that rescales O
+constexpr uint32_t kTmemCols = 256;  // S and P: two buffers of 64, then O
 
 template <int D>
 struct Conf {
-    static constexpr int kSlabs = D / 64, kStages = 2;
-    static constexpr int kSBufs = D == 64 ? 1 : 2;
-    static constexpr int kCols = D == 64 ? 256 : 512;  // TMEM: S buffers, P, O
-    static constexpr int kP = kSBufs * 128, kO = kP + 64;
-    static constexpr int kBytes = kSlabs * kSlab;      // of a tile's keys or values, and of Q
-    static constexpr size_t kSmem = 1024 + (size_t)kBytes * (1 + 2 * kStages) + 256;
-    static_assert(kO + D <= kCols, "TMEM columns");
+    static constexpr int kSlabs = D / 64, kStages = D == 64 ? 4 : 2;
+    static constexpr int kBytes = kSlabs * kSlab, kQBytes = kSlabs * kQSlab;
+    static constexpr size_t kSmem = 1024 + (size_t)kQBytes + 2 * kStages * kBytes + 256;
 };
+constexpr uint32_t kOCol = 128;
 struct Bars {
-    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_empty[2], p_full, pv_done, drain;
+    uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done, drain;
     uint32_t tmem;
     int failed;
 };
@@ -72,6 +71,7 @@ TMAC_DEV void mma_f16_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_
         "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u));
 }
 #define TMAC_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define TMAC_RW8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
 #define TMAC_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
 TMAC_DEV void tmem_ld32(uint32_t addr, uint32_t (&r)[32])
 {
@@ -81,6 +81,14 @@ TMAC_DEV void tmem_ld32(uint32_t addr, uint32_t (&r)[32])
         : TMAC_R8(r, 0), TMAC_R8(r, 8), TMAC_R8(r, 16), TMAC_R8(r, 24)
         : "r"(addr));
 }
+// Waits for this thread's loads; their registers pass through, so no use moves before it.
+TMAC_DEV void tmem_wait_ld32(uint32_t (&r)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : TMAC_RW8(r, 0), TMAC_RW8(r, 8), TMAC_RW8(r, 16), TMAC_RW8(r, 24)
+                 :
+                 : "memory");
+}
 TMAC_DEV void tmem_st32(uint32_t addr, const uint32_t (&r)[32])
 {
     asm volatile(
@@ -89,23 +97,32 @@ TMAC_DEV void tmem_st32(uint32_t addr, const uint32_t (&r)[32])
         TMAC_I8(r, 8), TMAC_I8(r, 16), TMAC_I8(r, 24), "r"(addr)
         : "memory");
 }
-TMAC_DEV void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
-{
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::TMAC_I8(r, 0),
-        TMAC_I8(r, 8), "r"(addr)
-        : "memory");
-}
 TMAC_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 values of a row's sums from dim d on.
+template <typename T, int D>
+TMAC_DEV void put_row_of(const AttnArgs& a, const Job& j, const RowOf& row, int d, float m, float l, const uint32_t (&x)[32])
+{
+    if (a.parts == 1) {
+#pragma unroll
+        for (int i = 0; i < 32; i++) put_result<T, D>(a, j, row.token, row.head, d + i, m, l, __uint_as_float(x[i]));
+        return;
+    }
+    const int64_t at = ((int64_t)row.token * a.heads + row.head) * a.parts + j.part;
+    const uint32_t keep = l == 0.0f ? 0u : ~0u;  // saw no key: zeros
+    uint4* to = reinterpret_cast<uint4*>(a.part_o + at * D + d);
+#pragma unroll
+    for (int i = 0; i < 8; i++) to[i] = make_uint4(x[4 * i] & keep, x[4 * i + 1] & keep, x[4 * i + 2] & keep, x[4 * i + 3] & keep);
+    if (d == 0) a.part_ml[at] = make_float2(m, l);
+}
 
 // The row's result key by key from the pools, only over the keys that it sees: for
 // jobs whose products met an infinite or NaN value, which 0 times is not 0.
 template <typename T, int D>
-TMAC_DEV void row_by_keys(const AttnArgs& a, const Job& j, const RowOf& row, int key0, int key1, float scale, float* m_out,
-                          float* l_out, float (&o)[D])
+__device__ __noinline__ void row_by_keys(const AttnArgs& a, const Job& j, const RowOf& row, int key0, int key1, float scale)
 {
     const T* q = (const T*)a.q + row.token * a.q_stride + row.head * D;
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f, o[D];
     for (int d = 0; d < D; d++) o[d] = 0.0f;
     const int shift = a.cache.page_shift;
     for (int key = key0; key < min(key1, row.p_limit); key++) {
@@ -124,25 +141,24 @@ TMAC_DEV void row_by_keys(const AttnArgs& a, const Job& j, const RowOf& row, int
         }
         m = mx;
     }
-    *m_out = m;
-    *l_out = l;
+    for (int d = 0; d < D; d++) put_result<T, D>(a, j, row.token, row.head, d, m, l, o[d]);
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kTcThreads, D == 64 ? 2 : 1)
+__global__ void __launch_bounds__(kTcThreads, 2)
     attn_tc_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map)
 {
     using C = Conf<D>;
     extern __shared__ __align__(16) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + (1024 - (smem_addr(smem_raw) & 1023)) % 1024;
-    uint8_t *q_s = smem, *k_s = q_s + C::kBytes, *v_s = k_s + C::kStages * C::kBytes;
+    uint8_t *q_s = smem, *k_s = q_s + C::kQBytes, *v_s = k_s + C::kStages * C::kBytes;
     Bars& bar = *reinterpret_cast<Bars*>(v_s + C::kStages * C::kBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch();  // the own part may start beside this kernel
     Job j;
     find_job<kTcRows>(a, &j);
     const int key0 = j.tile0 * kTile, key1 = min(j.p_keys, j.tile1 * kTile);
-    const int n_tiles = (key1 - key0 + kTcTile - 1) / kTcTile;
+    const int n_tiles = tiles_of(key1 - key0);
 
     if (threadIdx.x == 0) {
         mbar_init(&bar.q_full, 128);
@@ -152,17 +168,16 @@ __global__ void __launch_bounds__(kTcThreads, D == 64 ? 2 : 1)
             mbar_init(&bar.v_full[i], 1);
             mbar_init(&bar.v_empty[i], 1);
         }
-        for (int i = 0; i < C::kSBufs; i++) {
+        for (int i = 0; i < 2; i++) {
             mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.s_empty[i], 128);
+            mbar_init(&bar.p_full[i], 128);
         }
-        mbar_init(&bar.p_full, 128);
         mbar_init(&bar.pv_done, 1);
         mbar_init(&bar.drain, 1);
         bar.failed = 0;
         fence_mbar_init();
     }
-    if (warp == 1) tmem_alloc(&bar.tmem, C::kCols);
+    if (warp == 1) tmem_alloc(&bar.tmem, kTmemCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -175,12 +190,12 @@ __global__ void __launch_bounds__(kTcThreads, D == 64 ? 2 : 1)
 
     if (warp == 0) {
         // ---- copies: a lane to a page
-        const int shift = a.cache.page_shift, page_rows = min(1 << shift, kTcTile), boxes = kTcTile / page_rows;
+        const int shift = a.cache.page_shift, page_rows = min(1 << shift, kTile), boxes = kTile / page_rows;
         const int rows_all = (int)((a.cache.n_pages * a.cache.kv_heads) << shift);  // past the pool: reads zeros
         int issued = 0;
         bool ok = true;
         for (int t = 0; t < n_tiles; t++) {
-            const int st = t % C::kStages, key = key0 + t * kTcTile;
+            const int st = t % C::kStages, key = key0 + t * kTile;
             const int here = min(boxes, (key1 - key + page_rows - 1) / page_rows);
             int row = rows_all;
             if (lane < here) {
@@ -215,31 +230,34 @@ __global__ void __launch_bounds__(kTcThreads, D == 64 ? 2 : 1)
         // ---- products
         if (lane == 0) {
             constexpr uint32_t kBf16 = std::is_same_v<T, __nv_bfloat16>;
-            constexpr uint32_t kIdS = idesc_f16(kBf16, kTcTile, 0), kIdO = idesc_f16(kBf16, D, 1);
+            constexpr uint32_t kIdS = idesc_f16(kBf16, kTile, 0), kIdO = idesc_f16(kBf16, D, 1);
             bool ok = wait(&bar.q_full, 0);
             const auto scores = [&](int t) {
-                const int st = t % C::kStages, sb = t % C::kSBufs;
+                const int st = t % C::kStages;
                 if (!ok || !(ok = wait(&bar.k_full[st], t / C::kStages))) return;
-                if (t >= C::kSBufs && !(ok = wait(&bar.s_empty[sb], t / C::kSBufs - 1))) return;
+                // P of tile t - 2, in the same place, has been read
+                if (t >= 2 && !(ok = wait(&bar.pv_done, t - 2))) return;
                 tc_fence_after();
-                for (int i = 0; i < D / 16; i++) {
-                    const int at = i / 4 * kSlab + i % 4 * 32;
-                    mma_f16(tmem + sb * 128, desc_sw128(smem_addr(q_s) + at), desc_sw128(smem_addr(k_s + st * C::kBytes) + at), kIdS, i > 0);
-                }
+#pragma unroll
+                for (int i = 0; i < D / 16; i++)
+                    mma_f16(tmem + t % 2 * 64, desc_sw128(smem_addr(q_s) + i / 4 * kQSlab + i % 4 * 32),
+                            desc_sw128(smem_addr(k_s + st * C::kBytes) + i / 4 * kSlab + i % 4 * 32), kIdS, i > 0);
                 mma_commit(&bar.k_empty[st]);
-                mma_commit(&bar.s_full[sb]);
+                mma_commit(&bar.s_full[t % 2]);
             };
             scores(0);
+            if (n_tiles > 1) scores(1);
             for (int t = 0; ok && t < n_tiles; t++) {
-                if (t + 1 < n_tiles) scores(t + 1);
                 const int st = t % C::kStages;
-                if (!ok || !(ok = wait(&bar.v_full[st], t / C::kStages)) || !(ok = wait(&bar.p_full, t))) break;
+                if (!(ok = wait(&bar.v_full[st], t / C::kStages)) || !(ok = wait(&bar.p_full[t % 2], t / 2))) break;
                 tc_fence_after();
-                for (int i = 0; i < kTcTile / 16; i++)
-                    mma_f16_tmem(tmem + C::kO, tmem + C::kP + 8 * i, desc_v(smem_addr(v_s + st * C::kBytes) + i * 16 * 128), kIdO,
+#pragma unroll
+                for (int i = 0; i < kTile / 16; i++)
+                    mma_f16_tmem(tmem + kOCol, tmem + t % 2 * 64 + 8 * i, desc_v(smem_addr(v_s + st * C::kBytes) + i * 16 * 128), kIdO,
                                  t > 0 || i > 0);
                 mma_commit(&bar.v_empty[st]);
                 mma_commit(&bar.pv_done);
+                if (t + 2 < n_tiles) scores(t + 2);
             }
             mma_commit(&bar.drain);
             mbar_wait_bounded(&bar.drain, 0, a.err);  // nothing in flight when TMEM is freed
@@ -257,20 +275,24 @@ __global__ void __launch_bounds__(kTcThreads, D == 64 ? 2 : 1)
             const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0;
             const T* src = (const T*)a.q + row.token * a.q_stride + row.head * D;
             const bool aligned = ((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) % 16 == 0;
+            uint4 x[D / 8];
+#pragma unroll
             for (int c = 0; c < D / 8; c++) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (r < j.rows) {
-                    if (aligned) {
-                        x = __ldg(reinterpret_cast<const uint4*>(src) + c);
-                    } else {
-                        T e[8];
-                        for (int i = 0; i < 8; i++) e[i] = src[8 * c + i];
-                        x = *reinterpret_cast<const uint4*>(e);
-                    }
+                x[c] = make_uint4(0, 0, 0, 0);
+                if (r >= j.rows) continue;
+                if (aligned) {
+                    x[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+                } else {
+                    T e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) e[i] = src[8 * c + i];
+                    x[c] = *reinterpret_cast<const uint4*>(e);
                 }
-                x.x ^= sign, x.y ^= sign, x.z ^= sign, x.w ^= sign;
-                *reinterpret_cast<uint4*>(q_s + c / 8 * kSlab + r * 128 + ((c & 7) ^ (r & 7)) * 16) = x;
             }
+#pragma unroll
+            for (int c = 0; c < D / 8; c++)
+                *reinterpret_cast<uint4*>(q_s + c / 8 * kQSlab + r * 128 + ((c & 7) ^ (r & 7)) * 16) =
+                    make_uint4(x[c].x ^ sign, x[c].y ^ sign, x[c].z ^ sign, x[c].w ^ sign);
             fence_proxy_async_smem();
             mbar_arrive(&bar.q_full);
         }
@@ -281,7 +303,7 @@ __global__ void __launch_bounds__(kTcThreads, D == 64 ? 2 : 1)
         const auto zero_values = [&](int t) {
             const int st = t % C::kStages;
             if (!__all_sync(0xffffffffu, wait(&bar.v_full[st], t / C::kStages))) return false;
-            if (r >= key1 - (key0 + t * kTcTile))
+            if (r < kTile && r >= key1 - (key0 + t * kTile))
                 for (int h = 0; h < C::kSlabs; h++)
 #pragma unroll
                     for (int c = 0; c < 8; c++)
@@ -290,115 +312,88 @@ __global__ void __launch_bounds__(kTcThreads, D == 64 ? 2 : 1)
             return true;
         };
         for (int t = 0; t < n_tiles; t++) {
-            const int sb = t % C::kSBufs, key = key0 + t * kTcTile, seen = min(row.p_limit, key1) - key;
-            const uint32_t s_at = mine + sb * 128;
-            ok = __all_sync(0xffffffffu, wait(&bar.s_full[sb], t / C::kSBufs));
-            if (!ok) break;
+            const int key = key0 + t * kTile, seen = min(row.p_limit, key1) - key;
+            const uint32_t s_at = mine + t % 2 * 64;
+            if (!(ok = __all_sync(0xffffffffu, wait(&bar.s_full[t % 2], t / 2)))) break;
             tc_fence_after();
-            if (idle) {
-                if (t > 0 && !(ok = __all_sync(0xffffffffu, wait(&bar.pv_done, t - 1)))) break;
-                mbar_arrive(&bar.s_empty[sb]);
-                if (key1 - key < kTcTile && !(ok = zero_values(t))) break;
-                mbar_arrive(&bar.p_full);
-                continue;
-            }
-            const bool masked = __any_sync(0xffffffffu, seen < kTcTile);
-            uint32_t x[32];
-            float mx = -INFINITY;
+            if (!idle) {
+                uint32_t x[2][32];
+                tmem_ld32(s_at, x[0]);
+                tmem_ld32(s_at + 32, x[1]);
+                tmem_wait_ld32(x[0]);
+                tmem_wait_ld32(x[1]);
+                const bool masked = __any_sync(0xffffffffu, seen < kTile);
+                if (masked)
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tmem_ld32(s_at + 32 * c, x);
-                tmem_wait_ld();
-                if (masked) {
+                    for (int c = 0; c < 64; c++)
+                        if (c >= seen) x[c / 32][c % 32] = 0xFF800000u;  // -inf
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (32 * c + i < seen) mx = fmaxf(mx, __uint_as_float(x[i]));
-                } else {
+                for (int c = 0; c < 64; c++) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(x[c / 32][c % 32]));
+                const float mx = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), scale);
+                const bool grown = mx > m + kGrow || (m == -INFINITY && mx > m);
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float al = grown ? exp2_fast(__fsub_rn(m, mx)) : 1.0f;
+                    if (grown) m = mx;
+                    l = __fmul_rn(l, al);
+                    if (t > 0) {  // the sums so far must be complete
+                        if (!(ok = __all_sync(0xffffffffu, wait(&bar.pv_done, t - 1)))) break;
+                        tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(x[i]));
-                }
-            }
-            mx = __fmul_rn(mx, scale);
-            // the last tile's weights must have been read before they are written anew,
-            // and its sums be complete before they are rescaled
-            if (t > 0) {
-                ok = __all_sync(0xffffffffu, wait(&bar.pv_done, t - 1));
-                if (!ok) break;
-                tc_fence_after();
-            }
-            const bool grown = mx > m + kGrow || (m == -INFINITY && mx > m);
-            if (__any_sync(0xffffffffu, grown)) {
-                const float al = grown ? exp2_fast(__fsub_rn(m, mx)) : 1.0f;
-                if (grown) m = mx;
-                l = __fmul_rn(l, al);
-                if (t > 0) {
+                        for (int c = 0; c < D / 32; c++) {
+                            uint32_t y[32];
+                            tmem_ld32(mine + kOCol + 32 * c, y);
+                            tmem_wait_ld32(y);
 #pragma unroll
-                    for (int c = 0; c < D / 32; c++) {
-                        tmem_ld32(mine + C::kO + 32 * c, x);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) x[i] = __float_as_uint(__fmul_rn(__uint_as_float(x[i]), al));
-                        tmem_st32(mine + C::kO + 32 * c, x);
+                            for (int i = 0; i < 32; i++) y[i] = __float_as_uint(__fmul_rn(__uint_as_float(y[i]), al));
+                            tmem_st32(mine + kOCol + 32 * c, y);
+                        }
                     }
                 }
-            }
-            const float base = m == -INFINITY ? 0.0f : -m;
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float base = m == -INFINITY ? 0.0f : -m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t p[32];
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                tmem_ld32(s_at + 32 * c, x);
-                tmem_wait_ld();
-                uint32_t p[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float p0 = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * i]), scale, base));
-                    float p1 = exp2_fast(__fmaf_rn(__uint_as_float(x[2 * i + 1]), scale, base));
+                for (int i = 0; i < 32; i++) {
+                    float p0 = exp2_fast(__fmaf_rn(__uint_as_float(x[i / 16][2 * i % 32]), scale, base));
+                    float p1 = exp2_fast(__fmaf_rn(__uint_as_float(x[i / 16][2 * i % 32 + 1]), scale, base));
                     if (masked) {
-                        if (32 * c + 2 * i >= seen) p0 = 0.0f;
-                        if (32 * c + 2 * i + 1 >= seen) p1 = 0.0f;
+                        if (2 * i >= seen) p0 = 0.0f;
+                        if (2 * i + 1 >= seen) p1 = 0.0f;
                     }
                     sum[i & 3] = __fadd_rn(sum[i & 3], __fadd_rn(p0, p1));
                     p[i] = pack2<T>(p0, p1);
                 }
-                tmem_st16(mine + C::kP + 16 * c, p);
+                tmem_st32(s_at, p);
+                l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
             }
-            tc_fence_before();
-            mbar_arrive(&bar.s_empty[sb]);
-            l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
-            if (key1 - key < kTcTile && !(ok = zero_values(t))) break;
+            if (key1 - key < kTile && !(ok = zero_values(t))) break;
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&bar.p_full);
+            mbar_arrive(&bar.p_full[t % 2]);
         }
-        if (ok && n_tiles > 0) ok = __all_sync(0xffffffffu, wait(&bar.pv_done, n_tiles - 1));
+        // One after the other: a wait by parity takes a barrier two uses behind for complete.
+        for (int t = max(0, n_tiles - 2); ok && t < n_tiles; t++) ok = __all_sync(0xffffffffu, wait(&bar.pv_done, t));
         if (ok && !idle) {
             tc_fence_after();
             bool finite = true;
-            float o[D];
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
                 uint32_t x[32];
-                tmem_ld32(mine + C::kO + 32 * c, x);
-                tmem_wait_ld();
+                tmem_ld32(mine + kOCol + 32 * c, x);
+                tmem_wait_ld32(x);
 #pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    o[32 * c + i] = __uint_as_float(x[i]);
-                    finite &= fabsf(o[32 * c + i]) < INFINITY;
-                }
+                for (int i = 0; i < 32; i++) finite &= fabsf(__uint_as_float(x[i])) < INFINITY;
+                if (r < j.rows) put_row_of<T, D>(a, j, row, 32 * c, m, l, x);
             }
-            if (r < j.rows) {
-                if (!finite && row.p_limit < key1) row_by_keys<T, D>(a, j, row, key0, key1, __fmul_rn(a.scale, 1.44269504f), &m, &l, o);
-                if (l == 0.0f)
-                    for (int d = 0; d < D; d++) o[d] = 0.0f;
-#pragma unroll
-                for (int d = 0; d < D; d++) put_result<T, D>(a, j, row.token, row.head, d, m, l, o[d]);
-            }
+            if (r < j.rows && !finite && row.p_limit < key1)
+                row_by_keys<T, D>(a, j, row, key0, key1, __fmul_rn(a.scale, 1.44269504f));
         }
         tc_fence_before();
     }
     __syncthreads();
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem, C::kCols);
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
 }
 
 template <typename T, int D>
@@ -407,7 +402,7 @@ int launch_tc(const AttnArgs& a, cudaStream_t s)
     using C = Conf<D>;
     auto encode = encode_fn();
     if (!encode) return fail(TMAC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    const int page_rows = std::min(1 << a.cache.page_shift, kTcTile);
+    const int page_rows = std::min(1 << a.cache.page_shift, kTile);
     CUtensorMap maps[2];
     for (int i = 0; i < 2; i++) {
         const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)(a.cache.n_pages * a.cache.kv_heads) << a.cache.page_shift};
