@@ -94,12 +94,13 @@ TMAC_DEV int tiles_of(int keys) { return (keys + kTile - 1) / kTile; }
 template <int kJobRows>
 TMAC_DEV bool find_job(const AttnArgs& a, Job* j)
 {
-    int64_t id = blockIdx.x;
-    if (id < a.p_jobs) {
-        const int tile = (int)(id % a.p_tiles);
-        id /= a.p_tiles;
-        j->kvh = (int)(id % a.cache.kv_heads);
-        j->part = (int)(id / a.cache.kv_heads);
+    uint32_t id = blockIdx.x;  // below 2^31; 32-bit divisions
+    const uint32_t hk = (uint32_t)a.cache.kv_heads;
+    if (id < (uint32_t)a.p_jobs) {
+        const int tile = (int)(id % (uint32_t)a.p_tiles);
+        id /= (uint32_t)a.p_tiles;
+        j->kvh = (int)(id % hk);
+        j->part = (int)(id / hk);
         j->seq = -1;
         j->token0 = 0;
         j->row0 = tile * kJobRows;
@@ -111,13 +112,13 @@ TMAC_DEV bool find_job(const AttnArgs& a, Job* j)
         j->tile1 = min(j->p_tiles, j->tile0 + a.p_range);
         return true;
     }
-    id -= a.p_jobs;
-    const int tile = (int)(id % a.o_tiles);
-    id /= a.o_tiles;
-    j->kvh = (int)(id % a.cache.kv_heads);
-    id /= a.cache.kv_heads;
-    const int split = (int)(id % a.o_splits);
-    j->seq = (int)(id / a.o_splits);
+    id -= (uint32_t)a.p_jobs;
+    const int tile = (int)(id % (uint32_t)a.o_tiles);
+    id /= (uint32_t)a.o_tiles;
+    j->kvh = (int)(id % hk);
+    id /= hk;
+    const int split = (int)(id % (uint32_t)a.o_splits);
+    j->seq = (int)(id / (uint32_t)a.o_splits);
     j->part = a.p_splits + split;
     j->token0 = first_token(a, j->seq);
     j->row0 = tile * kJobRows;

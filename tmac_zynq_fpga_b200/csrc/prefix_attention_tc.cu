@@ -5,9 +5,10 @@
 // key tiles of 64.  Scores S = Q K^T are one tcgen05.mma chain per tile, both
 // operands in shared memory; four softmax warps (a thread per row) read S from
 // TMEM, keep the running maximum and sum, and store the weights P as 16-bit
-// pairs over S, where they are the first operand of O += P V; V's tile is the
-// second as it lies ([keys][dims], the dims contiguous).  S has two buffers, so the
-// next tile's scores are ready when a tile's weights are.  O stays in TMEM; it is
+// pairs into TMEM, where they are the first operand of O += P V; V's tile is the
+// second as it lies ([keys][dims], the dims contiguous).  A row's scores are in its
+// thread's registers before their weights are formed, so the next tile's product
+// runs beneath them; P has two buffers.  O stays in TMEM; it is
 // rescaled only when a row's maximum has grown by 2^8 and more, so the weights stay
 // below 2^8 and the sums keep their precision.  One thread issues the products, one
 // warp the TMA copies of the pages (a box per page, 128-byte swizzle).
@@ -24,7 +25,7 @@ constexpr int kTcThreads = 6 * 32;  // warp 0 copies, warp 1 products, warps 2-5
 constexpr int kSlab = kTile * 128;   // bytes of a tile's keys (or values) in 64 dims
 constexpr int kQSlab = kTcRows * 128;
 constexpr float kGrow = 8.0f;        // log2 of the growth that rescales O
-constexpr uint32_t kTmemCols = 256;  // S and P: two buffers of 64, then O
+constexpr uint32_t kTmemCols = 256, kPCol = 64, kOCol = 128;  // S at 0, two buffers of P, O
 
 template <int D>
 struct Conf {
@@ -32,9 +33,8 @@ struct Conf {
     static constexpr int kBytes = kSlabs * kSlab, kQBytes = kSlabs * kQSlab;
     static constexpr size_t kSmem = 1024 + (size_t)kQBytes + 2 * kStages * kBytes + 256;
 };
-constexpr uint32_t kOCol = 128;
 struct Bars {
-    uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2], p_full[2], pv_done, drain;
+    uint64_t q_full, k_full[4], k_empty[4], v_full[4], v_empty[4], s_full, s_empty, p_full[2], pv_done[2], drain;
     uint32_t tmem;
     int failed;
 };
@@ -168,11 +168,12 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             mbar_init(&bar.v_full[i], 1);
             mbar_init(&bar.v_empty[i], 1);
         }
+        mbar_init(&bar.s_full, 1);
+        mbar_init(&bar.s_empty, 128);
         for (int i = 0; i < 2; i++) {
-            mbar_init(&bar.s_full[i], 1);
             mbar_init(&bar.p_full[i], 128);
+            mbar_init(&bar.pv_done[i], 1);
         }
-        mbar_init(&bar.pv_done, 1);
         mbar_init(&bar.drain, 1);
         bar.failed = 0;
         fence_mbar_init();
@@ -182,7 +183,9 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bar.tmem;
-    const auto wait = [&](uint64_t* b, int use) {  // the use-th completion (from 0) of a barrier
+    // The use-th completion (from 0) of a barrier.  By parity: at the time of the wait the
+    // barrier must have seen use or use + 1 of them, which is why some come in pairs.
+    const auto wait = [&](uint64_t* b, int use) {
         if (mbar_wait_bounded(b, (uint32_t)(use & 1), a.err)) return true;
         *(volatile int*)&bar.failed = 1;
         return false;
@@ -235,29 +238,27 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             const auto scores = [&](int t) {
                 const int st = t % C::kStages;
                 if (!ok || !(ok = wait(&bar.k_full[st], t / C::kStages))) return;
-                // P of tile t - 2, in the same place, has been read
-                if (t >= 2 && !(ok = wait(&bar.pv_done, t - 2))) return;
+                if (t >= 1 && !(ok = wait(&bar.s_empty, t - 1))) return;
                 tc_fence_after();
 #pragma unroll
                 for (int i = 0; i < D / 16; i++)
-                    mma_f16(tmem + t % 2 * 64, desc_sw128(smem_addr(q_s) + i / 4 * kQSlab + i % 4 * 32),
+                    mma_f16(tmem, desc_sw128(smem_addr(q_s) + i / 4 * kQSlab + i % 4 * 32),
                             desc_sw128(smem_addr(k_s + st * C::kBytes) + i / 4 * kSlab + i % 4 * 32), kIdS, i > 0);
                 mma_commit(&bar.k_empty[st]);
-                mma_commit(&bar.s_full[t % 2]);
+                mma_commit(&bar.s_full);
             };
             scores(0);
-            if (n_tiles > 1) scores(1);
             for (int t = 0; ok && t < n_tiles; t++) {
+                if (t + 1 < n_tiles) scores(t + 1);
                 const int st = t % C::kStages;
-                if (!(ok = wait(&bar.v_full[st], t / C::kStages)) || !(ok = wait(&bar.p_full[t % 2], t / 2))) break;
+                if (!ok || !(ok = wait(&bar.v_full[st], t / C::kStages)) || !(ok = wait(&bar.p_full[t % 2], t / 2))) break;
                 tc_fence_after();
 #pragma unroll
                 for (int i = 0; i < kTile / 16; i++)
-                    mma_f16_tmem(tmem + kOCol, tmem + t % 2 * 64 + 8 * i, desc_v(smem_addr(v_s + st * C::kBytes) + i * 16 * 128), kIdO,
-                                 t > 0 || i > 0);
+                    mma_f16_tmem(tmem + kOCol, tmem + kPCol + t % 2 * 32 + 8 * i, desc_v(smem_addr(v_s + st * C::kBytes) + i * 16 * 128),
+                                 kIdO, t > 0 || i > 0);
                 mma_commit(&bar.v_empty[st]);
-                mma_commit(&bar.pv_done);
-                if (t + 2 < n_tiles) scores(t + 2);
+                mma_commit(&bar.pv_done[t % 2]);
             }
             mma_commit(&bar.drain);
             mbar_wait_bounded(&bar.drain, 0, a.err);  // nothing in flight when TMEM is freed
@@ -313,15 +314,19 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         };
         for (int t = 0; t < n_tiles; t++) {
             const int key = key0 + t * kTile, seen = min(row.p_limit, key1) - key;
-            const uint32_t s_at = mine + t % 2 * 64;
-            if (!(ok = __all_sync(0xffffffffu, wait(&bar.s_full[t % 2], t / 2)))) break;
+            if (!(ok = __all_sync(0xffffffffu, wait(&bar.s_full, t)))) break;
             tc_fence_after();
-            if (!idle) {
+            if (idle) {
+                mbar_arrive(&bar.s_empty);
+                if (t > 1 && !(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[t % 2], t / 2 - 1)))) break;
+            } else {
                 uint32_t x[2][32];
-                tmem_ld32(s_at, x[0]);
-                tmem_ld32(s_at + 32, x[1]);
+                tmem_ld32(mine, x[0]);
+                tmem_ld32(mine + 32, x[1]);
                 tmem_wait_ld32(x[0]);
                 tmem_wait_ld32(x[1]);
+                tc_fence_before();
+                mbar_arrive(&bar.s_empty);
                 const bool masked = __any_sync(0xffffffffu, seen < kTile);
                 if (masked)
 #pragma unroll
@@ -331,13 +336,15 @@ __global__ void __launch_bounds__(kTcThreads, 2)
 #pragma unroll
                 for (int c = 0; c < 64; c++) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(x[c / 32][c % 32]));
                 const float mx = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), scale);
+                // this buffer's last weights have been read
+                if (t > 1 && !(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[t % 2], t / 2 - 1)))) break;
                 const bool grown = mx > m + kGrow || (m == -INFINITY && mx > m);
                 if (__any_sync(0xffffffffu, grown)) {
                     const float al = grown ? exp2_fast(__fsub_rn(m, mx)) : 1.0f;
                     if (grown) m = mx;
                     l = __fmul_rn(l, al);
                     if (t > 0) {  // the sums so far must be complete
-                        if (!(ok = __all_sync(0xffffffffu, wait(&bar.pv_done, t - 1)))) break;
+                        if (!(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[(t - 1) % 2], (t - 1) / 2)))) break;
                         tc_fence_after();
 #pragma unroll
                         for (int c = 0; c < D / 32; c++) {
@@ -364,7 +371,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                     sum[i & 3] = __fadd_rn(sum[i & 3], __fadd_rn(p0, p1));
                     p[i] = pack2<T>(p0, p1);
                 }
-                tmem_st32(s_at, p);
+                tmem_st32(mine + kPCol + t % 2 * 32, p);
                 l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
             }
             if (key1 - key < kTile && !(ok = zero_values(t))) break;
@@ -372,8 +379,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             tc_fence_before();
             mbar_arrive(&bar.p_full[t % 2]);
         }
-        // One after the other: a wait by parity takes a barrier two uses behind for complete.
-        for (int t = max(0, n_tiles - 2); ok && t < n_tiles; t++) ok = __all_sync(0xffffffffu, wait(&bar.pv_done, t));
+        for (int t = max(0, n_tiles - 2); ok && t < n_tiles; t++) ok = __all_sync(0xffffffffu, wait(&bar.pv_done[t % 2], t / 2));
         if (ok && !idle) {
             tc_fence_after();
             bool finite = true;
