@@ -8,10 +8,14 @@
 // pairs into TMEM, where they are the first operand of O += P V; V's tile is the
 // second as it lies ([keys][dims], the dims contiguous).  A row's scores are in its
 // thread's registers before their weights are formed, so the next tile's product
-// runs beneath them; P has two buffers.  O stays in TMEM; it is
-// rescaled only when a row's maximum has grown by 2^8 and more, so the weights stay
-// below 2^8 and the sums keep their precision.  One thread issues the products, one
-// warp the TMA copies of the pages (a box per page, 128-byte swizzle).
+// runs beneath them; P has two buffers.  O stays in TMEM.
+//
+// A weight is 2^(s - m) with m the largest score of the row's first tile, kept as
+// long as no tile's sum of weights passes a limit (2^8 in f16, which ends at 2^16;
+// 2^30 in bf16): a product and a rounding do not lose precision by a common factor.
+// Only a tile that passes it pays for a new maximum, the rescaling of O, and its
+// weights anew.  One thread issues the products, one warp the TMA copies of the pages
+// (a box per page, 128-byte swizzle).
 //
 // Bound: the exponentials, 128 x 64 per tile at 16 a clock, 512 clocks against 128
 // of products at 64 dims.  Two CTAs share an SM: one's waits are the other's work.
@@ -24,7 +28,6 @@ namespace {
 constexpr int kTcThreads = 6 * 32;  // warp 0 copies, warp 1 products, warps 2-5 softmax
 constexpr int kSlab = kTile * 128;   // bytes of a tile's keys (or values) in 64 dims
 constexpr int kQSlab = kTcRows * 128;
-constexpr float kGrow = 8.0f;        // log2 of the growth that rescales O
 constexpr uint32_t kTmemCols = 256, kPCol = 64, kOCol = 128;  // S at 0, two buffers of P, O
 
 template <int D>
@@ -97,7 +100,62 @@ TMAC_DEV void tmem_st32(uint32_t addr, const uint32_t (&r)[32])
         TMAC_I8(r, 8), TMAC_I8(r, 16), TMAC_I8(r, 24), "r"(addr)
         : "memory");
 }
+TMAC_DEV void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::TMAC_I8(r, 0),
+        TMAC_I8(r, 8), "r"(addr)
+        : "memory");
+}
 TMAC_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two 32-bit floats at once.
+struct Two {
+    uint64_t v;
+    TMAC_DEV Two(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+    TMAC_DEV explicit Two(uint64_t x) : v(x) {}
+    TMAC_DEV float lo() const { float a, b; asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); return a; }
+    TMAC_DEV float hi() const { float a, b; asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); return b; }
+};
+TMAC_DEV Two fma2(Two a, Two b, Two c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return Two(d);
+}
+TMAC_DEV Two add2(Two a, Two b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
+    return Two(d);
+}
+// The weights 2^(x scale - m) of 32 scores, as pairs; kMasked: those from `seen` on
+// are 0.  Returns their sum.
+template <typename T, bool kMasked>
+TMAC_DEV float weights(const uint32_t (&x)[32], float scale, float m, int seen, uint32_t (&p)[16])
+{
+    const float base = m == -INFINITY ? 0.0f : -m;
+    const Two scale2(scale, scale), base2(base, base);
+    Two sum[2] = {Two(0.0f, 0.0f), Two(0.0f, 0.0f)};
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const Two e = fma2(Two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, base2);
+        float p0 = exp2_fast(e.lo()), p1 = exp2_fast(e.hi());
+        if (kMasked) {
+            if (2 * i >= seen) p0 = 0.0f;
+            if (2 * i + 1 >= seen) p1 = 0.0f;
+        }
+        sum[i & 1] = add2(sum[i & 1], Two(p0, p1));
+        p[i] = pack2<T>(p0, p1);
+    }
+    const Two all = add2(sum[0], sum[1]);
+    return __fadd_rn(all.lo(), all.hi());
+}
+template <typename T>
+TMAC_DEV float weights(const uint32_t (&x)[32], float scale, float m, bool masked, int seen, uint32_t (&p)[16])
+{
+    return masked ? weights<T, true>(x, scale, m, seen, p) : weights<T, false>(x, scale, m, seen, p);
+}
 
 // 32 values of a row's sums from dim d on.
 template <typename T, int D>
@@ -159,6 +217,29 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     find_job<kTcRows>(a, &j);
     const int key0 = j.tile0 * kTile, key1 = min(j.p_keys, j.tile1 * kTile);
     const int n_tiles = tiles_of(key1 - key0);
+
+    // the softmax threads' rows of Q, on their way while the rest is set up
+    const int quarter = warp & 3, r = quarter * 32 + lane;
+    RowOf row = {0, 0, 0x7FFFFFFF, 0};
+    uint4 q[D / 8];
+    if (warp >= 2) {
+        if (r < j.rows) row = find_row(a, j, r);
+        const T* src = (const T*)a.q + row.token * a.q_stride + row.head * D;
+        const bool aligned = ((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) % 16 == 0;
+#pragma unroll
+        for (int c = 0; c < D / 8; c++) {
+            q[c] = make_uint4(0, 0, 0, 0);
+            if (r >= j.rows) continue;
+            if (aligned) {
+                q[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+            } else {
+                T e[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) e[i] = src[8 * c + i];
+                q[c] = *reinterpret_cast<const uint4*>(e);
+            }
+        }
+    }
 
     if (threadIdx.x == 0) {
         mbar_init(&bar.q_full, 128);
@@ -266,38 +347,20 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         __syncwarp();
     } else {
         // ---- softmax: thread = row
-        const int quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t mine = tmem + ((uint32_t)quarter << 21);  // lane quarter * 32 of TMEM
         const bool idle = quarter * 32 >= j.rows;  // no row of this warp: its weights are not read
-        RowOf row = {0, 0, 0x7FFFFFFF, 0};
-        if (r < j.rows) row = find_row(a, j, r);
         {
             // a negative scale turns Q's signs, so that the largest score has the largest weight
             const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0;
-            const T* src = (const T*)a.q + row.token * a.q_stride + row.head * D;
-            const bool aligned = ((uintptr_t)a.q | (uintptr_t)(a.q_stride * sizeof(T))) % 16 == 0;
-            uint4 x[D / 8];
-#pragma unroll
-            for (int c = 0; c < D / 8; c++) {
-                x[c] = make_uint4(0, 0, 0, 0);
-                if (r >= j.rows) continue;
-                if (aligned) {
-                    x[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
-                } else {
-                    T e[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) e[i] = src[8 * c + i];
-                    x[c] = *reinterpret_cast<const uint4*>(e);
-                }
-            }
 #pragma unroll
             for (int c = 0; c < D / 8; c++)
                 *reinterpret_cast<uint4*>(q_s + c / 8 * kQSlab + r * 128 + ((c & 7) ^ (r & 7)) * 16) =
-                    make_uint4(x[c].x ^ sign, x[c].y ^ sign, x[c].z ^ sign, x[c].w ^ sign);
+                    make_uint4(q[c].x ^ sign, q[c].y ^ sign, q[c].z ^ sign, q[c].w ^ sign);
             fence_proxy_async_smem();
             mbar_arrive(&bar.q_full);
         }
         const float scale = __fmul_rn(fabsf(a.scale), 1.44269504f);  // exponentials are powers of 2
+        constexpr float kLimit = std::is_same_v<T, __half> ? 256.0f : 1073741824.0f;
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         // V's rows past the keys hold what the page or an earlier tile holds: zeros instead
@@ -320,28 +383,35 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                 mbar_arrive(&bar.s_empty);
                 if (t > 1 && !(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[t % 2], t / 2 - 1)))) break;
             } else {
-                uint32_t x[2][32];
+                uint32_t x[2][32], p[2][16];
                 tmem_ld32(mine, x[0]);
-                tmem_ld32(mine + 32, x[1]);
                 tmem_wait_ld32(x[0]);
-                tmem_wait_ld32(x[1]);
+                tmem_ld32(mine + 32, x[1]);
+                const bool masked = __any_sync(0xffffffffu, seen < kTile);
+                bool fits = m > -INFINITY;
+                float sum = 0.0f;
+                if (__all_sync(0xffffffffu, fits)) {
+                    sum = weights<T>(x[0], scale, m, masked, seen, p[0]);
+                    tmem_wait_ld32(x[1]);
+                    sum = __fadd_rn(sum, weights<T>(x[1], scale, m, masked, seen - 32, p[1]));
+                    fits = !(sum > kLimit);
+                } else {
+                    tmem_wait_ld32(x[1]);
+                    fits = false;
+                }
                 tc_fence_before();
                 mbar_arrive(&bar.s_empty);
-                const bool masked = __any_sync(0xffffffffu, seen < kTile);
-                if (masked)
-#pragma unroll
-                    for (int c = 0; c < 64; c++)
-                        if (c >= seen) x[c / 32][c % 32] = 0xFF800000u;  // -inf
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 64; c++) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(x[c / 32][c % 32]));
-                const float mx = __fmul_rn(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), scale);
                 // this buffer's last weights have been read
                 if (t > 1 && !(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[t % 2], t / 2 - 1)))) break;
-                const bool grown = mx > m + kGrow || (m == -INFINITY && mx > m);
-                if (__any_sync(0xffffffffu, grown)) {
-                    const float al = grown ? exp2_fast(__fsub_rn(m, mx)) : 1.0f;
-                    if (grown) m = mx;
+                if (__any_sync(0xffffffffu, !fits)) {
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 64; c++)
+                        if (!masked || c < seen) mx = fmaxf(mx, __uint_as_float(x[c / 32][c % 32]));
+                    mx = fmaxf(m, __fmul_rn(mx, scale));
+                    if (fits) mx = m;
+                    const float al = mx == m ? 1.0f : exp2_fast(__fsub_rn(m, mx));
+                    m = mx;
                     l = __fmul_rn(l, al);
                     if (t > 0) {  // the sums so far must be complete
                         if (!(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[(t - 1) % 2], (t - 1) / 2)))) break;
@@ -356,23 +426,11 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                             tmem_st32(mine + kOCol + 32 * c, y);
                         }
                     }
+                    sum = __fadd_rn(weights<T>(x[0], scale, m, masked, seen, p[0]), weights<T>(x[1], scale, m, masked, seen - 32, p[1]));
                 }
-                const float base = m == -INFINITY ? 0.0f : -m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t p[32];
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    float p0 = exp2_fast(__fmaf_rn(__uint_as_float(x[i / 16][2 * i % 32]), scale, base));
-                    float p1 = exp2_fast(__fmaf_rn(__uint_as_float(x[i / 16][2 * i % 32 + 1]), scale, base));
-                    if (masked) {
-                        if (2 * i >= seen) p0 = 0.0f;
-                        if (2 * i + 1 >= seen) p1 = 0.0f;
-                    }
-                    sum[i & 3] = __fadd_rn(sum[i & 3], __fadd_rn(p0, p1));
-                    p[i] = pack2<T>(p0, p1);
-                }
-                tmem_st32(mine + kPCol + t % 2 * 32, p);
-                l = __fadd_rn(l, __fadd_rn(__fadd_rn(sum[0], sum[1]), __fadd_rn(sum[2], sum[3])));
+                tmem_st16(mine + kPCol + t % 2 * 32, p[0]);
+                tmem_st16(mine + kPCol + t % 2 * 32 + 16, p[1]);
+                l = __fadd_rn(l, sum);
             }
             if (key1 - key < kTile && !(ok = zero_values(t))) break;
             tmem_wait_st();
