@@ -10,9 +10,11 @@
 // cache's type.
 //
 // Bound: HBM, every value is read once and written once.  Where the pointers,
-// strides and head parts allow it a thread takes 8 adjoining values (16 bytes of a
-// 16-bit type), or 8 pairs of halves, so a warp moves whole lines; other layouts
-// take one pair per thread.
+// strides and head parts allow it a warp takes a token, its threads 8 adjoining
+// values each (16 bytes of a 16-bit type), or 8 pairs of halves: a thread's place
+// within the head stays the same from head to head, so its cosines and sines, and the
+// token's page, are looked up once, while several heads' values are on their way.
+// Other layouts take one pair per thread.
 #include "serving.cuh"
 
 #include <algorithm>
@@ -115,111 +117,152 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a)
     }
 }
 
-// 8 adjoining elements, in 16-byte (or, in 32 bits, two 16-byte) accesses.
+// 8 adjoining elements, as they lie and as floats.
 template <typename T>
-TMAC_DEV void load8(const T* p, float (&x)[8])
-{
-    constexpr int kVec = 16 / sizeof(T);
+struct Eight {
+    uint4 raw[sizeof(T) / 2];
+    TMAC_DEV void load(const T* p)
+    {
 #pragma unroll
-    for (int i = 0; i < 8; i += kVec) {
-        T r[kVec];
-        *reinterpret_cast<uint4*>(r) = __ldg(reinterpret_cast<const uint4*>(p + i));
-#pragma unroll
-        for (int j = 0; j < kVec; j++) x[i + j] = Elem<T>::load(r + j);
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
     }
-}
+    TMAC_DEV void floats(float (&x)[8]) const
+    {
+        const T* r = reinterpret_cast<const T*>(raw);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = Elem<T>::load(r + i);
+    }
+};
 template <typename T>
 TMAC_DEV void store8(T* p, const float (&x)[8])
 {
-    constexpr int kVec = 16 / sizeof(T);
+    Eight<T> e;
+    T* r = reinterpret_cast<T*>(e.raw);
 #pragma unroll
-    for (int i = 0; i < 8; i += kVec) {
-        T r[kVec];
+    for (int i = 0; i < 8; i++) Elem<T>::store(r + i, x[i]);
 #pragma unroll
-        for (int j = 0; j < kVec; j++) Elem<T>::store(r + j, x[i + j]);
-        *reinterpret_cast<uint4*>(p + i) = *reinterpret_cast<const uint4*>(r);
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4*>(p)[i] = e.raw[i];
 }
 TMAC_DEV void add8(float (&x)[8], const float* bias)
 {
+    Eight<float> e;
+    e.load(bias);
     float b[8];
-    load8(bias, b);
+    e.floats(b);
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = __fadd_rn(x[i], b[i]);
 }
 
-// Units of a token: for each q and k head, 8 values at a time (interleaved), or 8
-// pairs at a time of the rotated part and 8 values at a time of the rest; for
-// each v head, 8 values at a time.
+// Units of a q or k head: 8 values at a time (interleaved), or 8 pairs at a time of
+// the rotated part and 8 values at a time of the rest; of a v head: 8 values at a time.
 template <typename T, typename C, bool kInterleaved>
 __global__ void __launch_bounds__(256) rope_append_vec_kernel(RopeArgs a)
 {
-    const int d = a.cache.dim, hk = a.cache.kv_heads, pairs8 = kInterleaved ? 0 : a.rot / 16;
-    const int per_head = pairs8 + (kInterleaved ? d : d - a.rot) / 8, per_v = d / 8;
-    const int turned = (a.heads + hk) * per_head, per_token = turned + hk * per_v;
-    const int64_t first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, stride = (int64_t)gridDim.x * blockDim.x;
-    const int64_t step_t = stride / per_token;
-    const int step_u = (int)(stride - step_t * per_token);
-    int64_t t = first / per_token;
-    for (int u = (int)(first - t * per_token); t < a.tokens; t += step_t, u += step_u) {
-        if (u >= per_token) {
-            u -= per_token;
-            if (++t >= a.tokens) break;
-        }
-        const bool is_v = u >= turned;
-        const int at = is_v ? u - turned : u, per = is_v ? per_v : per_head;
-        const int row = at / per, unit = at - row * per;  // of q and k together, or of v
-        const bool is_q = !is_v && row < a.heads;
-        const int head = is_v || is_q ? row : row - a.heads;
-        const bool halves = !is_v && unit < pairs8;
-        const int d0 = halves ? unit * 8 : is_v || kInterleaved ? unit * 8 : a.rot + (unit - pairs8) * 8;
-        const int d1 = d0 + a.rot / 2;
-        const T* src = is_q   ? (const T*)a.q + t * a.q_stride
-                       : is_v ? (const T*)a.v + t * a.v_stride
-                              : (const T*)a.k + t * a.k_stride;
-        src += (int64_t)head * d;
-        float x[8], z[8];
-        load8(src + d0, x);
-        if (halves) load8(src + d1, z);
-        if (a.bias) {
-            const float* bias = a.bias + (int64_t)(is_v ? a.heads + hk + row : row) * d;
-            add8(x, bias + d0);
-            if (halves) add8(z, bias + d1);
-        }
-        const Place p = place_of(a, t);
-        C* dst;
-        if (is_q)
-            dst = (C*)a.q_out + (t * a.heads + head) * d;
-        else if (p.page >= 0)
-            dst = (C*)(is_v ? a.cache.v : a.cache.k) + (((p.page * hk + head) << a.cache.page_shift) + p.slot) * d;
-        else
-            continue;
-        if (!p.ok) {
+    constexpr int kFlight = sizeof(T) == 4 ? 2 : 4;  // heads of a thread on their way
+    const int d = a.cache.dim, hk = a.cache.kv_heads, lane = threadIdx.x & 31, shift = a.cache.page_shift;
+    const int pairs8 = kInterleaved ? 0 : a.rot / 16, per_head = pairs8 + (kInterleaved ? d : d - a.rot) / 8;
+    const int warps = (int)(gridDim.x * blockDim.x) >> 5;
+    // heads of a pass, and this lane's head and unit within it
+    const int at_once = 32 / per_head, my_row = lane / per_head, unit = lane - my_row * per_head;
+    const bool halves = unit < pairs8;
+    const int d0 = halves || kInterleaved ? unit * 8 : a.rot + (unit - pairs8) * 8, d1 = d0 + a.rot / 2;
+    const bool turn = kInterleaved ? d0 < a.rot : halves;
+    const int v_once = 32 / (d / 8), v_row = lane / (d / 8), v_d = lane % (d / 8) * 8;
+    const int qk = a.heads + hk;
+    for (int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < a.tokens; t += warps) {
+        const T *q = (const T*)a.q + t * a.q_stride, *k = (const T*)a.k + t * a.k_stride, *v = (const T*)a.v + t * a.v_stride;
+        Place p;
+        float c[8], s[8];
+        for (int base = 0; base < qk; base += at_once * kFlight) {
+            Eight<T> xr[kFlight], zr[kFlight];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = z[i] = 0.0f;
-        } else if (halves) {
-            float c[8], s[8];
-            load8(a.cos + (int64_t)p.pos * (a.rot / 2) + d0, c);
-            load8(a.sin + (int64_t)p.pos * (a.rot / 2) + d0, s);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float xr = __fadd_rn(__fmul_rn(x[i], c[i]), -__fmul_rn(z[i], s[i]));
-                z[i] = __fadd_rn(__fmul_rn(x[i], s[i]), __fmul_rn(z[i], c[i]));
-                x[i] = xr;
+            for (int f = 0; f < kFlight; f++) {
+                const int row = base + f * at_once + my_row;
+                if (my_row >= at_once || row >= qk) continue;
+                const T* src = row < a.heads ? q + row * d : k + (row - a.heads) * d;
+                xr[f].load(src + d0);
+                if (halves) zr[f].load(src + d1);
             }
-        } else if (kInterleaved && !is_v && d0 < a.rot) {
-            const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + (int64_t)p.pos * (a.rot / 2) + d0 / 2));
-            const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.sin + (int64_t)p.pos * (a.rot / 2) + d0 / 2));
-            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+            if (base == 0) {
+                p = place_of(a, t);
+                if (turn && p.ok) {
+                    const int64_t at = (int64_t)p.pos * (a.rot / 2);
+                    if (kInterleaved) {
+                        const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + at + d0 / 2));
+                        const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.sin + at + d0 / 2));
+                        c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w;
+                        s[0] = s4.x, s[1] = s4.y, s[2] = s4.z, s[3] = s4.w;
+                    } else {
+                        Eight<float> e;
+                        e.load(a.cos + at + d0);
+                        e.floats(c);
+                        e.load(a.sin + at + d0);
+                        e.floats(s);
+                    }
+                }
+            }
+            const int64_t page_row = p.page * hk;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float xr = __fadd_rn(__fmul_rn(x[2 * i], c[i]), -__fmul_rn(x[2 * i + 1], s[i]));
-                x[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i], s[i]), __fmul_rn(x[2 * i + 1], c[i]));
-                x[2 * i] = xr;
+            for (int f = 0; f < kFlight; f++) {
+                const int row = base + f * at_once + my_row;
+                if (my_row >= at_once || row >= qk) continue;
+                const bool is_q = row < a.heads;
+                C* dst;
+                if (is_q)
+                    dst = (C*)a.q_out + (t * a.heads + row) * d;
+                else if (p.page >= 0)
+                    dst = (C*)a.cache.k + (((page_row + row - a.heads) << shift) + p.slot) * d;
+                else
+                    continue;
+                float x[8], z[8];
+                xr[f].floats(x);
+                if (halves) zr[f].floats(z);
+                if (a.bias) {
+                    add8(x, a.bias + row * d + d0);
+                    if (halves) add8(z, a.bias + row * d + d1);
+                }
+                if (!p.ok) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = z[i] = 0.0f;
+                } else if (turn) {
+                    if (kInterleaved) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float y = __fadd_rn(__fmul_rn(x[2 * i], c[i]), -__fmul_rn(x[2 * i + 1], s[i]));
+                            x[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i], s[i]), __fmul_rn(x[2 * i + 1], c[i]));
+                            x[2 * i] = y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float y = __fadd_rn(__fmul_rn(x[i], c[i]), -__fmul_rn(z[i], s[i]));
+                            z[i] = __fadd_rn(__fmul_rn(x[i], s[i]), __fmul_rn(z[i], c[i]));
+                            x[i] = y;
+                        }
+                    }
+                }
+                store8(dst + d0, x);
+                if (halves) store8(dst + d1, z);
             }
         }
-        store8(dst + d0, x);
-        if (halves) store8(dst + d1, z);
+        if (p.page < 0) continue;
+        for (int base = 0; base < hk; base += v_once * kFlight) {
+            Eight<T> xr[kFlight];
+#pragma unroll
+            for (int f = 0; f < kFlight; f++) {
+                const int row = base + f * v_once + v_row;
+                if (v_row < v_once && row < hk) xr[f].load(v + row * d + v_d);
+            }
+#pragma unroll
+            for (int f = 0; f < kFlight; f++) {
+                const int row = base + f * v_once + v_row;
+                if (v_row >= v_once || row >= hk) continue;
+                float x[8];
+                xr[f].floats(x);
+                if (a.bias) add8(x, a.bias + (qk + row) * d + v_d);
+                store8((C*)a.cache.v + (((p.page * hk + row) << shift) + p.slot) * d + v_d, x);
+            }
+        }
     }
 }
 
@@ -229,7 +272,7 @@ bool vectors_fit(const RopeArgs& a, bool interleaved)
 {
     auto aligned = [](const void* p) { return (uintptr_t)p % 16 == 0; };
     const int64_t vec = 16 / (int64_t)sizeof(T);
-    return a.cache.dim % 8 == 0 && a.rot % (interleaved ? 8 : 16) == 0 && aligned(a.q) && aligned(a.k) && aligned(a.v) &&
+    return a.cache.dim % 8 == 0 && a.cache.dim <= 256 && a.rot % (interleaved ? 8 : 16) == 0 && aligned(a.q) && aligned(a.k) && aligned(a.v) &&
            a.q_stride % vec == 0 && a.k_stride % vec == 0 && a.v_stride % vec == 0 && aligned(a.q_out) &&
            aligned(a.bias) && aligned(a.cos) && aligned(a.sin);
 }
@@ -238,8 +281,9 @@ template <typename T, typename C>
 int launch_rope(const RopeArgs& a, bool interleaved, int sms, cudaStream_t s)
 {
     const bool vec = vectors_fit<T, C>(a, interleaved);
-    const int64_t n = a.tokens * (a.heads + 2 * a.cache.kv_heads) * (a.cache.dim / (vec ? 8 : 2));
-    const int grid = (int)std::min<int64_t>((n + 255) / 256, (int64_t)sms * 8);
+    // a warp to a token, or a thread to a pair
+    const int64_t threads = vec ? a.tokens * 32 : a.tokens * (a.heads + 2 * a.cache.kv_heads) * (a.cache.dim / 2);
+    const int grid = (int)std::min<int64_t>((threads + 255) / 256, (int64_t)sms * 8);
     auto fn = vec ? interleaved ? rope_append_vec_kernel<T, C, true> : rope_append_vec_kernel<T, C, false>
                   : interleaved ? rope_append_kernel<T, C, true> : rope_append_kernel<T, C, false>;
     fn<<<grid, 256, 0, s>>>(a);
