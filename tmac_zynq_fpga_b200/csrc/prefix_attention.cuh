@@ -215,19 +215,6 @@ TMAC_DEV float power(float x)
     return sizeof(T) == 4 ? expf(x) : exp2_fast(x);
 }
 
-// 16-bit elements as pairs, the first in the low half.
-template <typename T>
-TMAC_DEV uint32_t pack2(float lo, float hi)
-{
-    if constexpr (std::is_same_v<T, __half>) {
-        const __half2 h = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-}
-
 // prefix_attention_tc.cu: the prefix's jobs of 16-bit elements on tcgen05.
 constexpr int kTcRows = 128;  // rows of a job
 int launch_prefix_tc(const AttnArgs& a, int type, cudaStream_t s);

@@ -10,11 +10,12 @@
 // cache's type.
 //
 // Bound: HBM, every value is read once and written once.  Where the pointers,
-// strides and head parts allow it a warp takes a token, its threads 8 adjoining
-// values each (16 bytes of a 16-bit type), or 8 pairs of halves: a thread's place
-// within the head stays the same from head to head, so its cosines and sines, and the
-// token's page, are looked up once, while several heads' values are on their way.
-// Other layouts take one pair per thread.
+// strides and head parts allow it a thread takes 8 adjoining values (16 bytes of a
+// 16-bit type), or 8 pairs of halves (several of either at once run no faster: the
+// registers cost more warps than they gain); a CTA
+// takes a few tokens, whose pages, cosines and sines it first looks up into shared
+// memory, so nothing but the values is waited for.  Other layouts take one pair per
+// thread.
 #include "serving.cuh"
 
 #include <algorithm>
@@ -128,18 +129,32 @@ struct Eight {
     }
     TMAC_DEV void floats(float (&x)[8]) const
     {
-        const T* r = reinterpret_cast<const T*>(raw);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = Elem<T>::load(r + i);
+            for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) unpack2<T>(w[i], x[2 * i], x[2 * i + 1]);
+        }
+    }
+    TMAC_DEV void set(const float (&x)[8])
+    {
+        uint32_t* w = reinterpret_cast<uint32_t*>(raw);
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = __float_as_uint(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
+        }
     }
 };
 template <typename T>
 TMAC_DEV void store8(T* p, const float (&x)[8])
 {
     Eight<T> e;
-    T* r = reinterpret_cast<T*>(e.raw);
-#pragma unroll
-    for (int i = 0; i < 8; i++) Elem<T>::store(r + i, x[i]);
+    e.set(x);
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4*>(p)[i] = e.raw[i];
 }
@@ -153,116 +168,121 @@ TMAC_DEV void add8(float (&x)[8], const float* bias)
     for (int i = 0; i < 8; i++) x[i] = __fadd_rn(x[i], b[i]);
 }
 
+// Division of a number below 2^16 by a fixed one below 2^16.
+struct Divide {
+    uint32_t by, magic;
+    static Divide of(int by) { return {(uint32_t)by, (uint32_t)((0x100000000ull + by - 1) / by)}; }
+    TMAC_DEV int operator()(int x) const { return by == 1 ? x : (int)__umulhi((uint32_t)x, magic); }
+};
 // Units of a q or k head: 8 values at a time (interleaved), or 8 pairs at a time of
 // the rotated part and 8 values at a time of the rest; of a v head: 8 values at a time.
+constexpr int kMaxTokens = 16;  // of a CTA
+struct Deal {
+    int tokens;              // of a CTA
+    int turned;              // units of a token's q and k heads
+    Divide per_token, per_head, per_v;
+};
 template <typename T, typename C, bool kInterleaved>
-__global__ void __launch_bounds__(256) rope_append_vec_kernel(RopeArgs a)
+__global__ void __launch_bounds__(256) rope_append_vec_kernel(RopeArgs a, Deal deal)
 {
-    constexpr int kFlight = sizeof(T) == 4 ? 2 : 4;  // heads of a thread on their way
-    const int d = a.cache.dim, hk = a.cache.kv_heads, lane = threadIdx.x & 31, shift = a.cache.page_shift;
-    const int pairs8 = kInterleaved ? 0 : a.rot / 16, per_head = pairs8 + (kInterleaved ? d : d - a.rot) / 8;
-    const int warps = (int)(gridDim.x * blockDim.x) >> 5;
-    // heads of a pass, and this lane's head and unit within it
-    const int at_once = 32 / per_head, my_row = lane / per_head, unit = lane - my_row * per_head;
-    const bool halves = unit < pairs8;
-    const int d0 = halves || kInterleaved ? unit * 8 : a.rot + (unit - pairs8) * 8, d1 = d0 + a.rot / 2;
-    const bool turn = kInterleaved ? d0 < a.rot : halves;
-    const int v_once = 32 / (d / 8), v_row = lane / (d / 8), v_d = lane % (d / 8) * 8;
-    const int qk = a.heads + hk;
-    for (int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < a.tokens; t += warps) {
-        const T *q = (const T*)a.q + t * a.q_stride, *k = (const T*)a.k + t * a.k_stride, *v = (const T*)a.v + t * a.v_stride;
-        Place p;
-        float c[8], s[8];
-        for (int base = 0; base < qk; base += at_once * kFlight) {
-            Eight<T> xr[kFlight], zr[kFlight];
+    extern __shared__ __align__(16) float turns[];  // [tokens][2][rot / 2]: cosines, sines
+    __shared__ Place places[kMaxTokens];
+    const int d = a.cache.dim, hk = a.cache.kv_heads, shift = a.cache.page_shift, half = a.rot / 2;
+    const int pairs8 = kInterleaved ? 0 : a.rot / 16, per_token = (int)deal.per_token.by;
+    const int64_t t0 = (int64_t)blockIdx.x * deal.tokens;
+    const int n = (int)min((int64_t)deal.tokens, a.tokens - t0), units = n * per_token;
+    struct Unit {
+        int token, row, d0;  // row: of q, k and v together
+        bool is_v, halves;
+    };
+    const auto unit_of = [&](int u) {
+        Unit o;
+        o.token = deal.per_token(u);
+        u -= o.token * per_token;
+        o.is_v = u >= deal.turned;
+        if (o.is_v) {
+            u -= deal.turned;
+            const int head = deal.per_v(u);
+            o.row = a.heads + hk + head;
+            o.d0 = (u - head * (int)deal.per_v.by) * 8;
+            o.halves = false;
+        } else {
+            o.row = deal.per_head(u);
+            const int unit = u - o.row * (int)deal.per_head.by;
+            o.halves = unit < pairs8;
+            o.d0 = o.halves || kInterleaved ? unit * 8 : a.rot + (unit - pairs8) * 8;
+        }
+        return o;
+    };
+    Eight<T> xr, zr;
+    const auto load = [&](const Unit& u) {
+        const int64_t t = t0 + u.token;
+        const T* src = u.is_v              ? (const T*)a.v + t * a.v_stride + (u.row - a.heads - hk) * d
+                       : u.row < a.heads ? (const T*)a.q + t * a.q_stride + u.row * d
+                                           : (const T*)a.k + t * a.k_stride + (u.row - a.heads) * d;
+        xr.load(src + u.d0);
+        if (u.halves) zr.load(src + u.d0 + half);
+    };
+    Unit u = unit_of(threadIdx.x);
+    if ((int)threadIdx.x < units) load(u);
+    if ((int)threadIdx.x < n) places[threadIdx.x] = place_of(a, t0 + threadIdx.x);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * (a.rot / 4); i += 256) {
+        const int token = i / (a.rot / 4), at = i % (a.rot / 4) * 4;  // of cosines, then of sines
+        if (!places[token].ok) continue;
+        const float* from = (at < half ? a.cos + at : a.sin + at - half) + (int64_t)places[token].pos * half;
+        *reinterpret_cast<float4*>(turns + token * a.rot + at) = __ldg(reinterpret_cast<const float4*>(from));
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < units; at += 256) {
+        if (at >= 256) {
+            u = unit_of(at);
+            load(u);
+        }
+        const Place& p = places[u.token];
+        C* dst;
+        if (u.row < a.heads)
+            dst = (C*)a.q_out + ((t0 + u.token) * a.heads + u.row) * d;
+        else if (p.page >= 0)
+            dst = (C*)(u.is_v ? a.cache.v : a.cache.k) +
+                  (((p.page * hk + u.row - a.heads - (u.is_v ? hk : 0)) << shift) + p.slot) * d;
+        else
+            continue;
+        float x[8], z[8];
+        xr.floats(x);
+        if (u.halves) zr.floats(z);
+        if (a.bias) {
+            add8(x, a.bias + u.row * d + u.d0);
+            if (u.halves) add8(z, a.bias + u.row * d + u.d0 + half);
+        }
+        const float *c = turns + u.token * a.rot, *s = c + half;
+        if (!p.ok) {
 #pragma unroll
-            for (int f = 0; f < kFlight; f++) {
-                const int row = base + f * at_once + my_row;
-                if (my_row >= at_once || row >= qk) continue;
-                const T* src = row < a.heads ? q + row * d : k + (row - a.heads) * d;
-                xr[f].load(src + d0);
-                if (halves) zr[f].load(src + d1);
+            for (int i = 0; i < 8; i++) x[i] = z[i] = 0.0f;
+        } else if (kInterleaved && !u.is_v && u.d0 < a.rot) {
+            const float4 c4 = *reinterpret_cast<const float4*>(c + u.d0 / 2), s4 = *reinterpret_cast<const float4*>(s + u.d0 / 2);
+            const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float y = __fmaf_rn(x[2 * i], cv[i], -__fmul_rn(x[2 * i + 1], sv[i]));
+                x[2 * i + 1] = __fmaf_rn(x[2 * i], sv[i], __fmul_rn(x[2 * i + 1], cv[i]));
+                x[2 * i] = y;
             }
-            if (base == 0) {
-                p = place_of(a, t);
-                if (turn && p.ok) {
-                    const int64_t at = (int64_t)p.pos * (a.rot / 2);
-                    if (kInterleaved) {
-                        const float4 c4 = __ldg(reinterpret_cast<const float4*>(a.cos + at + d0 / 2));
-                        const float4 s4 = __ldg(reinterpret_cast<const float4*>(a.sin + at + d0 / 2));
-                        c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w;
-                        s[0] = s4.x, s[1] = s4.y, s[2] = s4.z, s[3] = s4.w;
-                    } else {
-                        Eight<float> e;
-                        e.load(a.cos + at + d0);
-                        e.floats(c);
-                        e.load(a.sin + at + d0);
-                        e.floats(s);
-                    }
+        } else if (u.halves) {
+#pragma unroll
+            for (int h = 0; h < 8; h += 4) {
+                const float4 c4 = *reinterpret_cast<const float4*>(c + u.d0 + h), s4 = *reinterpret_cast<const float4*>(s + u.d0 + h);
+                const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float y = __fmaf_rn(x[h + i], cv[i], -__fmul_rn(z[h + i], sv[i]));
+                    z[h + i] = __fmaf_rn(x[h + i], sv[i], __fmul_rn(z[h + i], cv[i]));
+                    x[h + i] = y;
                 }
-            }
-            const int64_t page_row = p.page * hk;
-#pragma unroll
-            for (int f = 0; f < kFlight; f++) {
-                const int row = base + f * at_once + my_row;
-                if (my_row >= at_once || row >= qk) continue;
-                const bool is_q = row < a.heads;
-                C* dst;
-                if (is_q)
-                    dst = (C*)a.q_out + (t * a.heads + row) * d;
-                else if (p.page >= 0)
-                    dst = (C*)a.cache.k + (((page_row + row - a.heads) << shift) + p.slot) * d;
-                else
-                    continue;
-                float x[8], z[8];
-                xr[f].floats(x);
-                if (halves) zr[f].floats(z);
-                if (a.bias) {
-                    add8(x, a.bias + row * d + d0);
-                    if (halves) add8(z, a.bias + row * d + d1);
-                }
-                if (!p.ok) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] = z[i] = 0.0f;
-                } else if (turn) {
-                    if (kInterleaved) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float y = __fadd_rn(__fmul_rn(x[2 * i], c[i]), -__fmul_rn(x[2 * i + 1], s[i]));
-                            x[2 * i + 1] = __fadd_rn(__fmul_rn(x[2 * i], s[i]), __fmul_rn(x[2 * i + 1], c[i]));
-                            x[2 * i] = y;
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float y = __fadd_rn(__fmul_rn(x[i], c[i]), -__fmul_rn(z[i], s[i]));
-                            z[i] = __fadd_rn(__fmul_rn(x[i], s[i]), __fmul_rn(z[i], c[i]));
-                            x[i] = y;
-                        }
-                    }
-                }
-                store8(dst + d0, x);
-                if (halves) store8(dst + d1, z);
             }
         }
-        if (p.page < 0) continue;
-        for (int base = 0; base < hk; base += v_once * kFlight) {
-            Eight<T> xr[kFlight];
-#pragma unroll
-            for (int f = 0; f < kFlight; f++) {
-                const int row = base + f * v_once + v_row;
-                if (v_row < v_once && row < hk) xr[f].load(v + row * d + v_d);
-            }
-#pragma unroll
-            for (int f = 0; f < kFlight; f++) {
-                const int row = base + f * v_once + v_row;
-                if (v_row >= v_once || row >= hk) continue;
-                float x[8];
-                xr[f].floats(x);
-                if (a.bias) add8(x, a.bias + (qk + row) * d + v_d);
-                store8((C*)a.cache.v + (((p.page * hk + row) << shift) + p.slot) * d + v_d, x);
-            }
-        }
+        store8(dst + u.d0, x);
+        if (u.halves) store8(dst + u.d0 + half, z);
     }
 }
 
@@ -280,13 +300,23 @@ bool vectors_fit(const RopeArgs& a, bool interleaved)
 template <typename T, typename C>
 int launch_rope(const RopeArgs& a, bool interleaved, int sms, cudaStream_t s)
 {
-    const bool vec = vectors_fit<T, C>(a, interleaved);
-    // a warp to a token, or a thread to a pair
-    const int64_t threads = vec ? a.tokens * 32 : a.tokens * (a.heads + 2 * a.cache.kv_heads) * (a.cache.dim / 2);
-    const int grid = (int)std::min<int64_t>((threads + 255) / 256, (int64_t)sms * 8);
-    auto fn = vec ? interleaved ? rope_append_vec_kernel<T, C, true> : rope_append_vec_kernel<T, C, false>
-                  : interleaved ? rope_append_kernel<T, C, true> : rope_append_kernel<T, C, false>;
-    fn<<<grid, 256, 0, s>>>(a);
+    const int hk = a.cache.kv_heads, per_head = interleaved ? a.cache.dim / 8 : a.rot / 16 + (a.cache.dim - a.rot) / 8;
+    const int64_t per_token = (int64_t)(a.heads + hk) * per_head + hk * (a.cache.dim / 8);
+    if (per_token < 4096 && vectors_fit<T, C>(a, interleaved)) {
+        Deal d;
+        // tokens of a CTA: as long as there are four CTAs to an SM
+        d.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxTokens, a.tokens / (4 * sms)));
+        d.turned = (a.heads + hk) * per_head;
+        d.per_token = Divide::of((int)per_token);
+        d.per_head = Divide::of(per_head);
+        d.per_v = Divide::of(a.cache.dim / 8);
+        auto fn = interleaved ? rope_append_vec_kernel<T, C, true> : rope_append_vec_kernel<T, C, false>;
+        fn<<<(unsigned)((a.tokens + d.tokens - 1) / d.tokens), 256, (size_t)d.tokens * a.rot * sizeof(float), s>>>(a, d);
+    } else {
+        const int64_t pairs = a.tokens * (a.heads + 2 * hk) * (a.cache.dim / 2);
+        auto fn = interleaved ? rope_append_kernel<T, C, true> : rope_append_kernel<T, C, false>;
+        fn<<<(unsigned)std::min<int64_t>((pairs + 255) / 256, (int64_t)sms * 8), 256, 0, s>>>(a);
+    }
     TMAC_CUDA_TRY(cudaGetLastError());
     return TMAC_OK;
 }

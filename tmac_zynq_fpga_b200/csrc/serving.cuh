@@ -11,6 +11,7 @@
 #include <cuda_bf16.h>
 
 #include <atomic>
+#include <type_traits>
 
 namespace tmac {
 
@@ -34,6 +35,32 @@ struct Elem<__nv_bfloat16> {
     static TMAC_DEV float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
     static TMAC_DEV void store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 };
+
+// 16-bit elements as pairs, the first in the low half.
+template <typename T>
+TMAC_DEV uint32_t pack2(float lo, float hi)
+{
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+template <typename T>
+TMAC_DEV void unpack2(uint32_t pair, float& lo, float& hi)
+{
+    if constexpr (std::is_same_v<T, __half>) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair));
+        lo = f.x;
+        hi = f.y;
+    } else {
+        lo = __uint_as_float(pair << 16);
+        hi = __uint_as_float(pair & 0xFFFF0000u);
+    }
+}
 
 inline int type_bytes(int type)
 {
