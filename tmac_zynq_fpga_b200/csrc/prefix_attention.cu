@@ -41,23 +41,22 @@ struct Copier {
     static constexpr int kAtOnce = 32 / kPer < 1 ? 1 : 32 / kPer;         // keys of a warp's one copy
     static constexpr int kKeys = kTile / kWarps;                          // keys of the warp
     static_assert(kPer <= 32 && kKeys <= 32 && kKeys == kCopies * kAtOnce, "a lane to a key");
-    int page;  // of this lane's key, for the tile to copy next
-
     // The tile's key that copy i of lane `lane` belongs to
     static TMAC_DEV int key_of(int i, int lane) { return (threadIdx.x >> 5) * kAtOnce + i * (kWarps * kAtOnce) + lane / kPer; }
-    TMAC_DEV void look_up(const AttnArgs& a, const Job& j, int t)
+    // The page of this lane's key in tile t
+    static TMAC_DEV int look_up(const AttnArgs& a, const Job& j, int t)
     {
         const int lane = threadIdx.x & 31;
-        if (t >= j.tile1 || lane >= kKeys) return;
+        if (t >= j.tile1 || lane >= kKeys) return 0;
         const TileOf tile = find_tile(a, j, t);
         const int g = tile.key0 + key_of(lane / kAtOnce, lane % kAtOnce * kPer);
-        page = g < tile.keys ? __ldg(tile.pages + (g >> a.cache.page_shift)) : 0;
+        return g < tile.keys ? __ldg(tile.pages + (g >> a.cache.page_shift)) : 0;
     }
-    // Starts tile t's copies, after its look_up; k_at(key, value) and v_at say where 16
+    // Starts tile t's copies, its look_up given; k_at(key, value) and v_at say where 16
     // bytes from that value on go.  Keys out of reach, and rows of a page outside the
     // pool (the error word says so), become zeros.
     template <typename FK, typename FV>
-    TMAC_DEV void start(const AttnArgs& a, const Job& j, int t, FK&& k_at, FV&& v_at) const
+    static TMAC_DEV void start(const AttnArgs& a, const Job& j, int t, int page, FK&& k_at, FV&& v_at)
     {
         const int lane = threadIdx.x & 31, shift = a.cache.page_shift;
         const TileOf tile = find_tile(a, j, t);
@@ -106,16 +105,16 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(AttnArgs a)
     if (!find_job<kJobRows>(a, &j)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const bool split_keys = j.rows <= kRows;
-    Copier<T, D> copier;
+    using Copy = Copier<T, D>;
+    int page = Copy::look_up(a, j, j.tile0);  // of the tile to start next
     const auto start = [&](int t) {
         if (t < j.tile1) {
             auto& st = sh.stage[(t - j.tile0) % kSimtStages];
-            copier.start(a, j, t, [&](int key, int c) { return &st.k[key][c]; }, [&](int key, int c) { return &st.v[key][c]; });
-            copier.look_up(a, j, t + 1);
+            Copy::start(a, j, t, page, [&](int key, int c) { return &st.k[key][c]; }, [&](int key, int c) { return &st.v[key][c]; });
+            page = Copy::look_up(a, j, t + 1);
         }
         cp_async_commit();
     };
-    copier.look_up(a, j, j.tile0);
     start(j.tile0);
     sh.rows.find(a, j);
     for (int i = threadIdx.x; i < kJobRows * D; i += kThreads) {
@@ -243,7 +242,8 @@ __global__ void __launch_bounds__(kThreads) attn_simt_kernel(AttnArgs a)
             sum = sh.ml[r / kRows][r % kRows][1];
             val = ow[r * D + d];
         }
-        put_result<T, D>(a, j, sh.rows.token[r], sh.rows.head[r], d, mx, sum, val);
+        const float one[1] = {val};
+        put_results<T, D, 1>(a, j, RowOf{sh.rows.token[r], sh.rows.head[r], 0, 0}, d, mx, sum, one);
     }
 }
 
@@ -262,7 +262,6 @@ struct MmaSmem {
         T k[kTile * D], v[kTile * D];
     } stage[MmaConf<T, D>::kStages];
     float ml[kWarps][kMmaRows][2];
-    Rows<kWarps * kMmaRows> rows;
 };
 // 16-byte pieces of a row lie turned by the row's number: eight rows of one column
 // fall on different banks.
@@ -308,40 +307,55 @@ TMAC_DEV void attn_mma(const AttnArgs& a)
     if (!find_job<kJobRows>(a, &j)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
     const bool split_keys = j.rows <= kMmaRows;
-    Copier<T, D> copier;
-    const auto start = [&](int t) {
+    using Copy = Copier<T, D>;
+    const auto copy = [&](int t, int page) {
         if (t < j.tile1) {
             auto& st = sh.stage[(t - j.tile0) % kStages];
-            copier.start(a, j, t, [&](int key, int c) { return &st.k[turned<D>(key, c)]; },
-                         [&](int key, int c) { return &st.v[turned<D>(key, c)]; });
-            copier.look_up(a, j, t + 1);
+            Copy::start(a, j, t, page, [&](int key, int c) { return &st.k[turned<D>(key, c)]; },
+                        [&](int key, int c) { return &st.v[turned<D>(key, c)]; });
         }
         cp_async_commit();
     };
-    copier.look_up(a, j, j.tile0);
+    int page[kStages];  // of the first tiles; then page[0], of the tile to copy next
 #pragma unroll
-    for (int i = 0; i < kStages - 1; i++) start(j.tile0 + i);
-    sh.rows.find(a, j);
+    for (int i = 0; i < kStages; i++) page[i] = Copy::look_up(a, j, j.tile0 + i);
 
     // this thread's rows g and g + 8 of the warp's, as the product's first operand
     const int r0 = split_keys ? 0 : warp * kMmaRows;
     uint32_t q[D / 16][4];
+    int p_limit[2], o_limit[2];
+    const bool pairs = ((uintptr_t)a.q % 4 | a.q_stride % 2) == 0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int r = r0 + g + 8 * h;
-        const T* src = (const T*)a.q + sh.rows.token[r] * a.q_stride + sh.rows.head[r] * D + c2;
+        RowOf row = {0, 0, 0x7FFFFFFF, 0x7FFFFFFF};
+        if (r < j.rows) row = find_row(a, j, r);
+        p_limit[h] = row.p_limit;
+        o_limit[h] = row.o_limit;
+        const T* src = (const T*)a.q + row.token * a.q_stride + row.head * D + c2;
 #pragma unroll
         for (int i = 0; i < D / 16; i++)
 #pragma unroll
             for (int w = 0; w < 2; w++) {
-                T pair[2] = {};
+                uint32_t x = 0;
                 if (r < j.rows) {
-                    pair[0] = src[16 * i + 8 * w];
-                    pair[1] = src[16 * i + 8 * w + 1];
+                    const T* at = src + 16 * i + 8 * w;
+                    if (pairs) {
+                        x = __ldg(reinterpret_cast<const uint32_t*>(at));
+                    } else {
+                        const T two[2] = {at[0], at[1]};
+                        x = *reinterpret_cast<const uint32_t*>(two);
+                    }
                 }
-                q[i][2 * w + h] = *reinterpret_cast<const uint32_t*>(pair);
+                q[i][2 * w + h] = x;
             }
     }
+#pragma unroll
+    for (int i = 0; i < kStages - 1; i++) copy(j.tile0 + i, page[i]);
+    page[0] = page[kStages - 1];
+    // below these limits no row of the warp needs a mask
+    const int p_least = __reduce_min_sync(0xffffffffu, min(p_limit[0], p_limit[1]));
+    const int o_least = __reduce_min_sync(0xffffffffu, min(o_limit[0], o_limit[1]));
     const float scale = __fmul_rn(a.scale, 1.44269504f);  // log2 e: exponentials are powers of 2
     float m[2], l[2], o[kN][4];
     bool careful = false;
@@ -356,11 +370,12 @@ again:
     for (int t = j.tile0; t < j.tile1; t++) {
         cp_async_wait<kStages - 2>();
         __syncthreads();
-        start(t + kStages - 1);
+        copy(t + kStages - 1, page[0]);
+        page[0] = Copy::look_up(a, j, t + kStages);
         const auto& st = sh.stage[(t - j.tile0) % kStages];
         const TileOf tile = find_tile(a, j, t);
-        const int* limits = tile.prefix ? sh.rows.p_limit : sh.rows.o_limit;
-        const int least = min(tile.prefix ? sh.rows.p_least : sh.rows.o_least, tile.keys);
+        const int least = min(tile.prefix ? p_least : o_least, tile.keys);
+        const int limits[2] = {min(tile.prefix ? p_limit[0] : o_limit[0], tile.keys), min(tile.prefix ? p_limit[1] : o_limit[1], tile.keys)};
         // kN8 * 8 keys from `step` on
         const auto keys = [&](auto n8, int step) {
             constexpr int kN8 = decltype(n8)::value;
@@ -378,7 +393,7 @@ again:
             float al[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const int limit = limits[r0 + g + 8 * h];
+                const int limit = limits[h];
                 float mx = -INFINITY;
 #pragma unroll
                 for (int n = 0; n < kN8; n++)
@@ -462,9 +477,8 @@ again:
             for (int c = 0; c < 4; c++) finite &= fabsf(o[n][c]) < INFINITY;
         if (__syncthreads_or(!finite)) {
             careful = true;
-            copier.look_up(a, j, j.tile0);
-#pragma unroll
-            for (int i = 0; i < kStages - 1; i++) start(j.tile0 + i);
+            for (int i = 0; i < kStages - 1; i++) copy(j.tile0 + i, Copy::look_up(a, j, j.tile0 + i));
+            page[0] = Copy::look_up(a, j, j.tile0 + kStages - 1);
             goto again;
         }
     }
@@ -473,6 +487,21 @@ again:
         l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 1));
         l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 2));
     }
+    if (!split_keys) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = r0 + g + 8 * h;
+            if (r >= j.rows) continue;
+            const RowOf row = find_row(a, j, r);
+#pragma unroll
+            for (int n = 0; n < kN; n++) {
+                const float two[2] = {o[n][2 * h], o[n][2 * h + 1]};
+                put_results<T, D, 2>(a, j, row, 8 * n + c2, m[h], l[h], two);
+            }
+        }
+        return;
+    }
+    // the warps' results, joined
     __syncthreads();
     float* ow = reinterpret_cast<float*>(&sh.stage[0]);  // [warps][16][D]
     static_assert(sizeof(float) * kWarps * kMmaRows * D <= sizeof(sh.stage), "join space");
@@ -488,26 +517,24 @@ again:
             *reinterpret_cast<float2*>(&ow[(warp * kMmaRows + r) * D + 8 * n + c2]) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < j.rows * D; i += kThreads) {
-        const int r = i / D, d = i % D;
-        float mx, sum, val;
-        if (split_keys) {
-            mx = -INFINITY;
-            for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, sh.ml[w][r][0]);
-            sum = val = 0.0f;
-            for (int w = 0; w < kWarps; w++) {
-                const float lw = sh.ml[w][r][1];
-                if (lw == 0.0f) continue;  // saw no key
-                const float f = exp2_fast(__fsub_rn(sh.ml[w][r][0], mx));
-                sum = __fmaf_rn(f, lw, sum);
-                val = __fmaf_rn(f, ow[(w * kMmaRows + r) * D + d], val);
-            }
-        } else {
-            mx = sh.ml[r / kMmaRows][r % kMmaRows][0];
-            sum = sh.ml[r / kMmaRows][r % kMmaRows][1];
-            val = ow[r * D + d];
+    for (int i = threadIdx.x; i < j.rows * (D / 4); i += kThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float mx = -INFINITY, sum = 0.0f, val[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, sh.ml[w][r][0]);
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) {
+            const float lw = sh.ml[w][r][1];
+            if (lw == 0.0f) continue;  // saw no key
+            const float f = exp2_fast(__fsub_rn(sh.ml[w][r][0], mx));
+            const float4 x = *reinterpret_cast<const float4*>(&ow[(w * kMmaRows + r) * D + d]);
+            sum = __fmaf_rn(f, lw, sum);
+            val[0] = __fmaf_rn(f, x.x, val[0]);
+            val[1] = __fmaf_rn(f, x.y, val[1]);
+            val[2] = __fmaf_rn(f, x.z, val[2]);
+            val[3] = __fmaf_rn(f, x.w, val[3]);
         }
-        put_result<T, D>(a, j, sh.rows.token[r], sh.rows.head[r], d, mx, sum, val);
+        put_results<T, D, 4>(a, j, find_row(a, j, r), d, mx, sum, val);
     }
 }
 

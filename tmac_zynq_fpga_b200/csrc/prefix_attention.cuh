@@ -189,16 +189,37 @@ TMAC_DEV TileOf find_tile(const AttnArgs& a, const Job& j, int t)
     o.keys = o.prefix ? j.p_keys : j.o_keys;
     return o;
 }
-// Row r's result, value d: the part's, or the rounded quotient when there is no other.
-template <typename T, int D>
-TMAC_DEV void put_result(const AttnArgs& a, const Job& j, int token, int head, int d, float m, float l, float o)
+// kN adjoining values of a row's result from dim d on: the part's, or the rounded
+// quotients when there is no other.
+template <typename T, int D, int kN>
+TMAC_DEV void put_results(const AttnArgs& a, const Job& j, const RowOf& row, int d, float m, float l, const float (&o)[kN])
 {
     if (a.parts == 1) {
-        Elem<T>::store((T*)a.out + token * a.out_stride + head * D + d, l == 0.0f ? 0.0f : __fdiv_rn(o, l));
+        T* to = (T*)a.out + row.token * a.out_stride + row.head * D + d;
+        const float by = l == 0.0f ? 0.0f : __frcp_rn(l);
+        float y[kN];
+#pragma unroll
+        for (int i = 0; i < kN; i++) y[i] = l == 0.0f ? 0.0f : sizeof(T) == 4 ? __fdiv_rn(o[i], l) : __fmul_rn(o[i], by);
+        if constexpr (sizeof(T) == 2 && kN % 2 == 0) {
+            if ((uintptr_t)to % 4 == 0) {
+#pragma unroll
+                for (int i = 0; i < kN / 2; i++) reinterpret_cast<uint32_t*>(to)[i] = pack2<T>(y[2 * i], y[2 * i + 1]);
+                return;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kN; i++) Elem<T>::store(to + i, y[i]);
         return;
     }
-    const int64_t at = ((int64_t)token * a.heads + head) * a.parts + j.part;
-    a.part_o[at * D + d] = o;
+    const int64_t at = ((int64_t)row.token * a.heads + row.head) * a.parts + j.part;
+    float* to = a.part_o + at * D + d;
+    if constexpr (kN == 4)
+        *reinterpret_cast<float4*>(to) = make_float4(o[0], o[1], o[2], o[3]);
+    else if constexpr (kN == 2)
+        *reinterpret_cast<float2*>(to) = make_float2(o[0], o[1]);
+    else
+#pragma unroll
+        for (int i = 0; i < kN; i++) to[i] = o[i];
     if (d == 0) a.part_ml[at] = make_float2(m, l);
 }
 // Maxima are in units of the exponential's base: e in 32 bits, where the difference

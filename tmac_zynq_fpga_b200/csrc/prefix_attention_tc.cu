@@ -114,8 +114,7 @@ struct Two {
     uint64_t v;
     TMAC_DEV Two(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
     TMAC_DEV explicit Two(uint64_t x) : v(x) {}
-    TMAC_DEV float lo() const { float a, b; asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); return a; }
-    TMAC_DEV float hi() const { float a, b; asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); return b; }
+    TMAC_DEV void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
 };
 TMAC_DEV Two fma2(Two a, Two b, Two c)
 {
@@ -129,49 +128,60 @@ TMAC_DEV Two add2(Two a, Two b)
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
     return Two(d);
 }
-// The weights 2^(x scale - m) of 32 scores, as pairs; kMasked: those from `seen` on
-// are 0.  Returns their sum.
-template <typename T, bool kMasked>
-TMAC_DEV float weights(const uint32_t (&x)[32], float scale, float m, int seen, uint32_t (&p)[16])
+// The weights 2^(x scale - m) of 32 scores, as pairs.  Returns their sum.
+template <typename T>
+TMAC_DEV float weights(const uint32_t (&x)[32], Two scale, Two base, uint32_t (&p)[16])
 {
-    const float base = m == -INFINITY ? 0.0f : -m;
-    const Two scale2(scale, scale), base2(base, base);
     Two sum[2] = {Two(0.0f, 0.0f), Two(0.0f, 0.0f)};
 #pragma unroll
     for (int i = 0; i < 16; i++) {
-        const Two e = fma2(Two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale2, base2);
-        float p0 = exp2_fast(e.lo()), p1 = exp2_fast(e.hi());
-        if (kMasked) {
-            if (2 * i >= seen) p0 = 0.0f;
-            if (2 * i + 1 >= seen) p1 = 0.0f;
-        }
+        float e0, e1;
+        fma2(Two(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), scale, base).get(e0, e1);
+        const float p0 = exp2_fast(e0), p1 = exp2_fast(e1);
         sum[i & 1] = add2(sum[i & 1], Two(p0, p1));
         p[i] = pack2<T>(p0, p1);
     }
-    const Two all = add2(sum[0], sum[1]);
-    return __fadd_rn(all.lo(), all.hi());
-}
-template <typename T>
-TMAC_DEV float weights(const uint32_t (&x)[32], float scale, float m, bool masked, int seen, uint32_t (&p)[16])
-{
-    return masked ? weights<T, true>(x, scale, m, seen, p) : weights<T, false>(x, scale, m, seen, p);
+    float s0, s1;
+    add2(sum[0], sum[1]).get(s0, s1);
+    return __fadd_rn(s0, s1);
 }
 
-// 32 values of a row's sums from dim d on.
+// Writes the warp's 32 rows of sums, as they lie in `rows` (kPad floats apart), each
+// row's adjoining values by adjoining threads: the parts, or the rounded quotients
+// when there are no others.
+template <int D>
+constexpr int kPad = D + 4;
 template <typename T, int D>
-TMAC_DEV void put_row_of(const AttnArgs& a, const Job& j, const RowOf& row, int d, float m, float l, const uint32_t (&x)[32])
+TMAC_DEV void put_rows(const AttnArgs& a, const Job& j, const RowOf& row, bool mine, float l, const float* rows)
 {
-    if (a.parts == 1) {
+    constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;
+    const int lane = threadIdx.x & 31, c = lane % kLanes * 4;
+    const int64_t at = a.parts == 1 ? row.token * a.out_stride + row.head * D
+                                    : (((int64_t)row.token * a.heads + row.head) * a.parts + j.part) * D;
+    const bool aligned = (((uintptr_t)a.out / sizeof(T)) | a.out_stride) % 4 == 0;
+    for (int i = 0; i < 32; i += kAtOnce) {
+        const int r = i + lane / kLanes;
+        const int64_t to = __shfl_sync(0xffffffffu, at, r);
+        const float sum = __shfl_sync(0xffffffffu, l, r);
+        const bool wanted = __shfl_sync(0xffffffffu, (int)mine, r);
+        float4 x = *reinterpret_cast<const float4*>(rows + r * kPad<D> + c);
+        if (!wanted) continue;
+        if (sum == 0.0f) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // saw no key
+        if (a.parts > 1) {
+            *reinterpret_cast<float4*>(a.part_o + to + c) = x;
+            continue;
+        }
+        const float by = sum == 0.0f ? 0.0f : __frcp_rn(sum);
+        T* out = (T*)a.out + to + c;
+        const uint2 y = make_uint2(pack2<T>(__fmul_rn(x.x, by), __fmul_rn(x.y, by)), pack2<T>(__fmul_rn(x.z, by), __fmul_rn(x.w, by)));
+        if (aligned) {
+            *reinterpret_cast<uint2*>(out) = y;
+        } else {
+            const T* e = reinterpret_cast<const T*>(&y);
 #pragma unroll
-        for (int i = 0; i < 32; i++) put_result<T, D>(a, j, row.token, row.head, d + i, m, l, __uint_as_float(x[i]));
-        return;
+            for (int k = 0; k < 4; k++) out[k] = e[k];
+        }
     }
-    const int64_t at = ((int64_t)row.token * a.heads + row.head) * a.parts + j.part;
-    const uint32_t keep = l == 0.0f ? 0u : ~0u;  // saw no key: zeros
-    uint4* to = reinterpret_cast<uint4*>(a.part_o + at * D + d);
-#pragma unroll
-    for (int i = 0; i < 8; i++) to[i] = make_uint4(x[4 * i] & keep, x[4 * i + 1] & keep, x[4 * i + 2] & keep, x[4 * i + 3] & keep);
-    if (d == 0) a.part_ml[at] = make_float2(m, l);
 }
 
 // The row's result key by key from the pools, only over the keys that it sees: for
@@ -199,7 +209,10 @@ __device__ __noinline__ void row_by_keys(const AttnArgs& a, const Job& j, const 
         }
         m = mx;
     }
-    for (int d = 0; d < D; d++) put_result<T, D>(a, j, row.token, row.head, d, m, l, o[d]);
+    for (int d = 0; d < D; d++) {
+        const float one[1] = {o[d]};
+        put_results<T, D, 1>(a, j, row, d, m, l, one);
+    }
 }
 
 template <typename T, int D>
@@ -359,7 +372,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             fence_proxy_async_smem();
             mbar_arrive(&bar.q_full);
         }
-        const float scale = __fmul_rn(fabsf(a.scale), 1.44269504f);  // exponentials are powers of 2
+        // exponentials are powers of 2; not 0, so that a masked score's -inf stays one
+        const float scale = fmaxf(__fmul_rn(fabsf(a.scale), 1.44269504f), 1e-37f);
         constexpr float kLimit = std::is_same_v<T, __half> ? 256.0f : 1073741824.0f;
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
@@ -385,49 +399,49 @@ __global__ void __launch_bounds__(kTcThreads, 2)
             } else {
                 uint32_t x[2][32], p[2][16];
                 tmem_ld32(mine, x[0]);
-                tmem_wait_ld32(x[0]);
                 tmem_ld32(mine + 32, x[1]);
-                const bool masked = __any_sync(0xffffffffu, seen < kTile);
-                bool fits = m > -INFINITY;
-                float sum = 0.0f;
-                if (__all_sync(0xffffffffu, fits)) {
-                    sum = weights<T>(x[0], scale, m, masked, seen, p[0]);
-                    tmem_wait_ld32(x[1]);
-                    sum = __fadd_rn(sum, weights<T>(x[1], scale, m, masked, seen - 32, p[1]));
-                    fits = !(sum > kLimit);
-                } else {
-                    tmem_wait_ld32(x[1]);
-                    fits = false;
-                }
+                tmem_wait_ld32(x[0]);
+                tmem_wait_ld32(x[1]);
                 tc_fence_before();
                 mbar_arrive(&bar.s_empty);
-                // this buffer's last weights have been read
-                if (t > 1 && !(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[t % 2], t / 2 - 1)))) break;
-                if (__any_sync(0xffffffffu, !fits)) {
-                    float mx = -INFINITY;
+                if (__any_sync(0xffffffffu, seen < kTile)) {
 #pragma unroll
                     for (int c = 0; c < 64; c++)
-                        if (!masked || c < seen) mx = fmaxf(mx, __uint_as_float(x[c / 32][c % 32]));
-                    mx = fmaxf(m, __fmul_rn(mx, scale));
-                    if (fits) mx = m;
-                    const float al = mx == m ? 1.0f : exp2_fast(__fsub_rn(m, mx));
-                    m = mx;
-                    l = __fmul_rn(l, al);
-                    if (t > 0) {  // the sums so far must be complete
-                        if (!(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[(t - 1) % 2], (t - 1) / 2)))) break;
-                        tc_fence_after();
+                        if (c >= seen) x[c / 32][c % 32] = 0xFF800000u;  // -inf
+                }
+                // this buffer's last weights have been read
+                if (t > 1 && !(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[t % 2], t / 2 - 1)))) break;
+                float sum = 0.0f;
+                for (bool fits = m > -INFINITY, found = false;; found = true) {
+                    if (__any_sync(0xffffffffu, !fits)) {  // a larger m
+                        float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int c = 0; c < D / 32; c++) {
-                            uint32_t y[32];
-                            tmem_ld32(mine + kOCol + 32 * c, y);
-                            tmem_wait_ld32(y);
+                        for (int c = 0; c < 64; c++) top[c & 3] = fmaxf(top[c & 3], __fmul_rn(__uint_as_float(x[c / 32][c % 32]), scale));
+                        const float mx = fits ? m : fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                        const float al = mx == m ? 1.0f : exp2_fast(__fsub_rn(m, mx));
+                        m = mx;
+                        l = __fmul_rn(l, al);
+                        if (t > 0) {  // the sums so far must be complete
+                            if (!(ok = __all_sync(0xffffffffu, wait(&bar.pv_done[(t - 1) % 2], (t - 1) / 2)))) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D / 32; c++) {
+                                uint32_t y[32];
+                                tmem_ld32(mine + kOCol + 32 * c, y);
+                                tmem_wait_ld32(y);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) y[i] = __float_as_uint(__fmul_rn(__uint_as_float(y[i]), al));
-                            tmem_st32(mine + kOCol + 32 * c, y);
+                                for (int i = 0; i < 32; i++) y[i] = __float_as_uint(__fmul_rn(__uint_as_float(y[i]), al));
+                                tmem_st32(mine + kOCol + 32 * c, y);
+                            }
                         }
                     }
-                    sum = __fadd_rn(weights<T>(x[0], scale, m, masked, seen, p[0]), weights<T>(x[1], scale, m, masked, seen - 32, p[1]));
+                    const float base = m == -INFINITY ? 0.0f : -m;
+                    const Two scale2(scale, scale), base2(base, base);
+                    sum = __fadd_rn(weights<T>(x[0], scale2, base2, p[0]), weights<T>(x[1], scale2, base2, p[1]));
+                    fits = !(sum > kLimit);
+                    if (found || __all_sync(0xffffffffu, fits)) break;
                 }
+                if (!ok) break;
                 tmem_st16(mine + kPCol + t % 2 * 32, p[0]);
                 tmem_st16(mine + kPCol + t % 2 * 32 + 16, p[1]);
                 l = __fadd_rn(l, sum);
@@ -441,6 +455,9 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         if (ok && !idle) {
             tc_fence_after();
             bool finite = true;
+            // the tiles' place is free: every product has run
+            float* rows = reinterpret_cast<float*>(smem) + quarter * 32 * kPad<D>;
+            static_assert(4 * 32 * kPad<D> * sizeof(float) <= C::kQBytes + 2 * C::kStages * C::kBytes, "room for the rows");
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
                 uint32_t x[32];
@@ -448,10 +465,16 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                 tmem_wait_ld32(x);
 #pragma unroll
                 for (int i = 0; i < 32; i++) finite &= fabsf(__uint_as_float(x[i])) < INFINITY;
-                if (r < j.rows) put_row_of<T, D>(a, j, row, 32 * c, m, l, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    *reinterpret_cast<uint4*>(rows + lane * kPad<D> + 32 * c + 4 * i) =
+                        make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             }
-            if (r < j.rows && !finite && row.p_limit < key1)
-                row_by_keys<T, D>(a, j, row, key0, key1, __fmul_rn(a.scale, 1.44269504f));
+            __syncwarp();
+            const bool wanted = r < j.rows, again = wanted && !finite && row.p_limit < key1;
+            if (wanted && a.parts > 1) a.part_ml[((int64_t)row.token * a.heads + row.head) * a.parts + j.part] = make_float2(m, l);
+            put_rows<T, D>(a, j, row, wanted && !again, l, rows);
+            if (again) row_by_keys<T, D>(a, j, row, key0, key1, __fmul_rn(a.scale, 1.44269504f));
         }
         tc_fence_before();
     }
