@@ -14,8 +14,14 @@
 // jobs.  Where that is less work than a second launch, every sequence reads the
 // prefix itself, and one job holds all of a row's keys and writes its result.
 //
-// Two kernels share this frame: 32-bit elements on the FMA units, 16-bit ones on
-// mma.sync.  Tiles come through cp.async, several in flight.
+// The products run on mma.sync with 32-bit sums.  16-bit elements are its operands
+// as they are; a 32-bit one is split into the nearest tf32 number and the rest
+// rounded to one, and three products of the parts make one of the elements but for
+// 2^-22 of it.  The tensor cores cut off what an addition to a sum loses, so products
+// with a rest have a sum of their own, and sums of few products are added to O by
+// the FMA units.  (Products on the FMA units too took 2 to 3 times as long.)  Tiles come through cp.async, several in flight.  The prefix's jobs
+// of 16-bit elements go to the tcgen05 kernel of prefix_attention_tc.cu where there
+// are rows enough.
 #include "prefix_attention.cuh"
 
 namespace tmac {
@@ -75,201 +81,42 @@ struct Copier {
         }
     }
 };
-// ---------------------------------------------------- 32-bit arithmetic ----
-// Tiles of 8 rows per warp.  A warp takes 16 keys at a time: lane = (key, half
-// of the rows) for the scores, lane = dims for the output.  With up to 8 rows
-// in the job the four warps take different keys of a tile and join at the end;
-// with more they take different rows and share the tile.
-constexpr int kRows = 8, kStep = 16, kSimtStages = 2;
-
-template <int D>
-struct SimtSmem {
-    float q[kWarps * kRows][D];
-    float p[kWarps][kStep][kRows];
-    float alpha[kWarps][kRows];
-    float ml[kWarps][kRows][2];
-    struct {
-        float k[kTile][D + 4];
-        float v[kTile][D];
-    } stage[kSimtStages];
-    Rows<kWarps * kRows> rows;
-};
-
+// ------------------------------------------------------------------ jobs ----
+// Tiles of 16 rows per warp.  With up to 16 rows in the job the four warps take
+// different 16 keys of a tile and join at the end; with more they take different rows.
+// 16-bit weights are rounded to the elements' type for the second product, as the
+// values are.
+constexpr int kMmaRows = 16, kStep = 16;
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) attn_simt_kernel(AttnArgs a)
-{
-    extern __shared__ __align__(16) uint8_t smem[];
-    SimtSmem<D>& sh = *reinterpret_cast<SimtSmem<D>*>(smem);
-    constexpr int kJobRows = kWarps * kRows, kDims = D / 32;
-    Job j;
-    if (!find_job<kJobRows>(a, &j)) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool split_keys = j.rows <= kRows;
-    using Copy = Copier<T, D>;
-    int page = Copy::look_up(a, j, j.tile0);  // of the tile to start next
-    const auto start = [&](int t) {
-        if (t < j.tile1) {
-            auto& st = sh.stage[(t - j.tile0) % kSimtStages];
-            Copy::start(a, j, t, page, [&](int key, int c) { return &st.k[key][c]; }, [&](int key, int c) { return &st.v[key][c]; });
-            page = Copy::look_up(a, j, t + 1);
-        }
-        cp_async_commit();
-    };
-    start(j.tile0);
-    sh.rows.find(a, j);
-    for (int i = threadIdx.x; i < kJobRows * D; i += kThreads) {
-        const int r = i / D, d = i % D;
-        sh.q[r][d] = r < j.rows ? __fmul_rn(a.scale, ((const T*)a.q)[sh.rows.token[r] * a.q_stride + sh.rows.head[r] * D + d]) : 0.0f;
-    }
-
-    const int r0 = split_keys ? 0 : warp * kRows;  // the warp's rows
-    const int half = lane >> 4;                    // this lane's scores: rows half * 4 ..
-    float m[4], l[4], o[kRows][kDims];
-#pragma unroll
-    for (int i = 0; i < 4; i++) m[i] = -INFINITY, l[i] = 0.0f;
-#pragma unroll
-    for (int r = 0; r < kRows; r++)
-#pragma unroll
-        for (int c = 0; c < kDims; c++) o[r][c] = 0.0f;
-
-    for (int t = j.tile0; t < j.tile1; t++) {
-        start(t + 1);
-        cp_async_wait<1>();
-        __syncthreads();
-        auto& st = sh.stage[(t - j.tile0) % kSimtStages];
-        const TileOf tile = find_tile(a, j, t);
-        const int* limits = tile.prefix ? sh.rows.p_limit : sh.rows.o_limit;
-        const int least = tile.prefix ? sh.rows.p_least : sh.rows.o_least;
-        for (int step = split_keys ? warp * kStep : 0; step < (split_keys ? (warp + 1) * kStep : kTile); step += kStep) {
-            if (tile.key0 + step >= tile.keys || r0 >= j.rows) break;
-            const int kk = step + (lane & 15), key = tile.key0 + kk;
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-            for (int d = 0; d < D; d += 4) {
-                const float4 kx = *reinterpret_cast<const float4*>(&st.k[kk][d]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4 qv = *reinterpret_cast<const float4*>(&sh.q[r0 + half * 4 + i][d]);
-                    s[i] = __fmaf_rn(qv.x, kx.x, s[i]);
-                    s[i] = __fmaf_rn(qv.y, kx.y, s[i]);
-                    s[i] = __fmaf_rn(qv.z, kx.z, s[i]);
-                    s[i] = __fmaf_rn(qv.w, kx.w, s[i]);
-                }
-            }
-            float p[4], al[4];
-            bool moved = false;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (key >= limits[r0 + half * 4 + i]) s[i] = -INFINITY;
-                float mx = s[i];
-#pragma unroll
-                for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-                mx = fmaxf(mx, m[i]);
-                al[i] = mx == m[i] ? 1.0f : expf(__fsub_rn(m[i], mx));
-                moved |= mx != m[i];
-                p[i] = s[i] == -INFINITY ? 0.0f : expf(__fsub_rn(s[i], mx));
-                m[i] = mx;
-                l[i] = __fmaf_rn(l[i], al[i], p[i]);
-            }
-            __syncwarp();
-            *reinterpret_cast<float4*>(&sh.p[warp][lane & 15][half * 4]) = make_float4(p[0], p[1], p[2], p[3]);
-            if (__any_sync(0xffffffffu, moved)) {
-                if ((lane & 15) == 0)
-                    *reinterpret_cast<float4*>(&sh.alpha[warp][half * 4]) = make_float4(al[0], al[1], al[2], al[3]);
-                __syncwarp();
-#pragma unroll
-                for (int r = 0; r < kRows; r++)
-#pragma unroll
-                    for (int c = 0; c < kDims; c++) o[r][c] = __fmul_rn(o[r][c], sh.alpha[warp][r]);
-            }
-            __syncwarp();
-            const bool some_masked = tile.key0 + step + kStep > least;
-#pragma unroll 4
-            for (int i = 0; i < kStep; i++) {
-                float pr[kRows], vx[kDims];
-#pragma unroll
-                for (int r = 0; r < kRows; r++) pr[r] = sh.p[warp][i][r];
-#pragma unroll
-                for (int c = 0; c < kDims; c++) vx[c] = st.v[step + i][lane * kDims + c];
-                // a row must not take 0 * inf from a key it does not see
-#pragma unroll
-                for (int r = 0; r < kRows; r++)
-                    if (!some_masked || pr[r] != 0.0f)
-#pragma unroll
-                        for (int c = 0; c < kDims; c++) o[r][c] = __fmaf_rn(pr[r], vx[c], o[r][c]);
-            }
-        }
-        __syncthreads();
-    }
-    // row sums over the 16 key lanes
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int w = 8; w > 0; w >>= 1) l[i] = __fadd_rn(l[i], __shfl_xor_sync(0xffffffffu, l[i], w));
-
-    // the warps' results, joined over the warps when they split the keys
-    cp_async_wait<0>();
-    __syncthreads();
-    float* ow = reinterpret_cast<float*>(&sh.stage[0]);  // [warps][8][D]
-    static_assert(sizeof(float) * kWarps * kRows * D <= sizeof(sh.stage), "join space");
-    if ((lane & 15) == 0)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            sh.ml[warp][half * 4 + i][0] = m[i];
-            sh.ml[warp][half * 4 + i][1] = l[i];
-        }
-#pragma unroll
-    for (int r = 0; r < kRows; r++)
-#pragma unroll
-        for (int c = 0; c < kDims; c++) ow[(warp * kRows + r) * D + lane * kDims + c] = o[r][c];
-    __syncthreads();
-    for (int i = threadIdx.x; i < j.rows * D; i += kThreads) {
-        const int r = i / D, d = i % D;
-        float mx, sum, val;
-        if (split_keys) {
-            mx = -INFINITY;
-            for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, sh.ml[w][r][0]);
-            sum = val = 0.0f;
-            for (int w = 0; w < kWarps; w++) {
-                const float lw = sh.ml[w][r][1];
-                if (lw == 0.0f) continue;  // saw no key
-                const float f = expf(__fsub_rn(sh.ml[w][r][0], mx));
-                sum = __fmaf_rn(f, lw, sum);
-                val = __fmaf_rn(f, ow[(w * kRows + r) * D + d], val);
-            }
-        } else {
-            mx = sh.ml[r / kRows][r % kRows][0];
-            sum = sh.ml[r / kRows][r % kRows][1];
-            val = ow[r * D + d];
-        }
-        const float one[1] = {val};
-        put_results<T, D, 1>(a, j, RowOf{sh.rows.token[r], sh.rows.head[r], 0, 0}, d, mx, sum, one);
-    }
-}
-
-// ------------------------------------------------- 16-bit tensor arithmetic ----
-// Tiles of 16 rows per warp, mma.sync m16n8k16 for both products with 32-bit sums; the weights are rounded to the elements' type for
-// the second, as the values are.  Keys split over the warps as above.
-constexpr int kMmaRows = 16;
+struct MmaConf;
+// 16-bit rows lie unpadded, their 16-byte pieces turned by the row's number: eight
+// rows of one column fall on different banks.
 template <typename T, int D>
-struct MmaConf {
-    static constexpr int kStages = D == 64 ? 4 : 3;
+struct MmaConf16 {
+    static constexpr int kStages = D == 64 ? 4 : 3, kKeyRow = D, kValueRow = D;
     static constexpr int kWide = D == 64 ? 64 : 32;  // keys at a time where warps hold different rows
+    static TMAC_DEV int key_at(int row, int c) { return row * D + ((c / 8 ^ (row & 7)) * 8 | c % 8); }
+    static TMAC_DEV int value_at(int row, int c) { return key_at(row, c); }
+};
+template <int D>
+struct MmaConf<__half, D> : MmaConf16<__half, D> {};
+template <int D>
+struct MmaConf<__nv_bfloat16, D> : MmaConf16<__nv_bfloat16, D> {};
+// 32-bit rows are padded so that the fragments' loads fall on different banks.
+template <int D>
+struct MmaConf<float, D> {
+    static constexpr int kStages = 3, kKeyRow = D + 8, kValueRow = D + 4;
+    static constexpr int kWide = 16;  // 32 is no faster
+    static TMAC_DEV int key_at(int row, int c) { return row * kKeyRow + c; }
+    static TMAC_DEV int value_at(int row, int c) { return row * kValueRow + c; }
 };
 template <typename T, int D>
 struct MmaSmem {
     struct {
-        T k[kTile * D], v[kTile * D];
+        T k[kTile * MmaConf<T, D>::kKeyRow], v[kTile * MmaConf<T, D>::kValueRow];
     } stage[MmaConf<T, D>::kStages];
     float ml[kWarps][kMmaRows][2];
 };
-// 16-byte pieces of a row lie turned by the row's number: eight rows of one column
-// fall on different banks.
-template <int D>
-TMAC_DEV int turned(int row, int c)
-{
-    return row * D + ((c / 8 ^ (row & 7)) * 8 | c % 8);
-}
 TMAC_DEV void ldmatrix4(uint32_t (&r)[4], const void* p)
 {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -296,13 +143,40 @@ TMAC_DEV void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint3
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+TMAC_DEV void mma1688(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x as the nearest tf32 number and the rest, rounded to one (the product reads the
+// upper 19 bits).
+TMAC_DEV void split_tf32(float x, uint32_t& hi, uint32_t& lo)
+{
+    hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi))) + 0x1000u;
+}
+// main += a b without the products of rests, which go to rest; a split already.
+TMAC_DEV void mma_f32(float (&main)[4], float (&rest)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], float b0, float b1)
+{
+    uint32_t h0, l0, h1, l1;
+    split_tf32(b0, h0, l0);
+    split_tf32(b1, h1, l1);
+    mma1688(rest, lo, h0, h1);
+    mma1688(rest, hi, l0, l1);
+    mma1688(main, hi, h0, h1);
+}
+
 template <typename T, int D>
 TMAC_DEV void attn_mma(const AttnArgs& a)
 {
     extern __shared__ __align__(16) uint8_t smem[];
     using Smem = MmaSmem<T, D>;
+    using Conf = MmaConf<T, D>;
     Smem& sh = *reinterpret_cast<Smem*>(smem);
-    constexpr int kJobRows = kWarps * kMmaRows, kStages = MmaConf<T, D>::kStages, kWide = MmaConf<T, D>::kWide, kN = D / 8;
+    constexpr bool k32 = sizeof(T) == 4;
+    constexpr int kJobRows = kWarps * kMmaRows, kStages = Conf::kStages, kN = D / 8;
+    constexpr int kDepth = k32 ? 8 : 16;  // of a product
     Job j;
     if (!find_job<kJobRows>(a, &j)) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c2 = (lane & 3) * 2;
@@ -311,8 +185,8 @@ TMAC_DEV void attn_mma(const AttnArgs& a)
     const auto copy = [&](int t, int page) {
         if (t < j.tile1) {
             auto& st = sh.stage[(t - j.tile0) % kStages];
-            Copy::start(a, j, t, page, [&](int key, int c) { return &st.k[turned<D>(key, c)]; },
-                        [&](int key, int c) { return &st.v[turned<D>(key, c)]; });
+            Copy::start(a, j, t, page, [&](int key, int c) { return &st.k[Conf::key_at(key, c)]; },
+                        [&](int key, int c) { return &st.v[Conf::value_at(key, c)]; });
         }
         cp_async_commit();
     };
@@ -322,9 +196,10 @@ TMAC_DEV void attn_mma(const AttnArgs& a)
 
     // this thread's rows g and g + 8 of the warp's, as the product's first operand
     const int r0 = split_keys ? 0 : warp * kMmaRows;
-    uint32_t q[D / 16][4];
+    // (32 bits: depth t and t + 4 of a product are values 2 t and 2 t + 1, of Q and K alike)
+    uint32_t q[D / kDepth][4];
     int p_limit[2], o_limit[2];
-    const bool pairs = ((uintptr_t)a.q % 4 | a.q_stride % 2) == 0;
+    const bool pairs = ((uintptr_t)a.q % (2 * sizeof(T)) | a.q_stride % 2) == 0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         const int r = r0 + g + 8 * h;
@@ -334,12 +209,16 @@ TMAC_DEV void attn_mma(const AttnArgs& a)
         o_limit[h] = row.o_limit;
         const T* src = (const T*)a.q + row.token * a.q_stride + row.head * D + c2;
 #pragma unroll
-        for (int i = 0; i < D / 16; i++)
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
+        for (int i = 0; i < D / 8; i++) {
+            const T* at = src + 8 * i;
+            if constexpr (k32) {
+                float2 x = make_float2(0.0f, 0.0f);
+                if (r < j.rows) x = pairs ? __ldg(reinterpret_cast<const float2*>(at)) : make_float2(at[0], at[1]);
+                q[i][h] = __float_as_uint(x.x);
+                q[i][2 + h] = __float_as_uint(x.y);
+            } else {
                 uint32_t x = 0;
                 if (r < j.rows) {
-                    const T* at = src + 16 * i + 8 * w;
                     if (pairs) {
                         x = __ldg(reinterpret_cast<const uint32_t*>(at));
                     } else {
@@ -347,8 +226,9 @@ TMAC_DEV void attn_mma(const AttnArgs& a)
                         x = *reinterpret_cast<const uint32_t*>(two);
                     }
                 }
-                q[i][2 * w + h] = x;
+                q[i / 2][2 * (i % 2) + h] = x;
             }
+        }
     }
 #pragma unroll
     for (int i = 0; i < kStages - 1; i++) copy(j.tile0 + i, page[i]);
@@ -356,7 +236,7 @@ TMAC_DEV void attn_mma(const AttnArgs& a)
     // below these limits no row of the warp needs a mask
     const int p_least = __reduce_min_sync(0xffffffffu, min(p_limit[0], p_limit[1]));
     const int o_least = __reduce_min_sync(0xffffffffu, min(o_limit[0], o_limit[1]));
-    const float scale = __fmul_rn(a.scale, 1.44269504f);  // log2 e: exponentials are powers of 2
+    const float scale = k32 ? a.scale : __fmul_rn(a.scale, 1.44269504f);  // log2 e: powers of 2
     float m[2], l[2], o[kN][4];
     bool careful = false;
 again:
@@ -380,15 +260,33 @@ again:
         const auto keys = [&](auto n8, int step) {
             constexpr int kN8 = decltype(n8)::value;
             float s[kN8][4] = {};
+            [[maybe_unused]] float rest[k32 ? kN8 : 1][4] = {};
 #pragma unroll
-            for (int i = 0; i < D / 16; i++)
+            for (int i = 0; i < D / kDepth; i++) {
+                if constexpr (k32) {
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int n = 0; n < kN8; n += 2) {
-                    uint32_t kx[4];  // keys 0-7 and 8-15, two halves of 16 dims each
-                    ldmatrix4(kx, &st.k[turned<D>(step + 8 * n + (lane & 7) + (lane >> 4) * 8, 16 * i + (lane >> 3 & 1) * 8)]);
-                    mma16816<T>(s[n], q[i], kx[0], kx[1]);
-                    mma16816<T>(s[n + 1], q[i], kx[2], kx[3]);
+                    for (int c = 0; c < 4; c++) split_tf32(__uint_as_float(q[i][c]), hi[c], lo[c]);
+#pragma unroll
+                    for (int n = 0; n < kN8; n++) {
+                        const float2 kx = *reinterpret_cast<const float2*>(&st.k[Conf::key_at(step + 8 * n + g, 8 * i + c2)]);
+                        mma_f32(s[n], rest[n], hi, lo, kx.x, kx.y);
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < kN8; n += 2) {
+                        uint32_t kx[4];  // keys 0-7 and 8-15, two halves of 16 dims each
+                        ldmatrix4(kx, &st.k[Conf::key_at(step + 8 * n + (lane & 7) + (lane >> 4) * 8, 16 * i + (lane >> 3 & 1) * 8)]);
+                        mma16816<T>(s[n], q[i], kx[0], kx[1]);
+                        mma16816<T>(s[n + 1], q[i], kx[2], kx[3]);
+                    }
                 }
+            }
+            if constexpr (k32)
+#pragma unroll
+                for (int n = 0; n < kN8; n++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s[n][c] = __fadd_rn(s[n][c], rest[n][c]);
             const bool some_masked = tile.key0 + step + 8 * kN8 > least;
             float al[2];
 #pragma unroll
@@ -407,7 +305,7 @@ again:
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 mx = fmaxf(mx, m[h]);
-                al[h] = mx == m[h] ? 1.0f : exp2_fast(__fsub_rn(m[h], mx));
+                al[h] = mx == m[h] ? 1.0f : power<T>(__fsub_rn(m[h], mx));
                 const float base = mx == -INFINITY ? 0.0f : mx;  // sees nothing yet: all 0
                 float sum = 0.0f;
 #pragma unroll
@@ -415,7 +313,7 @@ again:
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         float& x = s[n][2 * h + c];
-                        x = exp2_fast(__fsub_rn(x, base));
+                        x = power<T>(__fsub_rn(x, base));
                         sum = __fadd_rn(sum, x);
                     }
                 m[h] = mx;
@@ -427,16 +325,35 @@ again:
 #pragma unroll
                     for (int c = 0; c < 4; c++) o[n][c] = __fmul_rn(o[n][c], al[c >> 1]);
             if (!careful) {
+                if constexpr (k32) {
+                    // depth t and t + 4: keys 2 t and 2 t + 1, as the scores lie
+                    uint32_t hi[kN8][4], lo[kN8][4];
 #pragma unroll
-                for (int k = 0; k < kN8; k += 2) {
-                    const uint32_t p[4] = {pack2<T>(s[k][0], s[k][1]), pack2<T>(s[k][2], s[k][3]), pack2<T>(s[k + 1][0], s[k + 1][1]),
-                                           pack2<T>(s[k + 1][2], s[k + 1][3])};
+                    for (int k = 0; k < kN8; k++)
 #pragma unroll
-                    for (int n = 0; n < kN; n += 2) {
-                        uint32_t vx[4];  // keys 0-7 and 8-15 of dims 8n.., then of the next eight
-                        ldmatrix4_trans(vx, &st.v[turned<D>(step + 8 * k + (lane & 15), 8 * n + (lane >> 4) * 8)]);
-                        mma16816<T>(o[n], p, vx[0], vx[1]);
-                        mma16816<T>(o[n + 1], p, vx[2], vx[3]);
+                        for (int c = 0; c < 4; c++) split_tf32(s[k][c >> 1 | (c & 1) << 1], hi[k][c], lo[k][c]);
+#pragma unroll
+                    for (int n = 0; n < kN; n++) {
+                        float sum[4] = {}, small[4] = {};
+#pragma unroll
+                        for (int k = 0; k < kN8; k++)
+                            mma_f32(sum, small, hi[k], lo[k], st.v[Conf::value_at(step + 8 * k + c2, 8 * n + g)],
+                                    st.v[Conf::value_at(step + 8 * k + c2 + 1, 8 * n + g)]);
+#pragma unroll
+                        for (int c = 0; c < 4; c++) o[n][c] = __fadd_rn(o[n][c], __fadd_rn(sum[c], small[c]));
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kN8; k += 2) {
+                        const uint32_t p[4] = {pack2<T>(s[k][0], s[k][1]), pack2<T>(s[k][2], s[k][3]), pack2<T>(s[k + 1][0], s[k + 1][1]),
+                                               pack2<T>(s[k + 1][2], s[k + 1][3])};
+#pragma unroll
+                        for (int n = 0; n < kN; n += 2) {
+                            uint32_t vx[4];  // keys 0-7 and 8-15 of dims 8n.., then of the next eight
+                            ldmatrix4_trans(vx, &st.v[Conf::value_at(step + 8 * k + (lane & 15), 8 * n + (lane >> 4) * 8)]);
+                            mma16816<T>(o[n], p, vx[0], vx[1]);
+                            mma16816<T>(o[n + 1], p, vx[2], vx[3]);
+                        }
                     }
                 }
             } else {
@@ -451,7 +368,7 @@ again:
                             for (int n = 0; n < kN; n++)
 #pragma unroll
                                 for (int c = 0; c < 2; c++) {
-                                    const float v = Elem<T>::load(&st.v[turned<D>(step + 8 * k + 2 * u + c8, 8 * n + c2 + c)]);
+                                    const float v = Elem<T>::load(&st.v[Conf::value_at(step + 8 * k + 2 * u + c8, 8 * n + c2 + c)]);
                                     if (p0 != 0.0f) o[n][c] = __fmaf_rn(p0, v, o[n][c]);
                                     if (p1 != 0.0f) o[n][2 + c] = __fmaf_rn(p1, v, o[n][2 + c]);
                                 }
@@ -461,8 +378,8 @@ again:
         if (split_keys) {
             if (tile.key0 + warp * kStep < tile.keys) keys(std::integral_constant<int, 2>(), warp * kStep);
         } else if (r0 < j.rows) {
-            for (int step = 0; step < kTile && tile.key0 + step < tile.keys; step += kWide)
-                keys(std::integral_constant<int, kWide / 8>(), step);
+            for (int step = 0; step < kTile && tile.key0 + step < tile.keys; step += Conf::kWide)
+                keys(std::integral_constant<int, Conf::kWide / 8>(), step);
         }
     }
     cp_async_wait<0>();
@@ -526,7 +443,7 @@ again:
         for (int w = 0; w < kWarps; w++) {
             const float lw = sh.ml[w][r][1];
             if (lw == 0.0f) continue;  // saw no key
-            const float f = exp2_fast(__fsub_rn(sh.ml[w][r][0], mx));
+            const float f = power<T>(__fsub_rn(sh.ml[w][r][0], mx));
             const float4 x = *reinterpret_cast<const float4*>(&ow[(w * kMmaRows + r) * D + d]);
             sum = __fmaf_rn(f, lw, sum);
             val[0] = __fmaf_rn(f, x.x, val[0]);
@@ -625,7 +542,7 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(AttnArgs a)
 // How the work is cut.
 int plan(AttnArgs* a, int type, int sms)
 {
-    const int job_rows = type == TMAC_TYPE_F32 ? kWarps * kRows : kWarps * kMmaRows;
+    constexpr int job_rows = kWarps * kMmaRows;
     const int hk = a->cache.kv_heads;
     const auto tiles = [](int keys) { return (keys + kTile - 1) / kTile; };
     // key ranges so that there are about `per_sm` jobs per SM, of a tile at least
@@ -641,7 +558,7 @@ int plan(AttnArgs* a, int type, int sms)
     a->o_tiles = (int)(((int64_t)a->max_q * a->group + job_rows - 1) / job_rows);
     const int64_t o_jobs = (int64_t)a->batch * a->o_tiles * hk;
     const int all_tiles = tiles(a->prefix_len) + tiles(a->max_own);
-    a->alone = all_tiles <= kAloneTiles;
+    a->alone = all_tiles <= (type == TMAC_TYPE_F32 ? kAloneTiles32 : kAloneTiles16);
     if (a->alone) {
         a->p_tiles = a->p_splits = 0;
         a->o_splits = 1;
@@ -672,22 +589,15 @@ int launch_attention(const AttnArgs& a, cudaStream_t s)
     const int64_t o_jobs = (int64_t)a.batch * a.o_tiles * a.cache.kv_heads * a.o_splits;
     if (a.p_jobs + o_jobs > 0x7FFFFFFF) return fail(TMAC_ERR_SHAPE, "too many jobs for one grid");
     AttnArgs rest = a;  // without the prefix's jobs, where the tcgen05 kernel takes them
-    if (a.tc) {
+    if (a.tc) {  // 16-bit elements
         const int rc = launch_prefix_tc(a, std::is_same_v<T, __half> ? TMAC_TYPE_F16 : TMAC_TYPE_BF16, s);
         if (rc) return rc;
         rest.p_jobs = 0;
     }
     const int64_t jobs = rest.p_jobs + o_jobs;
     if (jobs) {
-        size_t smem;
-        void (*fn)(AttnArgs);
-        if constexpr (sizeof(T) == 4) {
-            fn = attn_simt_kernel<T, D>;
-            smem = sizeof(SimtSmem<D>);
-        } else {
-            fn = attn_mma_kernel<T, D>;
-            smem = sizeof(MmaSmem<T, D>);
-        }
+        constexpr size_t smem = sizeof(MmaSmem<T, D>);
+        auto fn = attn_mma_kernel<T, D>;
         static std::atomic<uint64_t> done{0};
         const int rc = set_once(done, a.device, [&] {
             return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);

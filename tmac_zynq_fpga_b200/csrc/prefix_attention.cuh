@@ -75,8 +75,10 @@ TMAC_DEV int sequence_of(const AttnArgs& a, int token)
     return lo;
 }
 
-// Up to so many key tiles (prefix and own) every sequence reads the prefix itself, in one job.
-constexpr int kAloneTiles = 8;
+// Up to so many key tiles (prefix and own) every sequence reads the prefix itself, in
+// one job.  Against shared and joined jobs: 16 bits, 3 tiles 6.5 / 8.2 us, 5 tiles 8.3 /
+// 9.4, 9 tiles 9.5 / 9.5; 32 bits, 8 tiles 17.1 / 12.3.
+constexpr int kAloneTiles16 = 8, kAloneTiles32 = 4;
 // From so many query rows on the prefix goes to the tcgen05 kernel.
 constexpr int kTcLeast = 48;
 constexpr int kTile = 64, kWarps = 4, kThreads = kWarps * 32;
@@ -150,30 +152,6 @@ TMAC_DEV RowOf find_row(const AttnArgs& a, const Job& j, int r)
     }
     return o;
 }
-// Rows of a job as the kernels keep them in shared memory.
-template <int kJobRows>
-struct Rows {
-    int token[kJobRows], head[kJobRows], p_limit[kJobRows], o_limit[kJobRows];
-    int p_least, o_least;  // smallest limits: tiles below them need no mask
-    TMAC_DEV void find(const AttnArgs& a, const Job& j)
-    {
-        if (threadIdx.x == 0) p_least = o_least = 0x7FFFFFFF;
-        __syncthreads();
-        for (int r = threadIdx.x; r < kJobRows; r += blockDim.x) {
-            RowOf o = {0, 0, 0, 0};
-            if (r < j.rows) {
-                o = find_row(a, j, r);
-                atomicMin(&p_least, o.p_limit);
-                atomicMin(&o_least, o.o_limit);
-            }
-            token[r] = o.token;
-            head[r] = o.head;
-            p_limit[r] = o.p_limit;
-            o_limit[r] = o.o_limit;
-        }
-        __syncthreads();
-    }
-};
 // Where tile t's keys lie: the page list, the first key's number in it, the keys in reach.
 struct TileOf {
     const int* pages;
