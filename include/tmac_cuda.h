@@ -576,7 +576,7 @@ int tmac_prefix_attention_workspace(const tmac_paged_cache* cache, int heads, in
  * temperature not above 0 (or its reciprocal infinite): the lowest index of the
  * largest logit.  A row without any logit above -inf: token -1, probability 0.
  *   logits: [batch] rows of `vocab` (up to 720000) values of `type`, row_stride in
- *           elements.  temperature, top_p, min_p: optional float [batch]; top_k:
+ *           elements (0: all rows are the same one).  temperature, top_p, min_p: optional float [batch]; top_k:
  *           optional int32 [batch]; u: float [batch] in [0, 1).
  *   tokens: int32 [batch]; probs: float [batch].
  */

@@ -576,6 +576,14 @@ def test_sample_strided_rows():
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_sample_of_one_row_for_many_draws():
+    row = random_logits(1, 6000)
+    u = torch.rand(50, device="cuda")
+    k = torch.full((50,), 12, dtype=torch.int32, device="cuda")
+    a, b = tm.sample(row.expand(50, -1), u, top_k=k), tm.sample(row.repeat(50, 1), u, top_k=k)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_sample_is_uniform_in_u():
     """Evenly spread u gives every kept token its weight's share of the draws."""
     logits = random_logits(1, 50, scale=1.0)
