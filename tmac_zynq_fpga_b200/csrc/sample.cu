@@ -43,6 +43,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 512;
 constexpr float kBinScale = 22.5f;  // bins per unit of d in the first round; d < 22.2 where w > 0
 constexpr int kCluster = 8, kMaxCluster = 16, kMaxSlice = 45000, kMaxVocab = kMaxCluster * kMaxSlice;
 constexpr int kList = 2048;                                    // tokens gathered in one CTA
+constexpr int kFew = 256;                                      // of these, so many are ordered by counting
 constexpr int kSteps = 64, kFirstStep = (127 - 4) << 3;        // bounds on d, eight to an octave from 1/16 to 16
 static_assert(kThreads >= kBins && kThreads * kMaxCluster / kBins <= 32, "the threads of a bin are lanes of a warp");
 static_assert(kBins / kMaxCluster % 32 == 0, "a share's bins go to the lanes of a warp");
@@ -66,10 +67,16 @@ struct SampleArgs {
 };
 
 struct Shared {
-    uint32_t cnt[kBins], hi[kBins], lo[kBins];  // this CTA's histogram: counts, weights in two words
+    union {
+        struct {
+            uint32_t cnt[kBins], hi[kBins], lo[kBins];  // this CTA's histogram: counts, weights in two words
+        };
+        alignas(16) unsigned long long pairs[2 * kFew];  // of count_before, when the histogram has been searched
+    };
     uint32_t mcnt[kBins];                       // this CTA's share of the bins, summed over the cluster
     unsigned long long mw[kBins];
     unsigned long long key[kList];  // gathered tokens: bits(d) << 32 | index
+    uint32_t n_few;
     unsigned long long share_w, red_w[kWarps];
     uint32_t share_c, red_c[kWarps];
     float red_f[kWarps], cta_max;
@@ -195,6 +202,47 @@ TMAC_DEV unsigned long long block_scan(unsigned long long v, unsigned long long*
     }
     *total = all;
     return before + up - v;
+}
+
+// Running sums in the order of few keys, by counting: threads 0 .. n - 1 hold a key
+// and a weight each; *rank and *before get the number of smaller keys and their weight.
+// `pairs` has room for 2 n numbers.
+TMAC_DEV void count_before(unsigned long long* pairs, int n, unsigned long long key, unsigned long long w, int* rank,
+                           unsigned long long* before)
+{
+    __syncthreads();
+    if ((int)threadIdx.x < n) {
+        pairs[2 * threadIdx.x] = key;
+        pairs[2 * threadIdx.x + 1] = w;
+    }
+    __syncthreads();
+    int r = 0;
+    unsigned long long b = 0;
+    if ((int)threadIdx.x < n) {
+        const ulonglong2* p = reinterpret_cast<const ulonglong2*>(pairs);
+#pragma unroll 4
+        for (int k = 0; k < n; k++) {
+            const ulonglong2 o = p[k];
+            const bool less = o.x < key;
+            r += less;
+            b += less ? o.y : 0;
+        }
+    }
+    *rank = r;
+    *before = b;
+}
+// The sum over the first n threads' v, n up to kFew, to all.
+TMAC_DEV unsigned long long sum_few(unsigned long long v, int n, unsigned long long* red)
+{
+    __syncthreads();
+    if ((int)(threadIdx.x & ~31u) < n) {
+        v = warp_sum((int)threadIdx.x < n ? v : 0);
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    }
+    __syncthreads();
+    unsigned long long s = 0;
+    for (int i = 0; i < (n + 31) / 32; i++) s += red[i];
+    return s;
 }
 
 template <typename T, bool kResident>
@@ -380,12 +428,14 @@ struct Row {
     // Copies every rank's listed tokens into this CTA's keys.
     TMAC_DEV void gather() const
     {
-        uint32_t at = 0;
-        for (int r = 0; r < ranks; r++) {
-            const uint32_t c = cl.map_shared_rank(sh, r)->n_local;
+        const int lane = threadIdx.x & 31;
+        const uint32_t c = lane < ranks ? cl.map_shared_rank(sh, lane)->n_local : 0, up = warp_scan(c);
+        for (int r = 0; r < ranks; r++) {  // a warp to a rank, or several
+            const uint32_t count = __shfl_sync(0xffffffffu, c, r), at = __shfl_sync(0xffffffffu, up - c, r);
             const unsigned long long* from = cl.map_shared_rank(local, r);
-            for (uint32_t i = threadIdx.x; i < c; i += kThreads) sh->key[at + i] = from[i];
-            at += c;
+            const int part = kWarps / ranks, warp = threadIdx.x >> 5;
+            if (warp / part == r)
+                for (uint32_t i = warp % part * 32 + lane; i < count; i += part * 32) sh->key[at + i] = from[i];
         }
         __syncthreads();
     }
@@ -404,8 +454,7 @@ struct Row {
                 const unsigned long long w = weight_of(weight_exp(e[i]));
                 if (!w) continue;
                 if (kCounts) atomicAdd(&sh->cnt[b], 1u);
-                const uint32_t low = (uint32_t)w, carry = atomicAdd(&sh->lo[b], low) > 0xFFFFFFFFu - low;
-                if (carry + (w >> 32)) atomicAdd(&sh->hi[b], carry + (uint32_t)(w >> 32));
+                add_weight(b, w);
             }
         });
         cl.sync();
@@ -531,7 +580,7 @@ struct Row {
         const int n = listed(&offset);
         if (n >= 0) {
             gather();
-            cut_list(n, k ? k - before_c : 0, t, before_w);
+            cut_list(n, cut.from, cut.to, k ? k - before_c : 0, t, before_w);
             cl.sync();  // the lists are free again
             cut.last = sh->cut_key;
             cut.weight = sh->cut_weight;
@@ -578,9 +627,74 @@ struct Row {
         return cut;
     }
 
-    // Cuts the n gathered tokens after their first k (k > 0), or where base plus their
-    // running weight reaches t: cut_key, and cut_weight with base.
-    TMAC_DEV void cut_list(int n, uint32_t k, double t, unsigned long long base)
+    // Cuts the n gathered tokens, with d from `from` to `to`, after their first k (k >
+    // 0), or where base plus their running weight reaches t: cut_key, and cut_weight
+    // with base.  Many are first narrowed to the one of kBins parts that holds the cut.
+    TMAC_DEV void cut_list(int n, float from, float to, uint32_t k, double t, unsigned long long base)
+    {
+        if (n > kFew) {
+            const float scale = __fdiv_rn((float)(kBins - 1), __fsub_rn(to, from));
+            const auto part_of = [&](unsigned long long key) {
+                return min(max((int)__fmul_rn(__fsub_rn(__uint_as_float((uint32_t)(key >> 32)), from), scale), 0), kBins - 1);
+            };
+            for (int i = threadIdx.x; i < kBins; i += kThreads) sh->cnt[i] = sh->hi[i] = sh->lo[i] = 0;
+            if (threadIdx.x == 0) sh->n_few = 0;
+            __syncthreads();
+            for (int i = threadIdx.x; i < n; i += kThreads) {
+                const int part = part_of(sh->key[i]);
+                add_weight(part, weight_of(weight_exp(__uint_as_float((uint32_t)(sh->key[i] >> 32)))));
+                atomicAdd(&sh->cnt[part], 1u);
+            }
+            __syncthreads();
+            // a part to a thread
+            unsigned long long all;
+            const uint32_t c = threadIdx.x < kBins ? sh->cnt[threadIdx.x] : 0;
+            const unsigned long long w = threadIdx.x < kBins ? ((unsigned long long)sh->hi[threadIdx.x] << 32) + sh->lo[threadIdx.x] : 0;
+            const uint32_t before_c = (uint32_t)block_scan(c, sh->red_w, &all);
+            const unsigned long long before_w = base + block_scan(w, sh->red_w, &all);
+            if (k ? before_c < k && k <= before_c + c : (double)before_w < t && (double)(before_w + w) >= t) {
+                sh->found_bin = threadIdx.x;
+                sh->before_c = before_c;
+                sh->before_w = before_w;
+            }
+            __syncthreads();
+            const int part = sh->found_bin;
+            for (int i = threadIdx.x; i < n; i += kThreads)
+                if (part_of(sh->key[i]) == part) {
+                    const uint32_t at = atomicAdd(&sh->n_few, 1u);
+                    if (at < kFew) sh->pairs[at] = sh->key[i];
+                }
+            __syncthreads();
+            if (sh->n_few <= kFew) {
+                n = (int)sh->n_few;
+                if (k) k -= sh->before_c;
+                base = sh->before_w;
+                if ((int)threadIdx.x < n) sh->key[threadIdx.x] = sh->pairs[threadIdx.x];
+                __syncthreads();
+            }
+        }
+        if (n <= kFew) {
+            const unsigned long long mine = (int)threadIdx.x < n ? sh->key[threadIdx.x] : ~0ull;
+            const unsigned long long w = (int)threadIdx.x < n ? weight_of(weight_exp(__uint_as_float((uint32_t)(mine >> 32)))) : 0;
+            unsigned long long before;
+            int rank;
+            count_before(sh->pairs, n, mine, w, &rank, &before);
+            before += base;
+            if ((int)threadIdx.x < n && (k ? rank == (int)k - 1 : (double)before < t && (double)(before + w) >= t)) {
+                sh->cut_key = mine;
+                sh->cut_weight = before + w;
+            }
+            __syncthreads();
+            return;
+        }
+        sort_and_cut(n, k, t, base);
+    }
+    TMAC_DEV void add_weight(int bin, unsigned long long w)
+    {
+        const uint32_t low = (uint32_t)w, carry = atomicAdd(&sh->lo[bin], low) > 0xFFFFFFFFu - low;
+        if (carry + (w >> 32)) atomicAdd(&sh->hi[bin], carry + (uint32_t)(w >> 32));
+    }
+    TMAC_DEV void sort_and_cut(int n, uint32_t k, double t, unsigned long long base)
     {
         constexpr int kPer = kList / kThreads;
         sort_keys(sh->key, n);
@@ -609,8 +723,30 @@ struct Row {
 // The cuts and the draw over the n gathered tokens, the first k of the order among them.
 TMAC_DEV void draw_from_list(const SampleArgs& a, Shared* sh, int b, int n, int k, float p, float m)
 {
-    constexpr int kPer = kList / kThreads;
     unsigned long long* key = sh->key;
+    if (n <= kFew) {
+        __syncthreads();
+        const unsigned long long mine = (int)threadIdx.x < n ? key[threadIdx.x] : ~0ull;
+        const float e = (int)threadIdx.x < n ? weight_exp(__uint_as_float((uint32_t)(mine >> 32))) : 0.0f;
+        unsigned long long w = (int)threadIdx.x < n ? weight_of(e) : 0, before;
+        int rank;
+        count_before(sh->pairs, n, mine, w, &rank, &before);
+        bool kept = (int)threadIdx.x < n && rank < k;
+        if (p < 1.0f) {
+            const unsigned long long all = sum_few(kept ? w : 0, n, sh->red_w);
+            kept = kept && ((double)before < __dmul_rn((double)p, (double)all) || rank == 0);
+        }
+        kept = kept && (e >= m || rank == 0);
+        if (!kept) w = 0;
+        const unsigned long long all = sum_few(w, n, sh->red_w), pick = pick_of(a.u[b], all);
+        count_before(sh->pairs, n, mine & 0xFFFFFFFFu, w, &rank, &before);  // in the order of the indexes
+        if (before <= pick && pick < before + w) {
+            a.tokens[b] = (int)(uint32_t)mine;
+            a.probs[b] = (float)__ddiv_rn((double)w, (double)all);
+        }
+        return;
+    }
+    constexpr int kPer = kList / kThreads;
     if (threadIdx.x == 0) sh->n_keep = 1;
     sort_keys(key, n);
     const int n_k = min(k, n);
@@ -800,6 +936,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
         if (step < kSteps) atomicAdd(&sh->maxima[max(step, 0)], 1u);
         row.cl.sync();
         uint32_t c0 = 0, c1 = 0;
+#pragma unroll 8
         for (int r = 0; r < row.ranks; r++) {
             const uint2 c = reinterpret_cast<const uint2*>(row.cl.map_shared_rank(sh, r)->maxima)[lane];
             c0 += c.x;
