@@ -106,7 +106,8 @@ TMAC_DEV unsigned long long weight_of(float e)
     // the conversion saturates at 2^32 - 1, which e = 1 alone reaches
     return (unsigned long long)(uint32_t)__float2uint_rz(__fmul_rn(e, 4294967296.0f)) + (e >= 1.0f);
 }
-TMAC_DEV int first_bin(float d) { return min((int)__fmul_rn(d, kBinScale), kBins - 1); }
+// Tokens of weight 0 lie past the last bin: they are asked for only where it does not matter.
+TMAC_DEV int first_bin(float d) { return __float2int_rz(__fmul_rn(d, kBinScale)); }
 
 // The first part of a row's order that is kept: first_bin(d) < bin, or == bin and
 // (bits(d), index) up to `last`.
@@ -348,9 +349,9 @@ struct Row {
         cl.sync();
     }
 
-    // The token at which the running sum of f(d, index), over the cluster in the order
-    // of the indexes, passes pick_of_total(total); the thread that holds it calls
-    // found(index, f of it, total).
+    // The token at which the running sum of the weights, over the cluster in the order of
+    // the indexes, passes pick_of_total(total); f(d, index, w) sets the weights w of four
+    // tokens from `index` on, and the thread that holds the token calls found(index, w, total).
     template <typename F, typename P, typename G>
     TMAC_DEV void draw(F&& f, P&& pick_of_total, G&& found)
     {
@@ -360,8 +361,9 @@ struct Row {
         for (int c = warp; c < n_chunks; c += kWarps) {
             unsigned long long s = 0;
             vectors(c * L::kChunkVecs + lane, min(vectors(), (c + 1) * L::kChunkVecs), 32, [&](const float (&e)[4], int j) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) s += f(e[i], begin + j + i);
+                unsigned long long w[4];
+                f(e, begin + j, w);
+                s += (w[0] + w[1]) + (w[2] + w[3]);
             });
             s = warp_sum(s);
             if (lane == 0) chunks[c] = s;
@@ -393,8 +395,7 @@ struct Row {
             if (threadIdx.x < L::kChunkVecs && v < vectors()) {
                 const float4 q = load4(v);
                 const float e[4] = {d_of(q.x), d_of(q.y), d_of(q.z), d_of(q.w)};
-#pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = f(e[i], begin + 4 * v - pad + i);
+                f(e, begin + 4 * v - pad, w);
             }
             unsigned long long at = sh->chunk_before + block_scan(w[0] + w[1] + w[2] + w[3], sh->red_w, &sum);
 #pragma unroll
@@ -408,7 +409,12 @@ struct Row {
     // The index of the m-th element (from 1) with bits(d) == key, over the cluster.
     TMAC_DEV int tie(uint32_t key, uint32_t m)
     {
-        draw([&](float v, int) -> unsigned long long { return __float_as_uint(v) == key; }, [&](unsigned long long) { return m - 1; },
+        draw(
+            [&](const float (&e)[4], int, unsigned long long (&w)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = __float_as_uint(e[i]) == key;
+            },
+            [&](unsigned long long) { return m - 1; },
              [&](int index, unsigned long long, unsigned long long) {
                  for (int r = 0; r < ranks; r++) cl.map_shared_rank(sh, r)->tie_index = index;
              });
@@ -449,10 +455,10 @@ struct Row {
         vectors(threadIdx.x, vectors(), kThreads, [&](const float (&e)[4], int) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const int b = bin_of(e[i]);
-                if (b < 0) continue;
                 const unsigned long long w = weight_of(weight_exp(e[i]));
                 if (!w) continue;
+                const int b = bin_of(e[i]);
+                if (b < 0) continue;
                 if (kCounts) atomicAdd(&sh->cnt[b], 1u);
                 add_weight(b, w);
             }
@@ -559,12 +565,10 @@ struct Row {
     TMAC_DEV Cut select(uint32_t k, float p, unsigned long long of)
     {
         Cut cut;
-        // far tokens (all of weight 0) fill the last bin: leave them out
-        const auto bin_of = [&](float v) { const int c = first_bin(v); return c < kBins - 1 ? c : -1; };
         if (k)
-            histogram<true>(bin_of);
+            histogram<true>([](float v) { return first_bin(v); });
         else
-            histogram<false>(bin_of);
+            histogram<false>([](float v) { return first_bin(v); });
         const int lane = threadIdx.x & 31;
         const unsigned long long row_w = warp_sum(lane < ranks ? cl.map_shared_rank(sh, lane)->share_w : 0);
         const double t = __dmul_rn((double)p, (double)(of ? of : row_w));
@@ -972,14 +976,28 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
         a.tokens[b] = index;
         a.probs[b] = (float)__ddiv_rn((double)w, (double)total);
     };
+    // no kept token lies as far: a bound on exp(-d) >= m, a little wide, and on the cut
+    const float farthest = fminf(cut.to, m > 0.0f ? __fadd_rn(__fmul_rn(-logf(m), 1.0001f), 1e-4f) : INFINITY);
     if (cut.bin == kBins && m == 0.0f)
-        row.draw([](float d, int) { return weight_of(weight_exp(d)); }, pick, found);
+        row.draw(
+            [](const float (&d)[4], int, unsigned long long (&w)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = weight_of(weight_exp(d[i]));
+            },
+            pick, found);
     else
         row.draw(
-            [&](float d, int index) -> unsigned long long {
-                if (!kept_by(cut, d, index)) return 0;
-                const float e = weight_exp(d);
-                return e >= m ? weight_of(e) : 0;
+            [&](const float (&d)[4], int index, unsigned long long (&w)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = 0;
+                if (!(fminf(fminf(d[0], d[1]), fminf(d[2], d[3])) < farthest)) return;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (!(d[i] < farthest)) continue;
+                    if (d[i] >= cut.from && !kept_by(cut, d[i], index + i)) continue;
+                    const float e = weight_exp(d[i]);
+                    if (e >= m) w[i] = weight_of(e);
+                }
             },
             pick, found);
 }
