@@ -79,8 +79,13 @@ TMAC_DEV int sequence_of(const AttnArgs& a, int token)
 // one job.  Against shared and joined jobs: 16 bits, 3 tiles 6.5 / 8.2 us, 5 tiles 8.3 /
 // 9.4, 9 tiles 9.5 / 9.5; 32 bits, 8 tiles 17.1 / 12.3.
 constexpr int kAloneTiles16 = 8, kAloneTiles32 = 4;
-// From so many query rows on the prefix goes to the tcgen05 kernel.
-constexpr int kTcLeast = 48;
+// The prefix goes to the tcgen05 kernel from so many rows on, and from so much work
+// (rows x keys x kv heads): at 64 dims 1.4 M took 13.2 us there and 11.8 in the mma
+// kernel, 3.7 M 15.4 and 15.4, 7.3 M 20.7 and 22.0, 59 M 51 and 85; at 128 dims 0.4 M 14.3
+// and 13.0, 1.7 M 21 and 29, 8.4 M 35 and 43.
+constexpr int kTcRowsLeast = 48;
+constexpr int64_t kTcWork64 = 4000000, kTcWork128 = 1000000;
+constexpr int kTcRange = 4;  // tiles of its job at least: below, its start outweighs them
 constexpr int kTile = 64, kWarps = 4, kThreads = kWarps * 32;
 
 // A job's rows and keys, the same for every kernel.
