@@ -18,10 +18,12 @@
 // as they are; a 32-bit one is split into the nearest tf32 number and the rest
 // rounded to one, and three products of the parts make one of the elements but for
 // 2^-22 of it.  The tensor cores cut off what an addition to a sum loses, so products
-// with a rest have a sum of their own, and sums of few products are added to O by
-// the FMA units.  (Products on the FMA units too took 2 to 3 times as long.)  Tiles come through cp.async, several in flight.  The prefix's jobs
-// of 16-bit elements go to the tcgen05 kernel of prefix_attention_tc.cu where there
-// are rows enough.
+// with a rest have a sum of their own, and sums of few products are added to the
+// scores and to O by the FMA units: half the plain form's error against 64 bits (sums
+// over a whole head of 128 on the tensor cores had 1.4 times it, and took as long).
+// (Products on the FMA units too took 2 to 3 times as long.)  Tiles come through
+// cp.async, several in flight.  The prefix's jobs of 16-bit elements go to the tcgen05
+// kernel of prefix_attention_tc.cu where there are rows enough.
 #include "prefix_attention.cuh"
 
 namespace tmac {
@@ -260,7 +262,8 @@ again:
         const auto keys = [&](auto n8, int step) {
             constexpr int kN8 = decltype(n8)::value;
             float s[kN8][4] = {};
-            [[maybe_unused]] float rest[k32 ? kN8 : 1][4] = {};
+            constexpr int kChain = 4;  // 32-bit products in a row on the tensor cores
+            [[maybe_unused]] float main[k32 ? kN8 : 1][4] = {}, rest[k32 ? kN8 : 1][4] = {};
 #pragma unroll
             for (int i = 0; i < D / kDepth; i++) {
                 if constexpr (k32) {
@@ -270,8 +273,16 @@ again:
 #pragma unroll
                     for (int n = 0; n < kN8; n++) {
                         const float2 kx = *reinterpret_cast<const float2*>(&st.k[Conf::key_at(step + 8 * n + g, 8 * i + c2)]);
-                        mma_f32(s[n], rest[n], hi, lo, kx.x, kx.y);
+                        mma_f32(main[n], rest[n], hi, lo, kx.x, kx.y);
                     }
+                    if (i % kChain == kChain - 1)
+#pragma unroll
+                        for (int n = 0; n < kN8; n++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++) {
+                                s[n][c] = __fadd_rn(s[n][c], __fadd_rn(main[n][c], rest[n][c]));
+                                main[n][c] = rest[n][c] = 0.0f;
+                            }
                 } else {
 #pragma unroll
                     for (int n = 0; n < kN8; n += 2) {
@@ -282,11 +293,6 @@ again:
                     }
                 }
             }
-            if constexpr (k32)
-#pragma unroll
-                for (int n = 0; n < kN8; n++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) s[n][c] = __fadd_rn(s[n][c], rest[n][c]);
             const bool some_masked = tile.key0 + step + 8 * kN8 > least;
             float al[2];
 #pragma unroll
