@@ -527,6 +527,57 @@ def test_sample_ties_at_the_cut(vocab):
     check_sample(logits, p=0.5)
 
 
+def shaped_logits(shape, vocab):
+    """A row whose likely tokens lie as `shape` says: any bound taken from a part of the row can then be far off."""
+    row = random_logits(1, vocab, seed=3)[0]
+    if shape == "falling":
+        row = row.sort(descending=True).values
+    elif shape == "rising":
+        row = row.sort().values
+    elif shape == "early":  # the first quarter above all others
+        row[: vocab // 4] += 20.0
+    elif shape == "late":
+        row[-9:] += 20.0
+    elif shape == "ties":
+        row = (row / 2).round() * 2
+    elif shape == "masked":
+        row[: vocab // 2] = -INF
+        row[vocab // 2 :: 3] = NAN
+    elif shape == "equal":
+        row[:] = -2.5
+    elif shape == "wide":
+        row *= 8
+    return row[None].contiguous()
+
+
+# more rows than the SMs hold: logits are read again, by one to four CTAs a row
+@pytest.mark.parametrize("draws", [60, 300])
+@pytest.mark.parametrize("vocab", [4099, 32003])
+@pytest.mark.parametrize("shape", ["random", "falling", "rising", "early", "late", "ties", "masked", "equal", "wide"])
+@pytest.mark.parametrize("f", [dict(k=2), dict(k=40), dict(k=199, p=0.9), dict(k=700), dict(p=0.8), dict(m=0.05), dict()], ids=str)
+def test_sample_of_many_rows(f, shape, vocab, draws):
+    check_sample(shaped_logits(shape, vocab), draws=draws, **f)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("k", [2, 40, 199])
+def test_sample_of_many_16_bit_rows(dtype, k):
+    check_sample(random_logits(1, 32003, dtype), draws=100, k=k)
+
+
+def test_sample_of_many_rows_with_infinite_ones():
+    logits = random_logits(200, 5000)
+    logits[:100, 4000] = INF       # past the first quarter
+    logits[50:100, 10] = INF       # and in it
+    logits[100:150] = -INF
+    tokens, probs = sample_one(logits, u=[0.6] * 200, top_k=[30] * 200)
+    assert tokens[:50] == [4000] * 50 and probs[:50] == [1.0] * 50
+    assert tokens[50:100] == [4000] * 50 and probs[50:100] == [0.5] * 50
+    assert tokens[100:150] == [-1] * 50 and probs[100:150] == [0.0] * 50
+    for row, token in zip(logits[150:], tokens[150:]):
+        assert token in row.topk(30).indices.tolist()
+
+
 def test_sample_masked_rows():
     v = 5000
     logits = random_logits(7, v)

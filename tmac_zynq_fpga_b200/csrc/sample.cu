@@ -21,6 +21,9 @@
 //  * top-k: the k-th largest of the threads' own maxima bounds the k-th largest
 //    logit from below, and closely, since a thread holds a few dozen logits.  The
 //    tokens above the bound are gathered in one CTA, sorted, and the draw ends there.
+//    Rows that are not held list the tokens in the pass that finds the maxima, above a
+//    bound from the row's first quarter, and read the logits again only where that
+//    bound proves too high (k up to 200 of 256 x 151936: 54 us, 74 with the second pass).
 //  * top-p alone: its cut may lie anywhere, so a histogram of the weights over d
 //    (bins of 1/22) is summed through distributed shared memory; every CTA then
 //    gathers and sorts the tokens of the one bin that holds the cut.
@@ -44,13 +47,15 @@ constexpr float kBinScale = 22.5f;  // bins per unit of d in the first round; d 
 constexpr int kCluster = 8, kMaxCluster = 16, kMaxSlice = 45000, kMaxVocab = kMaxCluster * kMaxSlice;
 constexpr int kList = 2048;                                    // tokens gathered in one CTA
 constexpr int kFew = 256;                                      // of these, so many are ordered by counting
-constexpr int kSteps = 64, kFirstStep = (127 - 4) << 3;        // bounds on d, eight to an octave from 1/16 to 16
 static_assert(kThreads >= kBins && kThreads * kMaxCluster / kBins <= 32, "the threads of a bin are lanes of a warp");
 static_assert(kBins / kMaxCluster % 32 == 0, "a share's bins go to the lanes of a warp");
 // Resident rows list up to 512 tokens per CTA and keep their x; others have the room for more.
 template <bool kResident>
 struct Layout {
     static constexpr int kLocal = kResident ? 512 : kList;
+    // Steps of the bounds on d, from 1/16 to 16: 8 or 16 to an octave.  The finer ones
+    // list fewer tokens, but eight CTAs read each other's counts: 9.8 and 11.6 us a row.
+    static constexpr int kStepShift = kResident ? 20 : 19, kSteps = kResident ? 64 : 128, kFirstStep = (127 - 4) << (23 - kStepShift);
     static constexpr int kChunkVecs = kResident ? 64 : 256;  // float4 of a chunk of the draw
     static constexpr int kChunks = ((kResident ? kMaxSlice : kMaxVocab) + 6) / (4 * kChunkVecs) + 1;
 };
@@ -79,9 +84,9 @@ struct Shared {
     uint32_t n_few;
     unsigned long long share_w, red_w[kWarps];
     uint32_t share_c, red_c[kWarps];
-    float red_f[kWarps], cta_max;
+    float red_f[kWarps], cta_max, least;  // least: every token of this CTA whose x is no less is listed
     int cta_min_index;
-    alignas(8) uint32_t maxima[kSteps];  // the threads' maxima by their distance from the row's
+    alignas(16) uint32_t maxima[Layout<false>::kSteps];  // the threads' maxima by their distance from the row's
     uint32_t n_local;                    // listed tokens; more than kLocal: not all of them
     uint32_t n_keep;
     unsigned long long kept, cut_weight, cut_key;
@@ -346,6 +351,97 @@ struct Row {
                         if (at < L::kLocal) local[at] = order_key(e[c], begin + j + c);
                     }
         });
+        cl.sync();
+    }
+
+    // The bound below which, by `maxima`, k of the threads have their maximum's distance, or inf.
+    // Steps of a lane, and what counts_of gives: their counts.
+    static constexpr int kMine = L::kSteps / 32;
+    using Counts = std::conditional_t<kMine == 4, uint4, uint2>;
+    template <typename F>
+    static TMAC_DEV float bound_of(uint32_t k, F&& counts_of)
+    {
+        const Counts c = counts_of();
+        uint32_t n[kMine], all = 0;
+#pragma unroll
+        for (int i = 0; i < kMine; i++) n[i] = all += reinterpret_cast<const uint32_t*>(&c)[i];
+        const uint32_t up = warp_scan(all), hit = __ballot_sync(0xffffffffu, up >= k);
+        if (!hit) return INFINITY;
+        int less = 0;
+#pragma unroll
+        for (int i = 0; i < kMine - 1; i++) less += up - all + n[i] < k;
+        const int at = __ffs(hit) - 1, step = kMine * at + __shfl_sync(0xffffffffu, less, at);
+        return __uint_as_float((uint32_t)(L::kFirstStep + step + 1) << L::kStepShift);
+    }
+    TMAC_DEV void count_maximum(float d)
+    {
+        const int step = (int)(__float_as_uint(d) >> L::kStepShift) - L::kFirstStep;
+        if (step < L::kSteps) atomicAdd(&sh->maxima[max(step, 0)], 1u);
+    }
+    // One pass over the logits for the largest x, in which the tokens are listed, as x and
+    // index, that are likely to be the first k and some more: those from `least` on, the
+    // least of the threads' (k / 2 + 16) largest maxima over the slice's first quarter,
+    // where k / 4 of them are to be expected.  The caller sees afterwards whether they
+    // are enough.  mx is 0 meanwhile: d is -x.
+    TMAC_DEV float max_and_list(uint32_t k, float* least)
+    {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = vectors() / 4;
+        float own = -INFINITY;
+        vectors(threadIdx.x, part, kThreads, [&](const float (&e)[4], int) {
+            own = fmaxf(own, -fminf(fminf(e[0], e[1]), fminf(e[2], e[3])));
+        });
+        float top = own;
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (lane == 0) sh->red_f[warp] = top;
+        if (threadIdx.x < L::kSteps) sh->maxima[threadIdx.x] = 0;
+        if (threadIdx.x == 0) sh->n_local = 0;
+        __syncthreads();
+        top = lane < kWarps ? sh->red_f[lane] : -INFINITY;
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool finite = fabsf(top) < INFINITY;
+        if (finite) count_maximum(__fsub_rn(top, own));
+        __syncthreads();
+        const float d = bound_of(min(k, k / 2 + 16), [&] { return reinterpret_cast<const Counts*>(sh->maxima)[lane]; });
+        // a little less, so that the distances of the k from the row's largest stay below it
+        const float from = __fsub_rn(__fsub_rn(top, d), __fmul_rn(1e-6f, fmaxf(fabsf(top), d)));
+        *least = finite && d < INFINITY ? from : INFINITY;
+        const float to = -*least;
+        const volatile uint32_t* listed = &sh->n_local;
+        const auto take = [&](const float (&e)[4], int j) {
+            const float first = fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
+            own = fmaxf(own, -first);
+            if (!(first <= to) || *listed > L::kLocal) return;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (e[c] <= to) {
+                    const uint32_t at = atomicAdd(&sh->n_local, 1u);
+                    if (at < L::kLocal) local[at] = order_key(-e[c], begin + j + c);
+                }
+        };
+        vectors(threadIdx.x, part, kThreads, take);
+        vectors(part + threadIdx.x, vectors(), kThreads, take);
+        return own;
+    }
+    // Of the tokens that max_and_list listed, those with d < to, listed as list() does.
+    TMAC_DEV void relist(float to)
+    {
+        constexpr int kPer = (L::kLocal + kThreads - 1) / kThreads;
+        const int n = (int)sh->n_local;
+        unsigned long long key[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int at = threadIdx.x + i * kThreads;
+            key[i] = ~0ull;
+            if (at >= n) continue;
+            const float d = d_of(__uint_as_float((uint32_t)(local[at] >> 32)));
+            if (d < to) key[i] = order_key(d, (int)(uint32_t)local[at]);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) sh->n_local = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+            if (key[i] != ~0ull) local[atomicAdd(&sh->n_local, 1u)] = key[i];
         cl.sync();
     }
 
@@ -877,11 +973,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     m = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
 
     // scaled logits, and the largest of the row
-    float own_max = -INFINITY;
+    float own_max = -INFINITY, least = INFINITY;
     if (kResident) {
         own_max = load_scaled<T>(row.l, row.n, row.inv, row.x, row.pad);
+    } else if (row.mx = 0.0f; k > 1 && !greedy) {
+        own_max = row.max_and_list((uint32_t)k, &least);
+        __syncthreads();  // the maxima's counts have been read
     } else {
-        row.mx = 0.0f;
         row.vectors(threadIdx.x, row.vectors(), kThreads, [&](const float (&e)[4], int) {  // here -x
             own_max = fmaxf(own_max, -fminf(fminf(e[0], e[1]), fminf(e[2], e[3])));
         });
@@ -889,11 +987,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     float mx = own_max;
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (lane == 0) sh->red_f[warp] = mx;
-    if (threadIdx.x < kSteps) sh->maxima[threadIdx.x] = 0;
+    if (threadIdx.x < R::L::kSteps) sh->maxima[threadIdx.x] = 0;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < kWarps; i++) mx = fmaxf(mx, sh->red_f[i]);
         sh->cta_max = mx;
+        sh->least = least < INFINITY && sh->n_local <= R::L::kLocal ? least : INFINITY;
     }
     row.cl.sync();
     mx = lane < row.ranks ? row.cl.map_shared_rank(sh, lane)->cta_max : -INFINITY;
@@ -936,22 +1035,29 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     Cut cut;
     if (k > 0) {
         // the least bound on d below which k threads have their maximum
-        const int step = (int)(__float_as_uint(row.d_of(own_max)) >> 20) - kFirstStep;
-        if (step < kSteps) atomicAdd(&sh->maxima[max(step, 0)], 1u);
+        row.count_maximum(row.d_of(own_max));
         row.cl.sync();
-        uint32_t c0 = 0, c1 = 0;
+        const float bound = R::bound_of((uint32_t)k, [&] {
+            typename R::Counts sum = {};
 #pragma unroll 8
-        for (int r = 0; r < row.ranks; r++) {
-            const uint2 c = reinterpret_cast<const uint2*>(row.cl.map_shared_rank(sh, r)->maxima)[lane];
-            c0 += c.x;
-            c1 += c.y;
-        }
-        const uint32_t up = warp_scan(c0 + c1);
-        const uint32_t hit = __ballot_sync(0xffffffffu, up >= (uint32_t)k);
-        if (hit) {
-            const int at = __ffs(hit) - 1;
-            const int bound = 2 * at + (__shfl_sync(0xffffffffu, up - c1, at) < (uint32_t)k);
-            row.list(0.0f, __uint_as_float((uint32_t)(kFirstStep + bound + 1) << 20), [](float) { return true; });
+            for (int r = 0; r < row.ranks; r++) {
+                const auto c = reinterpret_cast<const typename R::Counts*>(row.cl.map_shared_rank(sh, r)->maxima)[lane];
+#pragma unroll
+                for (int i = 0; i < R::kMine; i++) reinterpret_cast<uint32_t*>(&sum)[i] += reinterpret_cast<const uint32_t*>(&c)[i];
+            }
+            return sum;
+        });
+        if (bound < INFINITY) {
+            // Tokens that a rank has not listed lie at least as far as its `least`.
+            bool all_listed = !kResident;
+            if (!kResident) {
+                const float far = lane < row.ranks ? row.d_of(row.cl.map_shared_rank(sh, lane)->least) : INFINITY;
+                all_listed = __all_sync(0xffffffffu, far >= bound);
+            }
+            if (all_listed)
+                row.relist(bound);
+            else
+                row.list(0.0f, bound, [](float) { return true; });
             uint32_t offset;
             const int n = row.listed(&offset);
             if (n >= 0) {
