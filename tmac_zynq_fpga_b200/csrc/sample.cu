@@ -13,9 +13,9 @@
 // the token is the first kept index whose running weight passes u times the
 // kept weight.
 //
-// A row belongs to one cluster of CTAs.  With few rows eight CTAs hold its x in
+// A row belongs to one cluster of CTAs.  With few rows up to eight CTAs hold its x in
 // shared memory, so the logits are read once.  With many rows (more than the SMs
-// hold that way) fewer CTAs read the logits again for each pass, mostly from L2:
+// hold that way) as few CTAs read the logits again for each pass, mostly from L2:
 // then every row is in flight at once, instead of waiting for others' clusters.
 // Three ways to the cut:
 //  * top-k: the k-th largest of the threads' own maxima bounds the k-th largest
@@ -105,6 +105,12 @@ constexpr size_t list_bytes()  // up to where x starts
     return (kSharedBytes + sizeof(unsigned long long) * (Layout<kResident>::kLocal + Layout<kResident>::kChunks) + 15) / 16 * 16;
 }
 
+template <bool kResident>
+size_t sample_bytes(int slice)
+{
+    return list_bytes<kResident>() + (kResident ? ((size_t)slice + 6) * sizeof(float) : 0);
+}
+
 TMAC_DEV float weight_exp(float d) { return expf(-d); }
 TMAC_DEV unsigned long long weight_of(float e)
 {
@@ -114,12 +120,11 @@ TMAC_DEV unsigned long long weight_of(float e)
 // Tokens of weight 0 lie past the last bin: they are asked for only where it does not matter.
 TMAC_DEV int first_bin(float d) { return __float2int_rz(__fmul_rn(d, kBinScale)); }
 
-// The first part of a row's order that is kept: first_bin(d) < bin, or == bin and
-// (bits(d), index) up to `last`.
 TMAC_DEV unsigned long long order_key(float d, int index)
 {
     return (unsigned long long)__float_as_uint(d) << 32 | (uint32_t)index;
 }
+// The first part of a row's order that is kept, up to the key `last`, which lies in `bin`.
 struct Cut {
     int bin = kBins;
     float from = INFINITY, to = INFINITY;  // bounds on the d of the bin, widened for the product's rounding
@@ -132,14 +137,6 @@ struct Cut {
         to = __fmul_rn(__fdiv_rn((float)(b + 1), kBinScale), 1.000001f);
     }
 };
-TMAC_DEV bool kept_by(const Cut& c, float d, int index)
-{
-    if (d < c.from) return true;
-    if (!(d < c.to)) return false;
-    const int b = first_bin(d);
-    return b < c.bin || (b == c.bin && order_key(d, index) <= c.last);
-}
-
 template <typename V>
 TMAC_DEV V warp_sum(V v)
 {
@@ -331,6 +328,19 @@ struct Row {
         for (; i < to; i += stride) use(load4(i), i);
     }
 
+    // Lists those of a vector's four tokens that `wanted` marks, with these d (or x).
+    TMAC_DEV void put(const float (&v)[4], const bool (&wanted)[4], int index)
+    {
+        const volatile uint32_t* listed = &sh->n_local;
+        const uint32_t count = (uint32_t)wanted[0] + wanted[1] + wanted[2] + wanted[3];
+        if (!count || *listed > L::kLocal) return;
+        uint32_t at = atomicAdd(&sh->n_local, count);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            if (wanted[c] && at < L::kLocal) local[at] = order_key(v[c], index + c);
+            at += wanted[c];
+        }
+    }
     // Lists the tokens with from <= d < to for which `which` holds too, as long as
     // they fit, in any order, and waits for the cluster's lists.
     template <typename F>
@@ -338,18 +348,11 @@ struct Row {
     {
         if (threadIdx.x == 0) sh->n_local = 0;
         __syncthreads();
-        const volatile uint32_t* listed = &sh->n_local;
         vectors(threadIdx.x, vectors(), kThreads, [&](const float (&e)[4], int j) {
-            bool any = false;
+            bool wanted[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++) any |= e[c] < to && e[c] >= from;
-            if (any && *listed <= L::kLocal)
-#pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (e[c] >= from && e[c] < to && which(e[c])) {
-                        const uint32_t at = atomicAdd(&sh->n_local, 1u);
-                        if (at < L::kLocal) local[at] = order_key(e[c], begin + j + c);
-                    }
+            for (int c = 0; c < 4; c++) wanted[c] = e[c] < to && e[c] >= from && which(e[c]);
+            put(e, wanted, begin + j);
         });
         cl.sync();
     }
@@ -406,17 +409,16 @@ struct Row {
         const float from = __fsub_rn(__fsub_rn(top, d), __fmul_rn(1e-6f, fmaxf(fabsf(top), d)));
         *least = finite && d < INFINITY ? from : INFINITY;
         const float to = -*least;
-        const volatile uint32_t* listed = &sh->n_local;
         const auto take = [&](const float (&e)[4], int j) {
-            const float first = fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
-            own = fmaxf(own, -first);
-            if (!(first <= to) || *listed > L::kLocal) return;
+            float v[4];
+            bool wanted[4];
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (e[c] <= to) {
-                    const uint32_t at = atomicAdd(&sh->n_local, 1u);
-                    if (at < L::kLocal) local[at] = order_key(-e[c], begin + j + c);
-                }
+            for (int c = 0; c < 4; c++) {
+                v[c] = -e[c];
+                own = fmaxf(own, v[c]);
+                wanted[c] = e[c] <= to;
+            }
+            put(v, wanted, begin + j);
         };
         vectors(threadIdx.x, part, kThreads, take);
         vectors(part + threadIdx.x, vectors(), kThreads, take);
@@ -549,15 +551,24 @@ struct Row {
         for (int i = threadIdx.x; i < kBins; i += kThreads) sh->cnt[i] = sh->hi[i] = sh->lo[i] = 0;
         __syncthreads();
         vectors(threadIdx.x, vectors(), kThreads, [&](const float (&e)[4], int) {
+            // the four side by side: weights, then additions
+            unsigned long long w[4];
+            uint32_t old[4];
+            int b[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const unsigned long long w = weight_of(weight_exp(e[i]));
-                if (!w) continue;
-                const int b = bin_of(e[i]);
-                if (b < 0) continue;
-                if (kCounts) atomicAdd(&sh->cnt[b], 1u);
-                add_weight(b, w);
+                w[i] = weight_of(weight_exp(e[i]));
+                b[i] = w[i] ? bin_of(e[i]) : -1;
             }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (b[i] < 0) continue;
+                if (kCounts) atomicAdd(&sh->cnt[b[i]], 1u);
+                old[i] = atomicAdd(&sh->lo[b[i]], (uint32_t)w[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (b[i] >= 0) add_carry(b[i], w[i], old[i]);
         });
         cl.sync();
         // this rank's share of the bins, over all ranks: `each` threads to a bin
@@ -791,7 +802,12 @@ struct Row {
     }
     TMAC_DEV void add_weight(int bin, unsigned long long w)
     {
-        const uint32_t low = (uint32_t)w, carry = atomicAdd(&sh->lo[bin], low) > 0xFFFFFFFFu - low;
+        add_carry(bin, w, atomicAdd(&sh->lo[bin], (uint32_t)w));
+    }
+    // The upper word of an addition to a bin whose lower word was `old`.
+    TMAC_DEV void add_carry(int bin, unsigned long long w, uint32_t old)
+    {
+        const uint32_t carry = old > 0xFFFFFFFFu - (uint32_t)w;
         if (carry + (w >> 32)) atomicAdd(&sh->hi[bin], carry + (uint32_t)(w >> 32));
     }
     TMAC_DEV void sort_and_cut(int n, uint32_t k, double t, unsigned long long base)
@@ -1084,7 +1100,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
     };
     // no kept token lies as far: a bound on exp(-d) >= m, a little wide, and on the cut
     const float farthest = fminf(cut.to, m > 0.0f ? __fadd_rn(__fmul_rn(-logf(m), 1.0001f), 1e-4f) : INFINITY);
-    if (cut.bin == kBins && m == 0.0f)
+    const bool skip = !kResident || m > 0.0f;
+    if (cut.last == ~0ull && m == 0.0f)
         row.draw(
             [](const float (&d)[4], int, unsigned long long (&w)[4]) {
 #pragma unroll
@@ -1096,13 +1113,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
             [&](const float (&d)[4], int index, unsigned long long (&w)[4]) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) w[i] = 0;
-                if (!(fminf(fminf(d[0], d[1]), fminf(d[2], d[3])) < farthest)) return;
+                // Read anew, or by min-p, most vectors have no token near enough; others are
+                // worked on side by side (top-p of 32 held rows 39 us, 43 with the test).
+                if (skip && !(fminf(fminf(d[0], d[1]), fminf(d[2], d[3])) < farthest)) return;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    if (!(d[i] < farthest)) continue;
-                    if (d[i] >= cut.from && !kept_by(cut, d[i], index + i)) continue;
                     const float e = weight_exp(d[i]);
-                    if (e >= m) w[i] = weight_of(e);
+                    w[i] = order_key(d[i], index + i) <= cut.last && e >= m ? weight_of(e) : 0;
                 }
             },
             pick, found);
@@ -1111,7 +1128,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
 template <typename T, bool kResident>
 int launch_sample(const SampleArgs& a, int batch, int ranks, int device, cudaStream_t s)
 {
-    const size_t smem = list_bytes<kResident>() + (kResident ? ((size_t)a.slice + 6) * sizeof(float) : 0);
+    const size_t smem = sample_bytes<kResident>(a.slice);
     auto fn = sample_kernel<T, kResident>;
     static std::atomic<uint64_t> done{0};
     const int rc = set_once(done, device, [&] {
@@ -1164,12 +1181,13 @@ extern "C" int tmac_sample(const void* logits, int type, int64_t row_stride, int
     a.probs = probs;
     // Up to two CTAs per SM hold their rows; more rows than that are read anew for
     // each pass by as few CTAs as fill the SMs twice.  Top-k 40 of 151936 logits, held
-    // against read anew: 21.7 / 25.0 us for 32 rows, 36.2 / 23.5 for 64, 126 / 62 for 256.
-    const int room = 2 * num_sms(device);
-    int ranks = vocab <= 4096 ? 1 : vocab <= kCluster * kMaxSlice ? kCluster : kMaxCluster;
-    const bool resident = (int64_t)batch * ranks <= room;
-    while (!resident && ranks > 1 && (int64_t)batch * ranks > room) ranks /= 2;
+    // against read anew: 15.4 / 25.0 us for 32 rows, 36.2 / 18.0 for 64, 126 / 40 for 256.
+    // So are more rows of fewer logits: what half an SM's shared memory holds.
+    const int room = 2 * num_sms(device), most = vocab <= 4096 ? 1 : vocab <= kCluster * kMaxSlice ? kCluster : kMaxCluster;
+    int ranks = most;
+    while (ranks > 1 && (int64_t)batch * ranks > room) ranks /= 2;
     a.slice = ((vocab + ranks - 1) / ranks + 7) & ~7;  // every rank's first logit is as aligned as the row's
+    const bool resident = (int64_t)batch * ranks <= room && (ranks == most || sample_bytes<true>(a.slice) <= 113 * 1024);
     DeviceGuard dg(device);
     if (!dg.ok) return fail(TMAC_ERR_NODEV, "no such CUDA device");
     return with_type(type, [&](auto* t) {
