@@ -24,6 +24,11 @@
 // (Products on the FMA units too took 2 to 3 times as long.)  Tiles come through
 // cp.async, several in flight.  The prefix's jobs of 16-bit elements go to the tcgen05
 // kernel of prefix_attention_tc.cu where there are rows enough.
+//
+// Bound: latency.  48 sequences over 2051 + up to 509 keys (14/2 heads of 64, f16) take
+// 12.8 us, 10 of them jobs of 3 to 4 tiles, 3 the join; in 32 bits 25 us.  64
+// sequences with only their own keys, up to 1024, run at 1300 GB/s, of heads of 128
+// at 2200.
 #include "prefix_attention.cuh"
 
 namespace tmac {
@@ -262,7 +267,7 @@ again:
         const auto keys = [&](auto n8, int step) {
             constexpr int kN8 = decltype(n8)::value;
             float s[kN8][4] = {};
-            constexpr int kChain = 4;  // 32-bit products in a row on the tensor cores
+            [[maybe_unused]] constexpr int kChain = 4;  // 32-bit products in a row on the tensor cores
             [[maybe_unused]] float main[k32 ? kN8 : 1][4] = {}, rest[k32 ? kN8 : 1][4] = {};
 #pragma unroll
             for (int i = 0; i < D / kDepth; i++) {
@@ -473,6 +478,7 @@ __global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
 // ------------------------------------------------------------------- join ----
 // Joins the parts of one (token, head) per CTA: groups of D / 4 threads take every
 // kGroups-th part, four values a thread, several loads in flight.
+// Bound: latency and L2, 6 us for 1792 rows of 64 dims in 27 parts (12 MB).
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) attn_join_kernel(AttnArgs a)
 {

@@ -17,8 +17,11 @@
 // weights anew.  One thread issues the products, one warp the TMA copies of the pages
 // (a box per page, 128-byte swizzle).
 //
-// Bound: the exponentials, 128 x 64 per tile at 16 a clock, 512 clocks against 128
-// of products at 64 dims.  Two CTAs share an SM: one's waits are the other's work.
+// Bound: the exponentials, 128 x 64 per tile at 16 a clock, 512 clocks against 256
+// of products at 64 dims.  Two CTAs share an SM: one's waits are the other's work.  896 rows
+// a key/value head (two of 64 dims) over 32768 keys take 37 us, 410 TFLOP/s, 913 clocks a
+// tile: the rest is the latency of its 300 instructions a warp.  Three or four CTAs an
+// SM, with the weights in the scores' place, take as long.
 #include "prefix_attention.cuh"
 #include "tcgen05.cuh"
 
