@@ -10,13 +10,14 @@
 // cache's type.
 //
 // Bound: HBM, every value is read once and written once (32768 tokens of 16/4 heads of
-// 128, bf16, 98 us, 4240 GB/s; 512 tokens 3.8 us, 2 tokens 3.0, the launch).  Where the pointers,
-// strides and head parts allow it a thread takes 8 adjoining values (16 bytes of a
-// 16-bit type), or 8 pairs of halves (several of either at once run no faster: the
-// registers cost more warps than they gain); a CTA
-// takes a few tokens, whose pages, cosines and sines it first looks up into shared
-// memory, so nothing but the values is waited for.  Other layouts take one pair per
-// thread.
+// 128, bf16, 91 us, 4560 GB/s; 512 tokens 3.5 us, 2 tokens 3.4, the launch).  Where
+// the pointers, strides and head parts allow it a thread takes 8 adjoining values (16
+// bytes of a 16-bit type), or 8 pairs of halves, and keeps that place in a token for all
+// tokens of its CTA, the next one's values loaded beneath the work on this one's: 16-bit
+// values 98 -> 91 us and 21.3 -> 19.3 against places dealt out anew, 32-bit ones 34 ->
+// 36.6, 49 -> 50 and, of 512 tokens, 3.9 -> 3.5.  A CTA first looks up its tokens' pages,
+// cosines and sines into shared memory, so nothing but the values is waited for.  Other
+// layouts take one pair per thread.
 #include "serving.cuh"
 
 #include <algorithm>
@@ -178,112 +179,125 @@ struct Divide {
 // Units of a q or k head: 8 values at a time (interleaved), or 8 pairs at a time of
 // the rotated part and 8 values at a time of the rest; of a v head: 8 values at a time.
 constexpr int kMaxTokens = 16;  // of a CTA
+template <typename T>
+constexpr int kMaxThreads = sizeof(T) == 2 ? 512 : 384;  // 32-bit values take more registers
 struct Deal {
-    int tokens;              // of a CTA
-    int turned;              // units of a token's q and k heads
-    Divide per_token, per_head, per_v;
+    int tokens;     // of a CTA
+    int units;      // of a token
+    int turned;     // of these, of q and k heads
+    Divide per_head, per_v;
 };
 template <typename T, typename C, bool kInterleaved>
-__global__ void __launch_bounds__(256) rope_append_vec_kernel(RopeArgs a, Deal deal)
+__global__ void __launch_bounds__(kMaxThreads<T>, sizeof(T) == 2 ? 2 : 1) rope_append_vec_kernel(RopeArgs a, Deal deal)
 {
     extern __shared__ __align__(16) float turns[];  // [tokens][2][rot / 2]: cosines, sines
     __shared__ Place places[kMaxTokens];
     const int d = a.cache.dim, hk = a.cache.kv_heads, shift = a.cache.page_shift, half = a.rot / 2;
-    const int pairs8 = kInterleaved ? 0 : a.rot / 16, per_token = (int)deal.per_token.by;
+    const int pairs8 = kInterleaved ? 0 : a.rot / 16;
     const int64_t t0 = (int64_t)blockIdx.x * deal.tokens;
-    const int n = (int)min((int64_t)deal.tokens, a.tokens - t0), units = n * per_token;
-    struct Unit {
-        int token, row, d0;  // row: of q, k and v together
-        bool is_v, halves;
-    };
-    const auto unit_of = [&](int u) {
-        Unit o;
-        o.token = deal.per_token(u);
-        u -= o.token * per_token;
-        o.is_v = u >= deal.turned;
-        if (o.is_v) {
+    const int n = (int)min((int64_t)deal.tokens, a.tokens - t0);
+    // a thread keeps its unit for all tokens of the CTA
+    bool is_v, halves;
+    int row, d0;  // row: of q, k and v together
+    const T* src;
+    int64_t stride;
+    const auto take = [&](int u) {
+        is_v = u >= deal.turned;
+        if (is_v) {
             u -= deal.turned;
             const int head = deal.per_v(u);
-            o.row = a.heads + hk + head;
-            o.d0 = (u - head * (int)deal.per_v.by) * 8;
-            o.halves = false;
+            row = a.heads + hk + head;
+            d0 = (u - head * (int)deal.per_v.by) * 8;
+            halves = false;
+            src = (const T*)a.v + head * d;
+            stride = a.v_stride;
         } else {
-            o.row = deal.per_head(u);
-            const int unit = u - o.row * (int)deal.per_head.by;
-            o.halves = unit < pairs8;
-            o.d0 = o.halves || kInterleaved ? unit * 8 : a.rot + (unit - pairs8) * 8;
+            row = deal.per_head(u);
+            const int unit = u - row * (int)deal.per_head.by;
+            halves = unit < pairs8;
+            d0 = halves || kInterleaved ? unit * 8 : a.rot + (unit - pairs8) * 8;
+            const bool is_k = row >= a.heads;
+            src = is_k ? (const T*)a.k + (row - a.heads) * d : (const T*)a.q + row * d;
+            stride = is_k ? a.k_stride : a.q_stride;
         }
-        return o;
+        src += t0 * stride + d0;
     };
     Eight<T> xr, zr;
-    const auto load = [&](const Unit& u) {
-        const int64_t t = t0 + u.token;
-        const T* src = u.is_v              ? (const T*)a.v + t * a.v_stride + (u.row - a.heads - hk) * d
-                       : u.row < a.heads ? (const T*)a.q + t * a.q_stride + u.row * d
-                                           : (const T*)a.k + t * a.k_stride + (u.row - a.heads) * d;
-        xr.load(src + u.d0);
-        if (u.halves) zr.load(src + u.d0 + half);
+    const auto load = [&] {
+        xr.load(src);
+        if (halves) zr.load(src + half);
+        src += stride;
     };
-    Unit u = unit_of(threadIdx.x);
-    if ((int)threadIdx.x < units) load(u);
+    int u = threadIdx.x;
+    if (u < deal.units) {
+        take(u);
+        load();
+    }
     if ((int)threadIdx.x < n) places[threadIdx.x] = place_of(a, t0 + threadIdx.x);
     __syncthreads();
-    for (int i = threadIdx.x; i < n * (a.rot / 4); i += 256) {
+    for (int i = threadIdx.x; i < n * (a.rot / 4); i += blockDim.x) {
         const int token = i / (a.rot / 4), at = i % (a.rot / 4) * 4;  // of cosines, then of sines
         if (!places[token].ok) continue;
         const float* from = (at < half ? a.cos + at : a.sin + at - half) + (int64_t)places[token].pos * half;
         *reinterpret_cast<float4*>(turns + token * a.rot + at) = __ldg(reinterpret_cast<const float4*>(from));
     }
     __syncthreads();
-    for (int at = threadIdx.x; at < units; at += 256) {
-        if (at >= 256) {
-            u = unit_of(at);
-            load(u);
-        }
-        const Place& p = places[u.token];
-        C* dst;
-        if (u.row < a.heads)
-            dst = (C*)a.q_out + ((t0 + u.token) * a.heads + u.row) * d;
-        else if (p.page >= 0)
-            dst = (C*)(u.is_v ? a.cache.v : a.cache.k) +
-                  (((p.page * hk + u.row - a.heads - (u.is_v ? hk : 0)) << shift) + p.slot) * d;
-        else
-            continue;
-        float x[8], z[8];
-        xr.floats(x);
-        if (u.halves) zr.floats(z);
-        if (a.bias) {
-            add8(x, a.bias + u.row * d + u.d0);
-            if (u.halves) add8(z, a.bias + u.row * d + u.d0 + half);
-        }
-        const float *c = turns + u.token * a.rot, *s = c + half;
-        if (!p.ok) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = z[i] = 0.0f;
-        } else if (kInterleaved && !u.is_v && u.d0 < a.rot) {
-            const float4 c4 = *reinterpret_cast<const float4*>(c + u.d0 / 2), s4 = *reinterpret_cast<const float4*>(s + u.d0 / 2);
-            const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float y = __fmaf_rn(x[2 * i], cv[i], -__fmul_rn(x[2 * i + 1], sv[i]));
-                x[2 * i + 1] = __fmaf_rn(x[2 * i], sv[i], __fmul_rn(x[2 * i + 1], cv[i]));
-                x[2 * i] = y;
+    while (u < deal.units) {
+        const bool is_q = row < a.heads;
+        // q's row of the first token; of k and v the place in a page
+        C* const to = is_q ? (C*)a.q_out + (t0 * a.heads + row) * d + d0
+                           : (C*)(is_v ? a.cache.v : a.cache.k) + ((int64_t)(row - a.heads - (is_v ? hk : 0)) << shift) * d + d0;
+        for (int token = 0; token < n; token++) {
+            float x[8], z[8];
+            xr.floats(x);
+            if (halves) zr.floats(z);
+            if (token + 1 < n) load();  // beneath this token's arithmetic
+            const Place& p = places[token];
+            C* dst = to;
+            if (is_q)
+                dst += (int64_t)token * (a.heads * d);
+            else if (p.page >= 0)
+                dst += (((p.page * hk) << shift) + p.slot) * d;
+            else
+                continue;
+            if (a.bias) {
+                add8(x, a.bias + row * d + d0);
+                if (halves) add8(z, a.bias + row * d + d0 + half);
             }
-        } else if (u.halves) {
+            const float *c = turns + token * a.rot, *s = c + half;
+            if (!p.ok) {
 #pragma unroll
-            for (int h = 0; h < 8; h += 4) {
-                const float4 c4 = *reinterpret_cast<const float4*>(c + u.d0 + h), s4 = *reinterpret_cast<const float4*>(s + u.d0 + h);
+                for (int i = 0; i < 8; i++) x[i] = z[i] = 0.0f;
+            } else if (kInterleaved && !is_v && d0 < a.rot) {
+                const float4 c4 = *reinterpret_cast<const float4*>(c + d0 / 2), s4 = *reinterpret_cast<const float4*>(s + d0 / 2);
                 const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float y = __fmaf_rn(x[h + i], cv[i], -__fmul_rn(z[h + i], sv[i]));
-                    z[h + i] = __fmaf_rn(x[h + i], sv[i], __fmul_rn(z[h + i], cv[i]));
-                    x[h + i] = y;
+                    const float y = __fmaf_rn(x[2 * i], cv[i], -__fmul_rn(x[2 * i + 1], sv[i]));
+                    x[2 * i + 1] = __fmaf_rn(x[2 * i], sv[i], __fmul_rn(x[2 * i + 1], cv[i]));
+                    x[2 * i] = y;
+                }
+            } else if (halves) {
+#pragma unroll
+                for (int h = 0; h < 8; h += 4) {
+                    const float4 c4 = *reinterpret_cast<const float4*>(c + d0 + h), s4 = *reinterpret_cast<const float4*>(s + d0 + h);
+                    const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float y = __fmaf_rn(x[h + i], cv[i], -__fmul_rn(z[h + i], sv[i]));
+                        z[h + i] = __fmaf_rn(x[h + i], sv[i], __fmul_rn(z[h + i], cv[i]));
+                        x[h + i] = y;
+                    }
                 }
             }
+            store8(dst, x);
+            if (halves) store8(dst + half, z);
         }
-        store8(dst + u.d0, x);
-        if (u.halves) store8(dst + u.d0 + half, z);
+        u += blockDim.x;
+        if (u < deal.units) {
+            take(u);
+            load();
+        }
     }
 }
 
@@ -307,12 +321,14 @@ int launch_rope(const RopeArgs& a, bool interleaved, int sms, cudaStream_t s)
         Deal d;
         // tokens of a CTA: as long as there are four CTAs to an SM
         d.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxTokens, a.tokens / (4 * sms)));
+        d.units = (int)per_token;
         d.turned = (a.heads + hk) * per_head;
-        d.per_token = Divide::of((int)per_token);
         d.per_head = Divide::of(per_head);
         d.per_v = Divide::of(a.cache.dim / 8);
+        // threads: a token's units, or an even part of them
+        const int parts = (d.units + kMaxThreads<T> - 1) / kMaxThreads<T>, threads = ((d.units + parts - 1) / parts + 31) / 32 * 32;
         auto fn = interleaved ? rope_append_vec_kernel<T, C, true> : rope_append_vec_kernel<T, C, false>;
-        fn<<<(unsigned)((a.tokens + d.tokens - 1) / d.tokens), 256, (size_t)d.tokens * a.rot * sizeof(float), s>>>(a, d);
+        fn<<<(unsigned)((a.tokens + d.tokens - 1) / d.tokens), threads, (size_t)d.tokens * a.rot * sizeof(float), s>>>(a, d);
     } else {
         const int64_t pairs = a.tokens * (a.heads + 2 * hk) * (a.cache.dim / 2);
         auto fn = interleaved ? rope_append_kernel<T, C, true> : rope_append_kernel<T, C, false>;
