@@ -129,6 +129,17 @@ def test_append_lengths(tokens):
     check_append(append_case(BF16, BF16, 14, 2, 64, 64, 32, tokens, n_seq=min(tokens, 7)))
 
 
+# more places in a token than a CTA has threads, and few; several tokens a CTA, ragged at the end
+@pytest.mark.parametrize("heads,kv_heads,dim", [(48, 8, 128), (70, 2, 128), (1, 1, 16), (2, 1, 64)])
+@pytest.mark.parametrize("tokens", [1, 1999, 9500])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_append_many_and_few_heads(heads, kv_heads, dim, tokens, interleaved, dtype):
+    if heads * tokens > 200000:
+        tokens = 3001
+    check_append(append_case(dtype, F16, heads, kv_heads, dim, dim if dim == 16 else dim // 2, 32, tokens, interleaved, n_seq=min(tokens, 5)))
+
+
 def test_append_padding_and_bounds():
     c = append_case(F32, F32, 2, 1, 64, 64, 8, 6, n_seq=6)
     kc, vc = (p.clone() for p in c["pools"])
