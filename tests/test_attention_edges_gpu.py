@@ -1,0 +1,82 @@
+"""prefix_attention where numbers, lengths or layouts are out of the ordinary, against 64 bits.
+Tolerances as derived in test_serving_gpu.py; every sequence here sees one list of keys."""
+import math
+
+import pytest
+
+import tmac_zynq_fpga_b200 as tm
+from test_serving_gpu import BF16, F16, F32, INF, NAN, TINY, U, no_error
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+# (sequences, keys): each sequence reads the prefix itself; shared and joined; on tcgen05 (16 bits)
+LAYOUTS = [(2, 200), (9, 1100), (40, 1100), (100, 5000)]
+HEADS = {64: (14, 2), 128: (8, 2)}
+
+
+def random_rows(dim, batch, n, dtype, seed=0):
+    """q [batch, heads, dim], k and v [n, kv_heads, dim]"""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    h, hk = HEADS[dim]
+    return [(torch.randn(s, generator=g, device="cuda") * f).to(dtype) for s, f in (((batch, h, dim), 2.0), ((n, hk, dim), 1.0), ((n, hk, dim), 1.0))]
+
+
+def paged(rows, page, seed=1):
+    """Pools that hold rows [n, kv_heads, dim] in pages at random places, and the pages' numbers."""
+    n, hk, dim = rows[0].shape
+    count = -(-n // page)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pages = torch.randperm(count + 2, generator=g, device="cuda")[:count].int()
+    at = torch.arange(n, device="cuda")
+    pools = []
+    for r in rows:
+        pool = torch.full((count + 2, hk, page, dim), NAN, device="cuda", dtype=r.dtype)
+        pool[pages.long()[at // page], :, at % page] = r
+        pools.append(pool)
+    return pools, pages
+
+
+def attend(q, k, v, page=16, **kw):
+    """Every row over all keys."""
+    (kp, vp), pages = paged([k, v], page)
+    none = torch.zeros((len(q), 1), dtype=torch.int32, device="cuda")
+    out = tm.prefix_attention(q, tm.PagedCache(kp, vp), none, none[:, 0].contiguous(), prefix_pages=pages, prefix_len=len(k), max_own=0, **kw)
+    no_error()
+    return out
+
+
+def formula(q, k, v, scale=None):
+    """The result in 64 bits and its tolerance; a key whose score is -inf weighs nothing."""
+    h, dim = q.shape[1:]
+    scale = dim ** -0.5 if scale is None else scale
+    kd, vd = (x.double().repeat_interleave(h // k.shape[1], 1) for x in (k, v))
+    want, tol = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    for t in range(len(q)):
+        terms = q[t].double() * kd * scale
+        score = terms.sum(2)
+        p = torch.softmax(score, 0)
+        want[t] = torch.einsum("kh,khd->hd", p, vd)
+        size = torch.einsum("kh,khd->hd", p, vd.abs())
+        most = torch.where(score == -INF, 0.0, terms.abs().sum(2)).amax(0)[:, None]
+        off = 2 * (dim + 4) * 2.0 ** -24 * most + (len(k) + 16) * 2.0 ** -24
+        tol[t] = U[q.dtype] * want[t].abs() + (off + (U[q.dtype] if q.dtype != F32 else 0)) * size + TINY[q.dtype]
+    return want, tol
+
+
+def check(out, want, tol):
+    off = (out.double() - want).abs() - tol
+    assert torch.isfinite(want).all() and (off <= 0).all(), f"worst {off.max().item():.3g} past the tolerance"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("batch,n", LAYOUTS)
+def test_large_values_whose_weights_grow_along_the_keys(dtype, batch, n):
+    """The first 64 keys weigh 2^-24 of the others each; sums of weight times value pass 32 bits' range
+    unless weights stay near 1."""
+    q, k, v = random_rows(64, batch, n, dtype)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 8.0
+    k[64:, :, 0] = 24 * math.log(2)  # times 8 / sqrt(64)
+    v = (v.float() * 2.0 ** 110).to(dtype)
+    check(attend(q, k, v), *formula(q, k, v))

@@ -123,6 +123,7 @@ struct MmaSmem {
         T k[kTile * MmaConf<T, D>::kKeyRow], v[kTile * MmaConf<T, D>::kValueRow];
     } stage[MmaConf<T, D>::kStages];
     float ml[kWarps][kMmaRows][2];
+    uint32_t bad[kWarps][2];
 };
 TMAC_DEV void ldmatrix4(uint32_t (&r)[4], const void* p)
 {
@@ -245,8 +246,6 @@ TMAC_DEV void attn_mma(const AttnArgs& a)
     const int o_least = __reduce_min_sync(0xffffffffu, min(o_limit[0], o_limit[1]));
     const float scale = k32 ? a.scale : __fmul_rn(a.scale, 1.44269504f);  // log2 e: powers of 2
     float m[2], l[2], o[kN][4];
-    bool careful = false;
-again:
 #pragma unroll
     for (int h = 0; h < 2; h++) m[h] = -INFINITY, l[h] = 0.0f;
 #pragma unroll
@@ -335,55 +334,36 @@ again:
                 for (int n = 0; n < kN; n++)
 #pragma unroll
                     for (int c = 0; c < 4; c++) o[n][c] = __fmul_rn(o[n][c], al[c >> 1]);
-            if (!careful) {
-                if constexpr (k32) {
-                    // depth t and t + 4: keys 2 t and 2 t + 1, as the scores lie
-                    uint32_t hi[kN8][4], lo[kN8][4];
-#pragma unroll
-                    for (int k = 0; k < kN8; k++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) split_tf32(s[k][c >> 1 | (c & 1) << 1], hi[k][c], lo[k][c]);
-#pragma unroll
-                    for (int n = 0; n < kN; n++) {
-                        float sum[4] = {}, small[4] = {};
-#pragma unroll
-                        for (int k = 0; k < kN8; k++)
-                            mma_f32(sum, small, hi[k], lo[k], st.v[Conf::value_at(step + 8 * k + c2, 8 * n + g)],
-                                    st.v[Conf::value_at(step + 8 * k + c2 + 1, 8 * n + g)]);
-#pragma unroll
-                        for (int c = 0; c < 4; c++) o[n][c] = __fadd_rn(o[n][c], __fadd_rn(sum[c], small[c]));
-                    }
-                } else {
-#pragma unroll
-                    for (int k = 0; k < kN8; k += 2) {
-                        const uint32_t p[4] = {pack2<T>(s[k][0], s[k][1]), pack2<T>(s[k][2], s[k][3]), pack2<T>(s[k + 1][0], s[k + 1][1]),
-                                               pack2<T>(s[k + 1][2], s[k + 1][3])};
-#pragma unroll
-                        for (int n = 0; n < kN; n += 2) {
-                            uint32_t vx[4];  // keys 0-7 and 8-15 of dims 8n.., then of the next eight
-                            ldmatrix4_trans(vx, &st.v[Conf::value_at(step + 8 * k + (lane & 15), 8 * n + (lane >> 4) * 8)]);
-                            mma16816<T>(o[n], p, vx[0], vx[1]);
-                            mma16816<T>(o[n + 1], p, vx[2], vx[3]);
-                        }
-                    }
-                }
-            } else {
+            if constexpr (k32) {
+                // depth t and t + 4: keys 2 t and 2 t + 1, as the scores lie
+                uint32_t hi[kN8][4], lo[kN8][4];
 #pragma unroll
                 for (int k = 0; k < kN8; k++)
 #pragma unroll
-                    for (int c8 = 0; c8 < 2; c8++)
-#pragma unroll 1
-                        for (int u = 0; u < 4; u++) {  // key 8 k + 2 u + c8, whose weights lane u of each row holds
-                            const float p0 = __shfl_sync(0xffffffffu, s[k][c8], g * 4 + u), p1 = __shfl_sync(0xffffffffu, s[k][2 + c8], g * 4 + u);
+                    for (int c = 0; c < 4; c++) split_tf32(s[k][c >> 1 | (c & 1) << 1], hi[k][c], lo[k][c]);
 #pragma unroll
-                            for (int n = 0; n < kN; n++)
+                for (int n = 0; n < kN; n++) {
+                    float sum[4] = {}, small[4] = {};
 #pragma unroll
-                                for (int c = 0; c < 2; c++) {
-                                    const float v = Elem<T>::load(&st.v[Conf::value_at(step + 8 * k + 2 * u + c8, 8 * n + c2 + c)]);
-                                    if (p0 != 0.0f) o[n][c] = __fmaf_rn(p0, v, o[n][c]);
-                                    if (p1 != 0.0f) o[n][2 + c] = __fmaf_rn(p1, v, o[n][2 + c]);
-                                }
-                        }
+                    for (int k = 0; k < kN8; k++)
+                        mma_f32(sum, small, hi[k], lo[k], st.v[Conf::value_at(step + 8 * k + c2, 8 * n + g)],
+                                st.v[Conf::value_at(step + 8 * k + c2 + 1, 8 * n + g)]);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) o[n][c] = __fadd_rn(o[n][c], __fadd_rn(sum[c], small[c]));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < kN8; k += 2) {
+                    const uint32_t p[4] = {pack2<T>(s[k][0], s[k][1]), pack2<T>(s[k][2], s[k][3]), pack2<T>(s[k + 1][0], s[k + 1][1]),
+                                           pack2<T>(s[k + 1][2], s[k + 1][3])};
+#pragma unroll
+                    for (int n = 0; n < kN; n += 2) {
+                        uint32_t vx[4];  // keys 0-7 and 8-15 of dims 8n.., then of the next eight
+                        ldmatrix4_trans(vx, &st.v[Conf::value_at(step + 8 * k + (lane & 15), 8 * n + (lane >> 4) * 8)]);
+                        mma16816<T>(o[n], p, vx[0], vx[1]);
+                        mma16816<T>(o[n + 1], p, vx[2], vx[3]);
+                    }
+                }
             }
         };
         if (split_keys) {
@@ -394,22 +374,19 @@ again:
         }
     }
     cp_async_wait<0>();
-    // The product adds 0 * v for a key that a row does not see, which an infinite or NaN
-    // v turns into NaN.  Where any sum is not finite the job runs again key by key,
-    // each row with those it sees.
-    if (!careful) {
+    // Rows with a sum that is not finite are computed again (row_by_keys): bit 4 (r & 7) of
+    // bad[r >> 3] for row r of the warp's.
+    uint32_t bad[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
         bool finite = true;
 #pragma unroll
-        for (int n = 0; n < kN; n++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) finite &= fabsf(o[n][c]) < INFINITY;
-        if (__syncthreads_or(!finite)) {
-            careful = true;
-            for (int i = 0; i < kStages - 1; i++) copy(j.tile0 + i, Copy::look_up(a, j, j.tile0 + i));
-            page[0] = Copy::look_up(a, j, j.tile0 + kStages - 1);
-            goto again;
-        }
+        for (int n = 0; n < kN; n++) finite &= fabsf(o[n][2 * h]) < INFINITY && fabsf(o[n][2 * h + 1]) < INFINITY;
+        bad[h] = __ballot_sync(0xffffffffu, !finite);
+        bad[h] |= bad[h] >> 1;
+        bad[h] = (bad[h] | bad[h] >> 2) & 0x11111111u;
     }
+    const auto is_bad = [](const uint32_t (&b)[2], int r) { return (b[r >> 3 & 1] >> (4 * (r & 7)) & 1) != 0; };
 #pragma unroll
     for (int h = 0; h < 2; h++) {
         l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 1));
@@ -419,7 +396,7 @@ again:
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int r = r0 + g + 8 * h;
-            if (r >= j.rows) continue;
+            if (r >= j.rows || is_bad(bad, g + 8 * h)) continue;
             const RowOf row = find_row(a, j, r);
 #pragma unroll
             for (int n = 0; n < kN; n++) {
@@ -427,6 +404,9 @@ again:
                 put_results<T, D, 2>(a, j, row, 8 * n + c2, m[h], l[h], two);
             }
         }
+        if (bad[0] | bad[1])
+            for (int r = 0; r < kMmaRows && r0 + r < j.rows; r++)
+                if (is_bad(bad, r)) row_by_keys<T, D>(a, j, r0 + r);
         return;
     }
     // the warps' results, joined
@@ -443,10 +423,21 @@ again:
 #pragma unroll
         for (int n = 0; n < kN; n++)
             *reinterpret_cast<float2*>(&ow[(warp * kMmaRows + r) * D + 8 * n + c2]) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+        if (lane == 0) sh.bad[warp][h] = bad[h];
     }
     __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        bad[h] = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) bad[h] |= sh.bad[w][h];
+    }
+    if (bad[0] | bad[1])
+        for (int r = warp; r < j.rows; r += kWarps)
+            if (is_bad(bad, r)) row_by_keys<T, D>(a, j, r);
     for (int i = threadIdx.x; i < j.rows * (D / 4); i += kThreads) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
+        if (is_bad(bad, r)) continue;
         float mx = -INFINITY, sum = 0.0f, val[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, sh.ml[w][r][0]);
@@ -466,8 +457,11 @@ again:
     }
 }
 
+// Jobs of an SM, by shared memory: the registers allow as many.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) attn_mma_kernel(AttnArgs a)
+constexpr int kJobsOfSm = 227 * 1024 / (sizeof(MmaSmem<T, D>) + 1024);
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, kJobsOfSm<T, D>) attn_mma_kernel(const __grid_constant__ AttnArgs a)
 {
     attn_mma<T, D>(a);
     // Where the tcgen05 kernel runs beside this one, this grid ends after it, so the
@@ -551,12 +545,10 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(AttnArgs a)
     }
 }
 
-// Jobs of the mma kernel that an SM holds, by its shared memory.
 int jobs_of_sm(int type, int dim)
 {
-    const size_t bytes = type == TMAC_TYPE_F32 ? dim == 64 ? sizeof(MmaSmem<float, 64>) : sizeof(MmaSmem<float, 128>)
-                                               : dim == 64 ? sizeof(MmaSmem<__half, 64>) : sizeof(MmaSmem<__half, 128>);
-    return (int)(227 * 1024 / (bytes + 1024));
+    if (type == TMAC_TYPE_F32) return dim == 64 ? kJobsOfSm<float, 64> : kJobsOfSm<float, 128>;
+    return dim == 64 ? kJobsOfSm<__half, 64> : kJobsOfSm<__half, 128>;
 }
 // How the work is cut: key ranges so that the jobs of a kernel are about as many as
 // the GPU holds at once, own parts counted as three quarters of their bound (they are

@@ -219,6 +219,54 @@ TMAC_DEV float power(float x)
     return sizeof(T) == 4 ? expf(x) : exp2_fast(x);
 }
 
+// Row r of a job by one warp, key by key on the FMA units and only over the keys that it
+// sees: for rows whose products met something that is not finite.  The matrix products
+// add 0 * v for a key that a row does not see, which an infinite or NaN v turns into
+// NaN; a large 32-bit number has no split; and weights above 1 overflow with large v
+// before the division by their sum.
+template <typename T, int D>
+__device__ __noinline__ void row_by_keys(const AttnArgs& a, Job j, int r)
+{
+    constexpr int kPer = D / 32;  // adjoining dims of a lane
+    const int d = (threadIdx.x & 31) * kPer, shift = a.cache.page_shift;
+    const RowOf row = find_row(a, j, r);
+    const float scale = sizeof(T) == 4 ? a.scale : __fmul_rn(a.scale, 1.44269504f);  // as power's base
+    float q[kPer], o[kPer], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+        q[i] = Elem<T>::load((const T*)a.q + row.token * a.q_stride + row.head * D + d + i);
+        o[i] = 0.0f;
+    }
+    for (int t = j.tile0; t < j.tile1; t++) {
+        const TileOf tile = find_tile(a, j, t);
+        const int end = min(min(tile.prefix ? row.p_limit : row.o_limit, tile.keys), tile.key0 + kTile);
+        for (int key = tile.key0; key < end; key++) {
+            const int64_t page = __ldg(tile.pages + (key >> shift));
+            const bool known = page >= 0 && page < a.cache.n_pages;  // else zeros; recorded before
+            const int64_t at = known ? (((page * a.cache.kv_heads + j.kvh) << shift) + (key & ((1 << shift) - 1))) * D + d : 0;
+            float s = 0.0f, v[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                s = __fmaf_rn(q[i], known ? Elem<T>::load((const T*)a.cache.k + at + i) : 0.0f, s);
+                v[i] = known ? Elem<T>::load((const T*)a.cache.v + at + i) : 0.0f;
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, w));
+            s = __fmul_rn(s, scale);
+            const float mx = fmaxf(m, s), al = m == mx ? 1.0f : power<T>(__fsub_rn(m, mx));
+            const float p = s == -INFINITY ? 0.0f : power<T>(__fsub_rn(s, mx));
+            l = __fmaf_rn(l, al, p);
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                o[i] = __fmul_rn(o[i], al);
+                if (p != 0.0f) o[i] = __fmaf_rn(p, v[i], o[i]);
+            }
+            m = mx;
+        }
+    }
+    put_results<T, D, kPer>(a, j, row, d, m, l, o);
+}
+
 // prefix_attention_tc.cu: the prefix's jobs of 16-bit elements on tcgen05.
 constexpr int kTcRows = 128;  // rows of a job
 int launch_prefix_tc(const AttnArgs& a, int type, cudaStream_t s);

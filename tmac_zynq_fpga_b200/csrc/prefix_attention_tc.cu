@@ -187,40 +187,9 @@ TMAC_DEV void put_rows(const AttnArgs& a, const Job& j, const RowOf& row, bool m
     }
 }
 
-// The row's result key by key from the pools, only over the keys that it sees: for
-// jobs whose products met an infinite or NaN value, which 0 times is not 0.
-template <typename T, int D>
-__device__ __noinline__ void row_by_keys(const AttnArgs& a, const Job& j, const RowOf& row, int key0, int key1, float scale)
-{
-    const T* q = (const T*)a.q + row.token * a.q_stride + row.head * D;
-    float m = -INFINITY, l = 0.0f, o[D];
-    for (int d = 0; d < D; d++) o[d] = 0.0f;
-    const int shift = a.cache.page_shift;
-    for (int key = key0; key < min(key1, row.p_limit); key++) {
-        const int64_t page = a.prefix_pages[key >> shift];
-        const bool known = page >= 0 && page < a.cache.n_pages;
-        const int64_t at = (((page * a.cache.kv_heads + j.kvh) << shift) + (key & ((1 << shift) - 1))) * D;
-        float s = 0.0f;
-        for (int d = 0; d < D; d++) s = __fmaf_rn(Elem<T>::load(q + d), known ? Elem<T>::load((const T*)a.cache.k + at + d) : 0.0f, s);
-        s = __fmul_rn(s, scale);
-        const float mx = fmaxf(m, s), al = m == mx ? 1.0f : exp2_fast(__fsub_rn(m, mx));
-        const float p = s == -INFINITY ? 0.0f : exp2_fast(__fsub_rn(s, mx));
-        l = __fmaf_rn(l, al, p);
-        for (int d = 0; d < D; d++) {
-            o[d] = __fmul_rn(o[d], al);
-            if (p != 0.0f) o[d] = __fmaf_rn(p, known ? Elem<T>::load((const T*)a.cache.v + at + d) : 0.0f, o[d]);
-        }
-        m = mx;
-    }
-    for (int d = 0; d < D; d++) {
-        const float one[1] = {o[d]};
-        put_results<T, D, 1>(a, j, row, d, m, l, one);
-    }
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kTcThreads, 2)
-    attn_tc_kernel(AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map)
+    attn_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map)
 {
     using C = Conf<D>;
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -474,10 +443,11 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                         make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
             }
             __syncwarp();
-            const bool wanted = r < j.rows, again = wanted && !finite && row.p_limit < key1;
+            const bool wanted = r < j.rows && finite;
             if (wanted && a.parts > 1) a.part_ml[((int64_t)row.token * a.heads + row.head) * a.parts + j.part] = make_float2(m, l);
-            put_rows<T, D>(a, j, row, wanted && !again, l, rows);
-            if (again) row_by_keys<T, D>(a, j, row, key0, key1, __fmul_rn(a.scale, 1.44269504f));
+            put_rows<T, D>(a, j, row, wanted, l, rows);
+            for (uint32_t again = __ballot_sync(0xffffffffu, r < j.rows && !finite); again; again &= again - 1)
+                row_by_keys<T, D>(a, j, quarter * 32 + __ffs(again) - 1);
         }
         tc_fence_before();
     }
