@@ -5,7 +5,7 @@ import math
 import pytest
 
 import tmac_zynq_fpga_b200 as tm
-from test_serving_gpu import BF16, F16, F32, INF, NAN, TINY, U, no_error
+from test_serving_gpu import BF16, F16, F32, INF, NAN, TINY, U, ints, no_error
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -69,6 +69,25 @@ def check(out, want, tol):
     assert torch.isfinite(want).all() and (off <= 0).all(), f"worst {off.max().item():.3g} past the tolerance"
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("batch,n", LAYOUTS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_key_of_minus_infinity_weighs_nothing(dtype, batch, n, dim):
+    q, k, v = random_rows(dim, batch, n, dtype)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    k[5::7, :, 3] = -INF
+    check(attend(q, k, v), *formula(q, k, v))
+
+
+@pytest.mark.parametrize("batch,n", LAYOUTS)
+def test_keys_as_large_as_the_type_allows(batch, n):
+    q, k, v = random_rows(64, batch, n, F32)
+    q[..., 9] = 2.0 ** -126
+    k[::3, :, 9] = torch.finfo(F32).max
+    k[1::3, :, 9] = -torch.finfo(F32).max
+    check(attend(q, k, v), *formula(q, k, v))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("batch,n", LAYOUTS)
 def test_large_values_whose_weights_grow_along_the_keys(dtype, batch, n):
@@ -80,3 +99,38 @@ def test_large_values_whose_weights_grow_along_the_keys(dtype, batch, n):
     k[64:, :, 0] = 24 * math.log(2)  # times 8 / sqrt(64)
     v = (v.float() * 2.0 ** 110).to(dtype)
     check(attend(q, k, v), *formula(q, k, v))
+
+
+# float32 NaNs as Python writes them, as the GPU's arithmetic gives them, and their negatives
+NANS = {F32: [0x7FC00000, 0x7FFFFFFF, -1, -0x400000, 0x7F800001, 0x7FFFF000], F16: [0x7E00, 0x7FFF, -1, 0x7C01], BF16: [0x7FC0, 0x7FFF, -1, 0x7F81]}
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("batch,n", LAYOUTS)
+@pytest.mark.parametrize("where", ["q", "k", "v"])
+def test_every_nan_reaches_the_rows_that_see_it(dtype, batch, n, where):
+    whole = torch.int32 if dtype == F32 else torch.int16
+    for bits in NANS[dtype]:
+        rows = dict(zip("qkv", random_rows(64, batch, n, dtype)))
+        at = 1 if where == "q" else n - 20
+        rows[where].view(whole)[at, :, 6] = bits
+        out = attend(**rows)
+        if where == "q":
+            assert torch.isnan(out[at]).all()
+            others = torch.arange(batch, device="cuda") != at
+            want, tol = formula(rows["q"][others], rows["k"], rows["v"])
+            check(out[others], want, tol)
+        elif where == "k":
+            assert torch.isnan(out).all()
+        else:
+            assert torch.isnan(out[..., 6]).all() and torch.isfinite(out[..., 7]).all()
+
+
+@pytest.mark.parametrize("batch,n", LAYOUTS)
+def test_nans_of_the_gpu_do_not_reach_rows_that_see_less(batch, n):
+    q, k, v = random_rows(64, batch, n, F32)
+    seen = n - 30
+    for x in (k, v):
+        x.view(torch.int32)[seen:, :, 6] = 0x7FFFFFFF
+    out = attend(q, k, v, prefix_lens=ints([seen] * batch))
+    check(out, *formula(q, k[:seen], v[:seen]))

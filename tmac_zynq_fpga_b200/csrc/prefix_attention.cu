@@ -157,12 +157,15 @@ TMAC_DEV void mma1688(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x as the nearest tf32 number and the rest, rounded to one (the product reads the
-// upper 19 bits).
+// x as the nearest tf32 number and the rest (the product reads the upper 19 bits of
+// each).  Nothing is added to the rest's bits: that of a NaN or an infinity is the NaN
+// 0x7FFFFFFF, which an addition would turn into -0, and so would be lost where the
+// addition above has turned x into -0 already.  A number that rounds to infinity has an
+// infinite rest of the other sign.  Rows with such sums are computed again (row_by_keys).
 TMAC_DEV void split_tf32(float x, uint32_t& hi, uint32_t& lo)
 {
     hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
-    lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi))) + 0x1000u;
+    lo = __float_as_uint(__fsub_rn(x, __uint_as_float(hi)));
 }
 // main += a b without the products of rests, which go to rest; a split already.
 TMAC_DEV void mma_f32(float (&main)[4], float (&rest)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], float b0, float b1)
