@@ -126,6 +126,16 @@ def test_every_nan_reaches_the_rows_that_see_it(dtype, batch, n, where):
             assert torch.isnan(out[..., 6]).all() and torch.isfinite(out[..., 7]).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_a_nan_far_below_the_largest_score_is_not_lost_in_the_join(dtype):
+    """The NaN's neighbours in its range of keys weigh nothing against a key of another range."""
+    q, k, v = random_rows(64, 9, 3000, dtype)
+    q[..., 0], k[:, :, 0] = 16.0, -60.0
+    k[0, :, 0] = 60.0
+    k[2500, :, 5] = NAN
+    assert torch.isnan(attend(q, k, v)).all()
+
+
 @pytest.mark.parametrize("batch,n", LAYOUTS)
 def test_nans_of_the_gpu_do_not_reach_rows_that_see_less(batch, n):
     q, k, v = random_rows(64, batch, n, F32)

@@ -505,7 +505,8 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(AttnArgs a)
         mx = m;
 #pragma unroll
         for (int w = 0; w < kWarps; w++) mx = fmaxf(mx, red[w][0]);
-        const float f = p.y == 0.0f ? 0.0f : power<T>(__fsub_rn(p.x, mx));  // 0: saw no key
+        // 0: saw no key; a NaN stays one, however little the part weighs
+        const float f = p.y == 0.0f || p.y != p.y ? p.y : power<T>(__fsub_rn(p.x, mx));
         weight[threadIdx.x] = f;
         float sum = f == 0.0f ? 0.0f : __fmul_rn(f, p.y);
 #pragma unroll
