@@ -144,3 +144,18 @@ def test_nans_of_the_gpu_do_not_reach_rows_that_see_less(batch, n):
         x.view(torch.int32)[seen:, :, 6] = 0x7FFFFFFF
     out = attend(q, k, v, prefix_lens=ints([seen] * batch))
     check(out, *formula(q, k[:seen], v[:seen]))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("batch,n", LAYOUTS)
+@pytest.mark.parametrize("gap", [12.0, 15.0, 17.5])
+@pytest.mark.parametrize("at", ["first", "last"])
+def test_many_small_weights_beside_a_key_without_value(dtype, batch, n, gap, at):
+    """One key takes nearly all of the weight and its value is 0: the result is the small weights' alone."""
+    q, k, v = random_rows(64, batch, n, dtype)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 8.0  # times k / sqrt(64)
+    one = 0 if at == "first" else n - 1
+    k[one, :, 0], v[one] = gap, 0
+    v = v.abs()
+    check(attend(q, k, v), *formula(q, k, v))

@@ -92,8 +92,11 @@ struct Copier {
 // Tiles of 16 rows per warp.  With up to 16 rows in the job the four warps take
 // different 16 keys of a tile and join at the end; with more they take different rows.
 // 16-bit weights are rounded to the elements' type for the second product, as the
-// values are.
+// values are.  f16 has its 11 bits down to 2^-14 only: there the largest weight is 2^15,
+// not 1, so that weights down to 2^-29 of it keep them and none above 2^-40 is lost.
 constexpr int kMmaRows = 16, kStep = 16;
+template <typename T>
+constexpr float kLargestPower = std::is_same_v<T, __half> ? 15.0f : 0.0f;
 template <typename T, int D>
 struct MmaConf;
 // 16-bit rows lie unpadded, their 16-byte pieces turned by the row's number: eight
@@ -317,7 +320,7 @@ TMAC_DEV void attn_mma(const AttnArgs& a)
                     }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                mx = fmaxf(mx, m[h]);
+                mx = fmaxf(__fsub_rn(mx, kLargestPower<T>), m[h]);
                 al[h] = mx == m[h] ? 1.0f : power<T>(__fsub_rn(m[h], mx));
                 const float base = mx == -INFINITY ? 0.0f : mx;  // sees nothing yet: all 0
                 float sum = 0.0f;

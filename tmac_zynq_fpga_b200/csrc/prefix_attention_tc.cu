@@ -10,8 +10,9 @@
 // thread's registers before their weights are formed, so the next tile's product
 // runs beneath them; P has two buffers.  O stays in TMEM.
 //
-// A weight is 2^(s - m) with m the largest score of the row's first tile, kept as
-// long as no tile's sum of weights passes a limit (2^8 in f16, which ends at 2^16;
+// A weight is 2^(s - m) with m from the largest score of the row's first tile (in f16
+// 8 less: its 11 bits end at 2^-14, and so at 2^-22 of the tile's largest weight), kept
+// as long as no tile's sum of weights passes a limit (2^15 in f16, which ends at 2^16;
 // 2^30 in bf16): a product and a rounding do not lose precision by a common factor.
 // Only a tile that passes it pays for a new maximum, the rescaling of O, and its
 // weights anew.  One thread issues the products, one warp the TMA copies of the pages
@@ -346,7 +347,8 @@ __global__ void __launch_bounds__(kTcThreads, 2)
         }
         // exponentials are powers of 2; not 0, so that a masked score's -inf stays one
         const float scale = fmaxf(__fmul_rn(fabsf(a.scale), 1.44269504f), 1e-37f);
-        constexpr float kLimit = std::is_same_v<T, __half> ? 256.0f : 1073741824.0f;
+        constexpr float kLimit = std::is_same_v<T, __half> ? 32768.0f : 1073741824.0f;
+        constexpr float kFirstPower = std::is_same_v<T, __half> ? 8.0f : 0.0f;  // the largest weight under a new m
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
         // V's rows past the keys hold what the page or an earlier tile holds: zeros instead
@@ -386,10 +388,11 @@ __global__ void __launch_bounds__(kTcThreads, 2)
                 float sum = 0.0f;
                 for (bool fits = m > -INFINITY, found = false;; found = true) {
                     if (__any_sync(0xffffffffu, !fits)) {  // a larger m
-                        float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int c = 0; c < 64; c++) top[c & 3] = fmaxf(top[c & 3], __fmul_rn(__uint_as_float(x[c / 32][c % 32]), scale));
-                        const float mx = fits ? m : fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                        const float mx = fits ? m : fmaxf(m, __fsub_rn(most, kFirstPower));
                         const float al = mx == m ? 1.0f : exp2_fast(__fsub_rn(m, mx));
                         m = mx;
                         l = __fmul_rn(l, al);
