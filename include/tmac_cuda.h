@@ -540,9 +540,11 @@ int tmac_rope_append(const tmac_paged_cache* cache, int type, const void* q, int
  *   q, out:       [tokens] rows of `heads` heads of head_dim (64 or 128) values of the
  *                 cache's type, token strides in elements; query heads
  *                 h * heads / kv_heads .. share key/value head h.
- *   q_start:      int32 [batch + 1], non-decreasing: sequence b's tokens are
- *                 q_start[b] .. q_start[b + 1], at most max_q; NULL: one each
- *                 (batch = tokens, max_q = 1).
+ *   q_start:      int32 [batch + 1], non-decreasing, 0 .. tokens (else recorded):
+ *                 sequence b's tokens are q_start[b] .. q_start[b + 1], at most max_q;
+ *                 NULL: one each (batch = tokens, max_q = 1).  The rows of tokens before
+ *                 q_start[0] and from q_start[batch] on (padding), and of a sequence's
+ *                 tokens past max_q (recorded), are zeros.
  *   prefix_pages: int32, the pages of the prefix's prefix_len positions in order.
  *   prefix_lens:  optional int32 [batch], how much of it each sequence shares;
  *                 NULL: all.  Larger than prefix_len: counts as prefix_len, recorded.

@@ -5,7 +5,7 @@ import math
 import pytest
 
 import tmac_zynq_fpga_b200 as tm
-from test_serving_gpu import BF16, F16, F32, INF, NAN, TINY, U, ints, no_error
+from test_serving_gpu import BF16, F16, F32, INF, NAN, TINY, U, attention_case, bounds_error, ints, no_error
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -159,3 +159,43 @@ def test_many_small_weights_beside_a_key_without_value(dtype, batch, n, gap, at)
     k[one, :, 0], v[one] = gap, 0
     v = v.abs()
     check(attend(q, k, v), *formula(q, k, v))
+
+
+# (prefix, own keys): every sequence reads the prefix itself; own keys alone, in one job and in several; joined;
+# one job over the prefix alone; on tcgen05 (16 bits), joined and in one job
+def rows_of_no_sequence_cases():
+    few, many = [2, 3, 0, 1], [2, 3, 0, 1] * 80
+    return [(75, [5, 40, 0, 17], few), (0, [5, 40, 0, 17], few), (0, [600] * 320, many), (0, [900, 700, 0, 1000], few), (1000, [5, 40, 0, 17], few),
+            (600, [0] * 320, many), (600, [0] * 2400, many[:240] * 10), (3500, [3, 9, 0, 2] * 30, many[:120])]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("case", range(8))
+def test_rows_of_no_sequence_are_zeros(dtype, case):
+    prefix, own, queries = rows_of_no_sequence_cases()[case]
+    c = attention_case(dtype, 14, 2, 64, 16, prefix, own, queries)
+    before, after = 3, 70
+    q = torch.cat([c["q"][:1].expand(before, -1, -1), c["q"], c["q"][:1].expand(after, -1, -1)])
+    out = torch.full_like(q, NAN)
+    kw = {**c["kw"], "q_start": c["kw"]["q_start"] + before, "max_own": max(own)}
+    tm.prefix_attention(q, tm.PagedCache(c["k"], c["v"]), c["tables"], c["lens"], out=out, **kw)
+    no_error()  # padding is no error
+    assert not out[:before].any() and not out[-after:].any()
+    check(out[before:-after], c["want"], c["tol"])
+    # tokens past max_q
+    out.fill_(NAN)
+    tm.prefix_attention(q, tm.PagedCache(c["k"], c["v"]), c["tables"], c["lens"], out=out, **{**kw, "max_q": 2})
+    bounds_error()
+    third = torch.tensor([sum(queries[:b]) + before + 2 for b, n in enumerate(queries) if n == 3], device="cuda")
+    assert torch.isfinite(out).all() and not out[third].any() and out[third - 1].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("prefix,own", [(75, 9), (1000, 9)])
+@pytest.mark.parametrize("starts", [[0, 2, 7], [0, 3, 2], [-1, 2, 3], [5, 5, 5]])
+def test_bad_starts_are_errors(dtype, prefix, own, starts):
+    c = attention_case(dtype, 14, 2, 64, 16, prefix, [own] * 2, [2, 1])
+    out = torch.full_like(c["q"], NAN)
+    tm.prefix_attention(c["q"], tm.PagedCache(c["k"], c["v"]), c["tables"], c["lens"], out=out, **{**c["kw"], "q_start": ints(starts), "max_q": 3})
+    bounds_error()
+    assert torch.isfinite(out).all()

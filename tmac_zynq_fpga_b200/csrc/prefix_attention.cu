@@ -470,6 +470,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, kJobsOfSm<T, D>) attn_mma_kernel(const __grid_constant__ AttnArgs a)
 {
     attn_mma<T, D>(a);
+    if (a.q_start && a.parts == 1) clear_rows<T, D, kWarps * kMmaRows>(a);
     // Where the tcgen05 kernel runs beside this one, this grid ends after it, so the
     // join, which waits for this grid, has waited for both.
     if (blockIdx.x == 0) pdl_wait();
@@ -489,9 +490,8 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(AttnArgs a)
     const int token = (int)(row / a.heads), head = (int)(row % a.heads);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = threadIdx.x / kLanes, d4 = threadIdx.x % kLanes;
     const int b = sequence_of(a, token);
-    int own = 0;
-    if (a.o_splits && token_count(a, b) > token - first_token(a, b)) own = (tiles_of(own_len(a, b)) + a.o_range - 1) / a.o_range;
-    const int n = a.p_splits + own;
+    int n = 0;
+    if (is_computed(a, token, b)) n = a.p_splits + (a.o_splits ? (tiles_of(own_len(a, b)) + a.o_range - 1) / a.o_range : 0);
     const float2* ml = a.part_ml + row * a.parts;
     const float4* po = reinterpret_cast<const float4*>(a.part_o + row * a.parts * D) + d4;
     pdl_wait();

@@ -39,13 +39,14 @@ struct AttnArgs {
 TMAC_DEV int first_token(const AttnArgs& a, int b)
 {
     const int t = a.q_start ? a.q_start[b] : b;
+    if (t < 0 || t > a.tokens) record_error(a.err, TMAC_ERR_BOUNDS);
     return max(0, min(t, a.tokens));
 }
 // Query tokens of sequence b: at most max_q are computed, more is an error.
 TMAC_DEV int token_count(const AttnArgs& a, int b)
 {
     const int n = first_token(a, b + 1) - first_token(a, b);
-    if (n > a.max_q) record_error(a.err, TMAC_ERR_BOUNDS);
+    if (n < 0 || n > a.max_q) record_error(a.err, TMAC_ERR_BOUNDS);
     return max(0, min(n, a.max_q));
 }
 TMAC_DEV int own_len(const AttnArgs& a, int b)
@@ -73,6 +74,13 @@ TMAC_DEV int sequence_of(const AttnArgs& a, int token)
             hi = mid - 1;
     }
     return lo;
+}
+// Whether a token's rows are computed, b its sequence_of: rows of tokens outside
+// q_start[0] .. q_start[batch], and past a sequence's max_q, are zeros.
+TMAC_DEV bool is_computed(const AttnArgs& a, int token, int b)
+{
+    const int i = token - first_token(a, b);
+    return i >= 0 && i < token_count(a, b);
 }
 
 // Up to so many key tiles (prefix and own) every sequence reads the prefix itself, in
@@ -265,6 +273,33 @@ __device__ __noinline__ void row_by_keys(const AttnArgs& a, Job j, int r)
         }
     }
     put_results<T, D, kPer>(a, j, row, d, m, l, o);
+}
+
+// Zeros for the rows that belong to no sequence or lie past its max_q, where jobs write
+// the result and no join follows: by jobs of the prefix for their own rows, when all
+// threads have written theirs; by a sequence's first job up to the next sequence.
+template <typename T, int D, int kJobRows>
+__device__ __noinline__ void clear_rows(const AttnArgs& a)
+{
+    Job j;
+    find_job<kJobRows>(a, &j);
+    const int width = a.group * D;
+    const auto clear = [&](int from, int to) {
+        for (int64_t i = threadIdx.x; i < (int64_t)(to - from) * width; i += blockDim.x)
+            Elem<T>::store((T*)a.out + (from + i / width) * a.out_stride + j.kvh * width + i % width, 0.0f);
+    };
+    if (j.seq < 0) {
+        __syncthreads();
+        for (int token = j.row0 / a.group; token * a.group < j.row0 + j.rows; token++)
+            if (!is_computed(a, token, sequence_of(a, token))) {
+                const int first = max(0, j.row0 - token * a.group), last = min(a.group, j.row0 + j.rows - token * a.group);
+                for (int i = first * D + threadIdx.x; i < last * D; i += blockDim.x)
+                    Elem<T>::store((T*)a.out + token * a.out_stride + j.kvh * width + i, 0.0f);
+            }
+    } else if (j.row0 == 0) {
+        if (j.seq == 0) clear(0, first_token(a, 0));
+        clear(j.token0 + token_count(a, j.seq), j.seq + 1 < a.batch ? first_token(a, j.seq + 1) : a.tokens);
+    }
 }
 
 // prefix_attention_tc.cu: the prefix's jobs of 16-bit elements on tcgen05.

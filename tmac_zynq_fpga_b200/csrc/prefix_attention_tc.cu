@@ -457,6 +457,7 @@ __global__ void __launch_bounds__(kTcThreads, 2)
     __syncthreads();
     tc_fence_after();
     if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+    if (a.q_start && a.parts == 1) clear_rows<T, D, kTcRows>(a);
 }
 
 template <typename T, int D>

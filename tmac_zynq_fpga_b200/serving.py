@@ -131,7 +131,8 @@ def prefix_attention(q, cache, tables, own_lens, *, prefix_pages=None, prefix_le
     default what the tables hold); prefix_pages int32, prefix_len: the shared positions;
     prefix_lens int32 [batch]: how much of them each sequence sees (all).  q_start int32
     [batch + 1] with max_q: several query tokens per sequence, each seeing the keys up to
-    its own; without it one per sequence.  See tmac_prefix_attention."""
+    its own, and zeros for tokens of no sequence; without it one per sequence.  See
+    tmac_prefix_attention."""
     if stream is not None:
         with _on(stream, cache.k.device):
             return prefix_attention(q, cache, tables, own_lens, prefix_pages=prefix_pages, prefix_len=prefix_len,
