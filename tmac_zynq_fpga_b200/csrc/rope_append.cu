@@ -6,8 +6,8 @@
 // For pair i of a head, with c = cos[pos][i], s = sin[pos][i]:
 //   (a, z) -> (a c - z s, a s + z c),
 // pairs (2i, 2i + 1) when interleaved, else (i, i + rot_dim / 2); the values past
-// rot_dim pass through.  Products and sums are 32-bit, rounded once to the
-// cache's type.
+// rot_dim pass through.  Products and sums are 32-bit, each rounded by itself as in the
+// reference, and the result once to the cache's type.
 //
 // Bound: HBM, every value is read once and written once (32768 tokens of 16/4 heads of
 // 128, bf16, 91 us, 4560 GB/s; 512 tokens 3.5 us, 2 tokens 3.4, the launch).  Where
@@ -24,6 +24,14 @@
 
 namespace tmac {
 namespace {
+
+// (a, z) by cosine c and sine s; every kernel rounds the same, whatever the layout.
+TMAC_DEV void rotate(float& a, float& z, float c, float s)
+{
+    const float x = __fadd_rn(__fmul_rn(a, c), -__fmul_rn(z, s));
+    z = __fadd_rn(__fmul_rn(a, s), __fmul_rn(z, c));
+    a = x;
+}
 
 struct RopeArgs {
     const void *q, *k, *v;
@@ -109,10 +117,7 @@ __global__ void __launch_bounds__(256) rope_append_kernel(RopeArgs a)
                 z = __fadd_rn(z, a.bias[(int64_t)row * d + d1]);
             }
             if (turn) {
-                const float c = a.cos[(int64_t)p.pos * (a.rot / 2) + pair], s = a.sin[(int64_t)p.pos * (a.rot / 2) + pair];
-                const float xr = __fadd_rn(__fmul_rn(x, c), -__fmul_rn(z, s));
-                z = __fadd_rn(__fmul_rn(x, s), __fmul_rn(z, c));
-                x = xr;
+                rotate(x, z, a.cos[(int64_t)p.pos * (a.rot / 2) + pair], a.sin[(int64_t)p.pos * (a.rot / 2) + pair]);
             }
         }
         Elem<C>::store(dst + d0, x);
@@ -272,22 +277,14 @@ __global__ void __launch_bounds__(kMaxThreads<T>, sizeof(T) == 2 ? 2 : 1) rope_a
                 const float4 c4 = *reinterpret_cast<const float4*>(c + d0 / 2), s4 = *reinterpret_cast<const float4*>(s + d0 / 2);
                 const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float y = __fmaf_rn(x[2 * i], cv[i], -__fmul_rn(x[2 * i + 1], sv[i]));
-                    x[2 * i + 1] = __fmaf_rn(x[2 * i], sv[i], __fmul_rn(x[2 * i + 1], cv[i]));
-                    x[2 * i] = y;
-                }
+                for (int i = 0; i < 4; i++) rotate(x[2 * i], x[2 * i + 1], cv[i], sv[i]);
             } else if (halves) {
 #pragma unroll
                 for (int h = 0; h < 8; h += 4) {
                     const float4 c4 = *reinterpret_cast<const float4*>(c + d0 + h), s4 = *reinterpret_cast<const float4*>(s + d0 + h);
                     const float cv[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float y = __fmaf_rn(x[h + i], cv[i], -__fmul_rn(z[h + i], sv[i]));
-                        z[h + i] = __fmaf_rn(x[h + i], sv[i], __fmul_rn(z[h + i], cv[i]));
-                        x[h + i] = y;
-                    }
+                    for (int i = 0; i < 4; i++) rotate(x[h + i], z[h + i], cv[i], sv[i]);
                 }
             }
             store8(dst, x);
