@@ -42,8 +42,8 @@ struct DeviceGuard {
     bool ok = true;
     explicit DeviceGuard(int dev)
     {
-        if (cudaGetDevice(&prev) != cudaSuccess) { ok = false; return; }
-        if (prev != dev && cudaSetDevice(dev) != cudaSuccess) ok = false;
+        ok = cudaGetDevice(&prev) == cudaSuccess && (prev == dev || cudaSetDevice(dev) == cudaSuccess);
+        if (!ok) cudaGetLastError();  // not the next launch's
     }
     ~DeviceGuard()
     {

@@ -61,12 +61,17 @@ int* device_error_word(int device)
 
 int num_sms(int device)
 {
+    constexpr int kSms = 148;  // of a B200: for a device that is not there, which the caller refuses
+    if (device < 0) return kSms;
     std::lock_guard<std::mutex> lk(g_dev_mutex);
-    if ((int)g_sms.size() <= device) g_sms.resize(device + 1, 0);
-    if (!g_sms[device]) {
+    if ((int)g_sms.size() <= device || !g_sms[device]) {
         int n = 0;
-        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
-        g_sms[device] = n > 0 ? n : 148;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) {
+            cudaGetLastError();  // not the next launch's
+            return kSms;
+        }
+        if ((int)g_sms.size() <= device) g_sms.resize(device + 1, 0);
+        g_sms[device] = n;
     }
     return g_sms[device];
 }

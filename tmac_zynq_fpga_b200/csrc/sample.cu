@@ -1168,6 +1168,7 @@ extern "C" int tmac_sample(const void* logits, int type, int64_t row_stride, int
     if (batch < 0 || batch > 0x7FFFFFF) return fail(TMAC_ERR_SHAPE, "batch out of range");
     if (vocab <= 0 || vocab > kMaxVocab) return fail(TMAC_ERR_SHAPE, "vocab must be 1 to 720000");
     if (batch > 1 && row_stride && row_stride < vocab) return fail(TMAC_ERR_SHAPE, "row_stride must cover a row");
+    if (device < 0) return fail(TMAC_ERR_NODEV, "no such CUDA device");
     if (batch == 0) return TMAC_OK;
     if (!logits || !u || !tokens || !probs) return fail(TMAC_ERR_INVALID, "NULL argument");
     if ((uintptr_t)logits % bytes) return fail(TMAC_ERR_INVALID, "logits are not aligned to their type");

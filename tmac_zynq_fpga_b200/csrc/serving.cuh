@@ -110,6 +110,7 @@ inline int check_cache(const tmac_paged_cache* c, CacheDev* out)
         return fail(TMAC_ERR_SHAPE, "page_size must be a power of two up to 256");
     if (c->head_dim < 2 || c->head_dim > 1024 || c->head_dim % 2)
         return fail(TMAC_ERR_SHAPE, "head_dim must be even, 2 to 1024");
+    if (c->device < 0) return fail(TMAC_ERR_NODEV, "no such CUDA device");
     if ((uintptr_t)c->k % 16 || (uintptr_t)c->v % 16) return fail(TMAC_ERR_INVALID, "cache pools must be 16-byte aligned");
     out->k = c->k;
     out->v = c->v;
