@@ -551,6 +551,7 @@ int tmac_rope_append(const tmac_paged_cache* cache, int type, const void* q, int
  *   tables:       int32 [batch][table_width], the pages of each sequence's own
  *                 positions in order; entries past its length are not read.
  *   own_lens:     int32 [batch], 0 .. max_own (larger: counts as max_own, recorded).
+ *   scale:        finite.
  *   workspace:    tmac_prefix_attention_workspace bytes, 16-byte aligned, free
  *                 for other use when the call's kernels have run.
  * Rows of a page outside the pool count as zeros (recorded).

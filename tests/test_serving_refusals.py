@@ -18,3 +18,9 @@ def test_no_such_device(device):
     n = ctypes.c_size_t(0)
     rc = tm.lib().tmac_prefix_attention_workspace(ctypes.addressof(c), 14, 3, 3, 1, 40000, 64, ctypes.addressof(n))
     assert rc == (NODEV if device < 0 else 0)  # a size needs no device
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_attention_refuses_a_scale_that_is_not_finite(scale):
+    assert attend(scale=scale) == -1
+    assert attend(scale=scale, prefix=40000) == -1

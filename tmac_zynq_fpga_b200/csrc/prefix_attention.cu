@@ -31,6 +31,8 @@
 // at 2200.
 #include "prefix_attention.cuh"
 
+#include <cmath>
+
 namespace tmac {
 namespace {
 
@@ -697,6 +699,7 @@ extern "C" int tmac_prefix_attention(const tmac_paged_cache* cache, const void* 
     if (batch == 0) return fail(TMAC_ERR_SHAPE, "tokens without sequences");
     if (!q_start && (batch != tokens || max_q != 1))
         return fail(TMAC_ERR_SHAPE, "without q_start there is one token per sequence");
+    if (!std::isfinite(scale)) return fail(TMAC_ERR_INVALID, "scale must be finite");
     if (prefix_len && !prefix_pages) return fail(TMAC_ERR_INVALID, "NULL prefix_pages");
     if (max_own && (!tables || !own_lens)) return fail(TMAC_ERR_INVALID, "NULL tables or own_lens");
     const int64_t row = (int64_t)heads * cache->head_dim;
