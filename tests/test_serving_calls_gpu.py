@@ -15,3 +15,39 @@ def test_a_refused_device_leaves_nothing_behind():
         assert draw(device=device) == -9 and append(cache(device=device)) == -9
         check_append(append_case(BF16, BF16, 14, 2, 64, 64, 16, 5))
         torch.zeros(3, device="cuda").add_(1)
+
+
+def busy_stream():
+    """A stream that is some tenths of a second behind."""
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)
+    return side
+
+
+@pytest.mark.parametrize("by_address", [False, True])
+@pytest.mark.parametrize("which", ["rope_append", "prefix_attention", "sample"])
+def test_arguments_dropped_after_a_call_on_another_stream(which, by_address):
+    """torch must not give their memory to the next tensor while that stream has yet to read it."""
+    c = append_case(BF16, BF16, 14, 2, 64, 64, 16, 64, n_seq=64)
+    cache = tm.PagedCache(*c["pools"])
+    inputs = {"rope_append": c["q"].contiguous(), "prefix_attention": c["q"].contiguous(), "sample": torch.randn(64, 5000, device="cuda")}[which]
+    lens, u = c["pos"] - c["starts"] + 1, torch.full((64,), 0.5, device="cuda")
+
+    def call(x, **kw):
+        if which == "rope_append":
+            return tm.rope_append(cache, x, c["k"], c["v"], c["pos"], c["tables"], c["cos"], c["sin"], starts=c["starts"], **kw)
+        if which == "prefix_attention":
+            return tm.prefix_attention(x, cache, c["tables"], lens, **kw)
+        return tm.sample(x, u, **kw)[0]
+
+    tm.rope_append(cache, c["q"], c["k"], c["v"], c["pos"], c["tables"], c["cos"], c["sin"], starts=c["starts"])
+    want = call(inputs)
+    temporary = inputs.clone()
+    torch.cuda.synchronize()
+    side = busy_stream()
+    got = call(temporary, stream=side.cuda_stream if by_address else side)
+    del temporary
+    later = [torch.full_like(inputs, -7.0) for _ in range(4)]
+    side.synchronize()
+    assert torch.equal(got, want) and len(later) == 4

@@ -8,7 +8,9 @@ decode step"): several sequences, which may share a prefix, advance together.
 * ``sample``            -- temperature, top-k, top-p, min-p and a draw
 
 Tensors are torch CUDA tensors; results are allocated on the stream that is used: the
-one given (a torch stream or a raw address), else torch's current stream.
+one given (a torch stream or a raw address), else torch's current stream.  Arguments may
+be dropped once the call has returned; what was queued on another stream must be waited
+for by the one that is used.
 """
 from __future__ import annotations
 
@@ -61,11 +63,15 @@ def _refuse(code, msg):
     raise tm.TmacError(code, msg)
 
 
-def _on(stream, device):
-    """The context in which `stream`, a torch stream or an address, is torch's current one."""
+def _on(stream, device, *tensors):
+    """The context in which `stream`, a torch stream or an address, is torch's current one.
+    The memory of `tensors` (None among them) is not reused before the stream has read it."""
     import torch
     if isinstance(stream, int):
         stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.is_cuda:
+            t.record_stream(stream)
     return torch.cuda.stream(stream)
 
 
@@ -115,7 +121,7 @@ def rope_append(cache, q, k, v, pos, tables, cos, sin, *, seq=None, starts=None,
     int32 [n_seq]; cos, sin float32 [max_pos, rot_dim / 2] (`rope_table`); bias float32
     [(heads + 2 kv_heads) * head_dim].  See tmac_rope_append for the places they name."""
     if stream is not None:
-        with _on(stream, cache.k.device):
+        with _on(stream, cache.k.device, cache.k, cache.v, q, k, v, pos, tables, cos, sin, seq, starts, bias, q_out):
             return rope_append(cache, q, k, v, pos, tables, cos, sin, seq=seq, starts=starts, interleaved=interleaved, bias=bias,
                                q_out=q_out)
     return (_native or _ext()).rope_append(cache.k, cache.v, q, k, v, pos, tables, cos, sin, seq, starts, interleaved, bias, q_out)
@@ -134,7 +140,7 @@ def prefix_attention(q, cache, tables, own_lens, *, prefix_pages=None, prefix_le
     its own, and zeros for tokens of no sequence; without it one per sequence.  See
     tmac_prefix_attention."""
     if stream is not None:
-        with _on(stream, cache.k.device):
+        with _on(stream, cache.k.device, q, cache.k, cache.v, tables, own_lens, prefix_pages, prefix_lens, q_start, out):
             return prefix_attention(q, cache, tables, own_lens, prefix_pages=prefix_pages, prefix_len=prefix_len,
                                     prefix_lens=prefix_lens, q_start=q_start, max_q=max_q, max_own=max_own, scale=scale, out=out)
     return (_native or _ext()).prefix_attention(q, cache.k, cache.v, tables, own_lens, prefix_pages, prefix_len, prefix_lens, q_start,
@@ -147,6 +153,6 @@ def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, s
     float32 [batch].  u float32 [batch] in [0, 1); temperature, top_p, min_p float32
     [batch], top_k int32 [batch], each optional.  See tmac_sample for the filters."""
     if stream is not None:
-        with _on(stream, logits.device):
+        with _on(stream, logits.device, logits, u, temperature, top_k, top_p, min_p):
             return sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
     return (_native or _ext()).sample(logits, u, temperature, top_k, top_p, min_p)
