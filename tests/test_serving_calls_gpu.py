@@ -51,3 +51,30 @@ def test_arguments_dropped_after_a_call_on_another_stream(which, by_address):
     later = [torch.full_like(inputs, -7.0) for _ in range(4)]
     side.synchronize()
     assert torch.equal(got, want) and len(later) == 4
+
+
+def test_a_tensor_that_requires_grad_is_refused():
+    """The operators have no gradient: a result without history would train nothing, silently."""
+    c = append_case(BF16, BF16, 14, 2, 64, 64, 16, 6, n_seq=6)
+    lens = c["pos"] - c["starts"] + 1
+    x = dict(q=c["q"].contiguous(), k=c["k"].contiguous(), v=c["v"].contiguous(), bias=c["bias"], cos=c["cos"], sin=c["sin"], kp=c["pools"][0],
+             vp=c["pools"][1], logits=torch.randn(6, 100, device="cuda"), t=torch.ones(6, device="cuda"))
+
+    def call(which, **kw):
+        d = {**x, **kw}
+        cache = tm.PagedCache(d["kp"], d["vp"])
+        if which == "append":
+            return tm.rope_append(cache, d["q"], d["k"], d["v"], c["pos"], c["tables"], d["cos"], d["sin"], starts=c["starts"], bias=d["bias"])
+        if which == "attention":
+            return tm.prefix_attention(d["q"], cache, c["tables"], lens)
+        return tm.sample(d["logits"], torch.zeros(6, device="cuda"), temperature=d["t"])[0]
+
+    for which, names in (("append", ["q", "k", "v", "bias", "cos", "sin", "kp", "vp"]), ("attention", ["q", "kp", "vp"]), ("sample", ["logits", "t"])):
+        want = call(which)
+        for name in names:
+            grad = {name: x[name].clone().requires_grad_()}
+            with pytest.raises(tm.TmacError, match="grad"):
+                call(which, **grad)
+            with torch.no_grad():
+                assert torch.equal(call(which, **grad), want)
+            assert torch.equal(call(which, **{name: grad[name].detach()}), want)

@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -58,7 +59,10 @@ int type_of(const at::Tensor& t)
 const at::Tensor& tensor(PyObject* o, const char* name)
 {
     if (!THPVariable_Check(o)) refuse(TMAC_ERR_INVALID, std::string(name) + " must be a torch tensor");
-    return THPVariable_Unpack(o);
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (t.requires_grad() && c10::GradMode::is_enabled())
+        refuse(TMAC_ERR_INVALID, std::string(name) + " requires grad, and these operators have no gradient: detach it, or call under torch.no_grad()");
+    return t;
 }
 int whole(PyObject* o, const char* name)
 {

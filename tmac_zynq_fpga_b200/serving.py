@@ -10,7 +10,8 @@ decode step"): several sequences, which may share a prefix, advance together.
 Tensors are torch CUDA tensors; results are allocated on the stream that is used: the
 one given (a torch stream or a raw address), else torch's current stream.  Arguments may
 be dropped once the call has returned; what was queued on another stream must be waited
-for by the one that is used.
+for by the one that is used.  There are no gradients: a tensor that requires one is refused
+where gradients are enabled.
 """
 from __future__ import annotations
 
