@@ -1,7 +1,9 @@
 """Builds libtmac_cuda.so in-tree: every .cu under csrc/ compiled for sm_100a
 (B200) with nvcc, FMA contraction off (-fmad=false) because results must match
-the reference's fp32/fp64 roundings bit for bit.  Then _serving.so, the CPython
-module that takes torch tensors to the batched decode operators."""
+the reference's fp32/fp64 roundings bit for bit.  Then, where torch is there to
+compile against, _serving.so, the CPython module that takes torch tensors to the
+batched decode operators; nothing else needs it."""
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -36,6 +38,20 @@ def up_to_date():
     return all(os.path.getmtime(d) <= t for d in deps())
 
 
+def binding_needs():
+    """What _serving.so cannot be compiled without and is not here, or None."""
+    if importlib.util.find_spec("torch") is None:
+        return "torch is not installed"
+    import torch
+    if torch.version.cuda is None:
+        return "torch is built without CUDA"
+    if not shutil.which(CXX):
+        return f"no C++ compiler ({CXX})"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "no Python headers"
+    return None
+
+
 def build_binding(force=False, verbose=False):
     """Compiles _serving.so against the installed torch (host code only)."""
     sources = (BINDING, os.path.join(HERE, "..", "include", "tmac_cuda.h"), os.path.abspath(__file__))
@@ -57,7 +73,11 @@ def build_binding(force=False, verbose=False):
 
 def build(force=False, verbose=False, jobs=8):
     out = build_library(force, verbose, jobs)
-    build_binding(force, verbose)
+    missing = binding_needs()
+    if missing:
+        print(f"{os.path.basename(BINDING_OUT)} (the batched decode operators on torch tensors) is not built: {missing}", file=sys.stderr)
+    else:
+        build_binding(force, verbose)
     return out
 
 

@@ -53,7 +53,10 @@ def _ext():
 
         import tmac_zynq_fpga_b200 as tm
         tm.lib()
-        from . import _serving
+        try:
+            from . import _serving
+        except ImportError as e:
+            raise tm.TmacError(-1, f"_serving.so, which buildlib.build() compiles against torch, is missing or of another torch: {e}") from e
         _serving.set_error_class(tm.TmacError)
         _native = _serving
     return _native
