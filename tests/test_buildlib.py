@@ -1,4 +1,4 @@
-"""buildlib.build(): the library alone where torch or a compiler is missing."""
+"""buildlib.build(): the library alone where torch or a compiler is missing, and when _serving.so is compiled anew."""
 import os
 import subprocess
 import sys
@@ -52,6 +52,17 @@ def test_a_compiler_error_is_raised(fresh, monkeypatch):
     monkeypatch.setattr(subprocess, "run", lambda cmd, check: (_ for _ in ()).throw(subprocess.CalledProcessError(1, cmd)))
     with pytest.raises(subprocess.CalledProcessError):
         buildlib.build()
+
+
+def test_the_module_is_compiled_once_for_a_torch_and_anew_for_another(fresh, monkeypatch):
+    torch = pytest.importorskip("torch")
+    buildlib.build()
+    buildlib.build()
+    assert len(fresh) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0.0+other")
+    buildlib.build()
+    buildlib.build()
+    assert len(fresh) == 2
 
 
 def test_operators_without_the_module_say_so():

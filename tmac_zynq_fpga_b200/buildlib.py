@@ -52,10 +52,18 @@ def binding_needs():
     return None
 
 
+def built_against():
+    """The installations that _serving.so is compiled for."""
+    import torch
+    return f"torch {torch.__version__} {os.path.dirname(torch.__file__)}, Python {sys.version}\n"
+
+
 def build_binding(force=False, verbose=False):
     """Compiles _serving.so against the installed torch (host code only)."""
     sources = (BINDING, os.path.join(HERE, "..", "include", "tmac_cuda.h"), os.path.abspath(__file__))
-    if not force and os.path.exists(BINDING_OUT) and all(os.path.getmtime(s) <= os.path.getmtime(BINDING_OUT) for s in sources):
+    stamp = os.path.join(HERE, "_build", os.path.basename(BINDING_OUT) + ".for")
+    if not force and os.path.exists(BINDING_OUT) and all(os.path.getmtime(s) <= os.path.getmtime(BINDING_OUT) for s in sources) and (
+            os.path.exists(stamp) and open(stamp).read() == built_against()):
         return BINDING_OUT
     import torch
     t = os.path.dirname(torch.__file__)
@@ -68,6 +76,9 @@ def build_binding(force=False, verbose=False):
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, BINDING_OUT)
+    os.makedirs(os.path.dirname(stamp), exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(built_against())
     return BINDING_OUT
 
 
