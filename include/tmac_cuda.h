@@ -563,6 +563,11 @@ int tmac_prefix_attention(const tmac_paged_cache* cache, const void* q, int64_t 
                           size_t workspace_bytes, void* stream);
 int tmac_prefix_attention_workspace(const tmac_paged_cache* cache, int heads, int tokens, int batch, int max_q,
                                     int prefix_len, int max_own, size_t* bytes);
+/* Who reads the prefix in a call of these sizes: 0 = each sequence's own jobs (short
+ * ones; also without a prefix), 1 = jobs shared by all sequences, 2 = such jobs on the
+ * tcgen05 kernel; negative: TMAC_ERR_*. */
+int tmac_prefix_attention_engine(const tmac_paged_cache* cache, int heads, int tokens, int batch, int max_q,
+                                 int prefix_len, int max_own);
 
 /*
  * The next token of each row of logits from a given uniform number (stands in

@@ -684,6 +684,14 @@ extern "C" int tmac_prefix_attention_workspace(const tmac_paged_cache* cache, in
     return TMAC_OK;
 }
 
+extern "C" int tmac_prefix_attention_engine(const tmac_paged_cache* cache, int heads, int tokens, int batch, int max_q,
+                                            int prefix_len, int max_own)
+{
+    AttnArgs a = {};
+    const int rc = prepare(cache, heads, tokens, batch, max_q, prefix_len, max_own, 0x7FFFFFFF, &a);
+    return rc ? rc : a.p_jobs == 0 ? 0 : a.tc ? 2 : 1;
+}
+
 extern "C" int tmac_prefix_attention(const tmac_paged_cache* cache, const void* q, int64_t q_stride, int heads,
                                      int tokens, int batch, const int32_t* q_start, int max_q,
                                      const int32_t* prefix_pages, int prefix_len, const int32_t* prefix_lens,

@@ -39,6 +39,7 @@ SIGNATURES = {
     "tmac_prefix_attention": (_INT, [_P, _P, _I64, _INT, _INT, _INT, _P, _INT, _P, _INT, _P, _P, _INT, _P, _INT,
                                      ctypes.c_float, _P, _I64, _P, ctypes.c_size_t, _P]),
     "tmac_prefix_attention_workspace": (_INT, [_P, _INT, _INT, _INT, _INT, _INT, _INT, _P]),
+    "tmac_prefix_attention_engine": (_INT, [_P, _INT, _INT, _INT, _INT, _INT, _INT]),
     "tmac_sample": (_INT, [_P, _INT, _I64, _INT, _INT, _P, _P, _P, _P, _P, _P, _P, _INT, _P]),
 }
 
