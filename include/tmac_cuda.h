@@ -532,7 +532,8 @@ int tmac_rope_append(const tmac_paged_cache* cache, int type, const void* q, int
 
 /*
  * Attention of a batch whose sequences share a prefix; the prefix's keys and
- * values are read once for all of them.  Query token i of sequence b (n_q
+ * values are read once for all of them (a short one may be read by each sequence,
+ * where that takes no longer: tmac_prefix_attention_engine).  Query token i of sequence b (n_q
  * tokens, the last of the sequence) sees the first prefix_lens[b] positions of the
  * prefix and the first own_lens[b] - n_q + 1 + i of the sequence's own; a token
  * that sees none gets zeros.  Keys that a row does not see do not reach its

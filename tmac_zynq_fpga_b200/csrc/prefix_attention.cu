@@ -574,7 +574,10 @@ int plan(AttnArgs* a, int type, int sms)
     };
     a->o_tiles = (int)(((int64_t)a->max_q * a->group + job_rows - 1) / job_rows);
     const int64_t o_jobs = (int64_t)a->batch * a->o_tiles * hk, o_keys = tiles(a->max_own), p_keys = tiles(a->prefix_len);
-    a->alone = o_keys + p_keys <= (type == TMAC_TYPE_F32 ? kAloneTiles32 : kAloneTiles16);
+    const bool wide = type == TMAC_TYPE_F32;
+    a->alone = o_keys + p_keys <= (wide ? kAloneTiles32 : p_keys ? kAloneTiles16 : kOwnTiles16) &&
+               (!p_keys || o_jobs <= (int64_t)sms * jobs_of_sm(type, dim) ||
+                p_keys * (wide ? kAloneRows32 : kAloneRows16) <= (int64_t)a->max_q * a->group);
     if (a->alone) {
         a->p_tiles = a->p_splits = a->p_range = 0;
         a->o_splits = 1;

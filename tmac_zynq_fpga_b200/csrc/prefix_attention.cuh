@@ -83,10 +83,21 @@ TMAC_DEV bool is_computed(const AttnArgs& a, int token, int b)
     return i >= 0 && i < token_count(a, b);
 }
 
-// Up to so many key tiles (prefix and own) every sequence reads the prefix itself, in
-// one job.  Against shared and joined jobs: 16 bits, 3 tiles 6.5 / 8.2 us, 5 tiles 8.3 /
-// 9.4, 9 tiles 9.5 / 9.5; 32 bits, 8 tiles 17.1 / 12.3.
-constexpr int kAloneTiles16 = 8, kAloneTiles32 = 4;
+// Every sequence reads the prefix itself, in one job for all of its keys and without a
+// join, up to so many key tiles in all (without a prefix up to kOwnTiles), and only where
+// that is not more work than the join saves: the jobs are held by the GPU at once, or a
+// sequence's query rows are at least kAloneRows for each tile of the prefix.  Against
+// shared and joined jobs, us, tiles of prefix + own, query/key heads x dims, sequences;
+// 16 bits:
+//   3 + 1  14/2 x 64: 48 7.0 / 9.5, 384 17.0 / 22.8;  16/4 x 128: 48 10.8 / 12.8, 96 19.5 / 16.7
+//   5 + 1  14/2 x 64: 48 8.6 / 9.9, 192 11.7 / 15.2;  8/8 x 64: 16 8.6 / 8.3, 192 37.4 / 22.3
+//   7 + 1  14/2 x 64: 48 10.1 / 9.9;  32/8 x 128: 16 13.4 / 12.7, 192 80.4 / 49.3
+//   0 + 8  14/2 x 64: 16 9.7 / 8.3, 192 13.1 / 19.4
+// 32 bits:
+//   1 + 1  14/2 x 64: 384 23.6 / 28.7;  16/4 x 128: 16 12.9 / 22.9, 192 66 / 55
+//   3 + 1  14/2 x 64: 48 10.7 / 12.4, 384 36.8 / 33.1;  32/8 x 128: 192 201 / 119
+constexpr int kAloneTiles16 = 6, kAloneTiles32 = 4, kOwnTiles16 = 8;
+constexpr int kAloneRows16 = 2, kAloneRows32 = 5;
 // The prefix goes to the tcgen05 kernel from so many rows on, and from so much work
 // (rows x keys x kv heads): at 64 dims 1.4 M took 13.2 us there and 11.8 in the mma
 // kernel, 3.7 M 15.4 and 15.4, 7.3 M 20.7 and 22.0, 59 M 51 and 85; at 128 dims 0.4 M 14.3
