@@ -1,4 +1,7 @@
 """How the operators of the batched decode step are called: devices, streams, gradients."""
+import threading
+import time
+
 import pytest
 
 import tmac_zynq_fpga_b200 as tm
@@ -78,3 +81,46 @@ def test_a_tensor_that_requires_grad_is_refused():
             with torch.no_grad():
                 assert torch.equal(call(which, **grad), want)
             assert torch.equal(call(which, **{name: grad[name].detach()}), want)
+
+
+@pytest.mark.parametrize("which", ["rope_append", "prefix_attention", "sample"])
+def test_other_threads_run_while_a_launch_waits(which):
+    """A stream that takes no more launches holds up the thread that launches, not the interpreter."""
+    c = append_case(BF16, BF16, 2, 1, 64, 64, 16, 2, n_seq=2)
+    cache = tm.PagedCache(*c["pools"])
+    logits, u, lens = torch.zeros(2, 100, device="cuda"), torch.zeros(2, device="cuda"), c["pos"] - c["starts"] + 1
+    q = torch.zeros(2, 2, 64, dtype=BF16, device="cuda")
+
+    def call():
+        if which == "rope_append":
+            tm.rope_append(cache, c["q"], c["k"], c["v"], c["pos"], c["tables"], c["cos"], c["sin"], starts=c["starts"], q_out=q)
+        elif which == "prefix_attention":
+            tm.prefix_attention(q, cache, c["tables"], lens, out=q)
+        else:
+            tm.sample(logits, u)
+
+    call()
+    torch.cuda._sleep(1000)
+    torch.cuda.synchronize()
+    ticks, done = [time.perf_counter()], threading.Event()
+
+    def tick():
+        while not done.is_set():
+            time.sleep(0.002)
+            ticks.append(time.perf_counter())
+
+    other = threading.Thread(target=tick)
+    side = torch.cuda.Stream()
+    other.start()
+    t0 = time.perf_counter()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(3_000_000_000)
+        for _ in range(4000):
+            call()
+    queued = time.perf_counter() - t0
+    done.set()
+    other.join()
+    side.synchronize()
+    longest = max(b - a for a, b in zip(ticks, ticks[1:]))
+    assert queued > 1.0  # the queue was full for most of the stream's sleep
+    assert longest < queued / 2

@@ -35,6 +35,17 @@ void check(int rc)
 {
     if (rc) refuse(rc, tmac_last_error());
 }
+// Calls f without the interpreter's lock: a launch waits while a stream's queue is full,
+// and other Python threads must not wait with it.
+template <typename F>
+int unlocked(F&& f)
+{
+    struct Lock {
+        PyThreadState* state = PyEval_SaveThread();
+        ~Lock() { PyEval_RestoreThread(state); }
+    } lock;
+    return f();
+}
 PyObject* raise(const Refusal& r)
 {
     PyObject* e = g_error ? PyObject_CallFunction(g_error, "is", r.code, r.message.c_str()) : nullptr;
@@ -175,10 +186,12 @@ PyObject* py_rope_append(PyObject*, PyObject* const* o, Py_ssize_t n)
             vector(o[13], "q_out", pages.scalar_type(), {tokens, heads, dim}, dev);
             out = THPVariable_Unpack(o[13]);
         }
-        check(tmac_rope_append(&c, type, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, whole(heads, "heads"),
-                               whole(tokens, "tokens"), bias, seq, pos, starts, table, whole(tables.size(0), "n_seq"),
-                               whole(tables.size(1), "width"), cosp, sinp, whole(cos.size(0), "max_pos"),
-                               whole(2 * cos.size(1), "rot_dim"), interleaved, out.data_ptr(), stream_of(dev)));
+        const int n_heads = whole(heads, "heads"), n_tokens = whole(tokens, "tokens"), n_seq = whole(tables.size(0), "n_seq");
+        const int width = whole(tables.size(1), "width"), max_pos = whole(cos.size(0), "max_pos"), rot = whole(2 * cos.size(1), "rot_dim");
+        check(unlocked([&] {
+            return tmac_rope_append(&c, type, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, n_heads, n_tokens, bias, seq, pos, starts,
+                                    table, n_seq, width, cosp, sinp, max_pos, rot, interleaved, out.data_ptr(), stream_of(dev));
+        }));
         return THPVariable_Wrap(out);
     });
 }
@@ -224,9 +237,10 @@ PyObject* py_prefix_attention(PyObject*, PyObject* const* o, Py_ssize_t n)
         }
         const int64_t os = rows(out, "out", c.head_dim, dev);
         if (need) work = at::empty({(int64_t)need}, pages.options().dtype(at::kByte));
-        check(tmac_prefix_attention(&c, q.data_ptr(), qs, heads, tokens, batch, starts, max_q, list, prefix_len, shared, table,
-                                    width, own, max_own, (float)scale, out.data_ptr(), os, need ? work.data_ptr() : nullptr, need,
-                                    stream_of(dev)));
+        check(unlocked([&] {
+            return tmac_prefix_attention(&c, q.data_ptr(), qs, heads, tokens, batch, starts, max_q, list, prefix_len, shared, table, width, own,
+                                         max_own, (float)scale, out.data_ptr(), os, need ? work.data_ptr() : nullptr, need, stream_of(dev));
+        }));
         if (o[12] != Py_None) {
             Py_INCREF(o[12]);
             return o[12];
@@ -253,8 +267,10 @@ PyObject* py_sample(PyObject*, PyObject* const* o, Py_ssize_t n)
         const auto* top_p = (const float*)vector(o[4], "top_p", at::kFloat, {batch}, dev);
         const auto* min_p = (const float*)vector(o[5], "min_p", at::kFloat, {batch}, dev);
         at::Tensor tokens = at::empty({batch}, l.options().dtype(at::kInt)), probs = at::empty({batch}, l.options().dtype(at::kFloat));
-        check(tmac_sample(l.data_ptr(), type, batch > 1 ? l.stride(0) : vocab, batch, vocab, u, temperature, top_k, top_p, min_p,
-                          tokens.data_ptr<int32_t>(), probs.data_ptr<float>(), dev.index(), stream_of(dev)));
+        check(unlocked([&] {
+            return tmac_sample(l.data_ptr(), type, batch > 1 ? l.stride(0) : vocab, batch, vocab, u, temperature, top_k, top_p, min_p,
+                               tokens.data_ptr<int32_t>(), probs.data_ptr<float>(), dev.index(), stream_of(dev));
+        }));
         return Py_BuildValue("NN", THPVariable_Wrap(tokens), THPVariable_Wrap(probs));
     });
 }
