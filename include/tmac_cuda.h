@@ -574,7 +574,8 @@ int tmac_prefix_attention_engine(const tmac_paged_cache* cache, int heads, int t
  * The next token of each row of logits from a given uniform number (stands in
  * for sample_token, sim/tmac_gguf.cpp:1974-1990, top-k 40 with rand()).
  *   x = logit * (1 / temperature);  d = max x - x;  w = floor(2^32 exp(-d))
- * with x and d in 32 bits (NaN counts as -inf) and whole-number sums, so the token
+ * with x and d in 32 bits (NaN counts as -inf, a product past their range as
+ * infinite, and infinite ones share the weight) and whole-number sums, so the token
  * does not depend on the order of the sums.  In the order of (d, index):
  *   top_k:  the first top_k tokens (<= 0: all);
  *   top_p:  the shortest first part whose weight reaches top_p times the weight of
@@ -583,7 +584,7 @@ int tmac_prefix_attention_engine(const tmac_paged_cache* cache, int heads, int t
  * A token must pass all three.  The result is the first kept index whose running
  * weight exceeds floor(u * kept weight); probs is its weight over the kept weight.
  * temperature not above 0 (or its reciprocal infinite): the lowest index of the
- * largest logit.  A row without any logit above -inf: token -1, probability 0.
+ * largest logit.  A row without any x above -inf: token -1, probability 0.
  *   logits: [batch] rows of `vocab` (up to 720000) values of `type`, row_stride in
  *           elements (0: all rows are the same one).  temperature, top_p, min_p: optional float [batch]; top_k:
  *           optional int32 [batch]; u: float [batch] in [0, 1).
