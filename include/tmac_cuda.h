@@ -480,7 +480,10 @@ int tmac_model_free(tmac_model_t m);
 /* The batched decode step: several sequences at once over a paged cache (the
  * reference decodes one sequence over one private cache,
  * forward_layer_with_cache, sim/tmac_gguf.cpp:1559-1711).  Elements are F32, F16
- * or BF16; arithmetic, softmax and sums are 32-bit, rounded once to the type.
+ * or BF16; arithmetic, softmax and sums are 32-bit, rounded once to the type.  One
+ * exception: with a 16-bit cache prefix_attention rounds each softmax weight to the
+ * cache's type, as the value that it multiplies is (products and sums stay 32-bit),
+ * which adds up to that rounding's 2^-11 (F16) or 2^-8 (BF16) of sum p |v|.
  * All pointers are device pointers on the cache's device; every call is
  * asynchronous on `stream` and keeps no state between calls, so calls on
  * several streams need no order among themselves unless they share buffers.
