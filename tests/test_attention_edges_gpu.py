@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 # (sequences, keys): each sequence reads the prefix itself; shared and joined; on tcgen05 (16 bits)
-LAYOUTS = [(2, 200), (9, 1100), (40, 1100), (100, 5000)]
+LAYOUTS = [(2, 200), (9, 1100), (40, 1100), (100, 6000)]
 HEADS = {64: (14, 2), 128: (8, 2)}
 
 

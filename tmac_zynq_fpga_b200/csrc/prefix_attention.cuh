@@ -98,12 +98,16 @@ TMAC_DEV bool is_computed(const AttnArgs& a, int token, int b)
 //   3 + 1  14/2 x 64: 48 10.7 / 12.4, 384 36.8 / 33.1;  32/8 x 128: 192 201 / 119
 constexpr int kAloneTiles16 = 6, kAloneTiles32 = 4, kOwnTiles16 = 8;
 constexpr int kAloneRows16 = 2, kAloneRows32 = 5;
-// The prefix goes to the tcgen05 kernel from so many rows on, and from so much work
-// (rows x keys x kv heads): at 64 dims 1.4 M took 13.2 us there and 11.8 in the mma
-// kernel, 3.7 M 15.4 and 15.4, 7.3 M 20.7 and 22.0, 59 M 51 and 85; at 128 dims 0.4 M 14.3
-// and 13.0, 1.7 M 21 and 29, 8.4 M 35 and 43.
+// The prefix goes to the tcgen05 kernel from so many rows on, and from so much work (rows
+// x keys x kv heads).  There and in the mma kernel, us, with 64 own keys each, query/key
+// heads, sequences x prefix:
+//   64 dims   14/2  64 x 5000 (4.5 M) 18.3 / 15.7, 32 x 16384 (7.3 M) 20.2 / 20.0, 128 x 4096 (7.3 M) 20.2 / 22.3,
+//             64 x 10000 (9.0 M) 20.2 / 21.4, 128 x 6000 (10.8 M) 21.6 / 26.1, 128 x 32768 (59 M) 41.9 / 78.8;
+//             8/8  64 x 8192 (4.2 M) 22.9 / 20.3, 64 x 16384 (8.4 M) 25.5 / 25.0, 128 x 16384 (17 M) 31.5 / 37.5
+//   128 dims  16/4  24 x 1100 (0.4 M) 14.9 / 13.5, 24 x 2500 (1.0 M) 15.9 / 15.0, 48 x 2200 (1.7 M) 16.0 / 20.6;
+//             32/8  24 x 1300 (1.0 M) 15.1 / 16.6
 constexpr int kTcRowsLeast = 48;
-constexpr int64_t kTcWork64 = 4000000, kTcWork128 = 1000000;
+constexpr int64_t kTcWork64 = 8000000, kTcWork128 = 1000000;
 constexpr int kTcRange = 4;  // tiles of its job at least: below, its start outweighs them
 constexpr int kTile = 64, kWarps = 4, kThreads = kWarps * 32;
 
