@@ -15,20 +15,21 @@
 // prefix itself, and one job holds all of a row's keys and writes its result.
 //
 // The products run on mma.sync with 32-bit sums.  16-bit elements are its operands
-// as they are; a 32-bit one is split into the nearest tf32 number and the rest
-// rounded to one, and three products of the parts make one of the elements but for
-// 2^-22 of it.  The tensor cores cut off what an addition to a sum loses, so products
-// with a rest have a sum of their own, and sums of few products are added to the
-// scores and to O by the FMA units: half the plain form's error against 64 bits (sums
-// over a whole head of 128 on the tensor cores had 1.4 times it, and took as long).
-// (Products on the FMA units too took 2 to 3 times as long.)  Tiles come through
-// cp.async, several in flight.  The prefix's jobs of 16-bit elements go to the tcgen05
-// kernel of prefix_attention_tc.cu where there are rows enough.
+// as they are; a 32-bit one is split into the nearest tf32 number and the rest, cut to
+// one, and three products of the parts make one of the elements but for 2^-21 of it.
+// The tensor cores cut off what an addition to a sum loses, so products with a rest have
+// a sum of their own, and sums of few products are added to the scores and to O by the
+// FMA units.  The error against 64 bits is the plain form's, or up to half less (rms over
+// 16384 keys of heads of 64 3.3e-8 and 3.2e-8, largest 7.6e-7 and 1.1e-6; sums over a whole
+// head of 128 on the tensor cores had 1.4 times it, and took as long).  (Products on
+// the FMA units too took 2 to 3 times as long.)  Tiles come through cp.async, several in
+// flight.  The prefix's jobs of 16-bit elements go to the tcgen05 kernel of
+// prefix_attention_tc.cu where there are rows enough.
 //
-// Bound: latency.  48 sequences over 2051 + up to 509 keys (14/2 heads of 64, f16) take
-// 12.8 us, 10 of them jobs of 3 to 4 tiles, 3 the join; in 32 bits 25 us.  64
-// sequences with only their own keys, up to 1024, run at 1300 GB/s, of heads of 128
-// at 2200.
+// Bound: latency where there is little work: 48 sequences over 2051 + up to 509 keys (14/2
+// heads of 64, f16) take 13.3 us, 10 of them jobs of 3 to 4 tiles, 3 the join; in 32 bits
+// 25.2 us.  64 sequences with only their own keys (bf16, 14/2 heads of 64 and 16/4 of 128)
+// run at 1900 and 3300 GB/s with 1024 each, at 3800 and 5100 with 8192.
 #include "prefix_attention.cuh"
 
 #include <cmath>

@@ -18,11 +18,14 @@
 // weights anew.  One thread issues the products, one warp the TMA copies of the pages
 // (a box per page, 128-byte swizzle).
 //
-// Bound: the exponentials, 128 x 64 per tile at 16 a clock, 512 clocks against 256
-// of products at 64 dims.  Two CTAs share an SM: one's waits are the other's work.  896 rows
-// a key/value head (two of 64 dims) over 32768 keys take 37 us, 410 TFLOP/s, 913 clocks a
-// tile: the rest is the latency of its 300 instructions a warp.  Three or four CTAs an
-// SM, with the weights in the scores' place, take as long.
+// Floor of the tile loop: the exponentials, 128 x 64 per tile at 16 a clock, 512 clocks
+// against 256 of products at 64 dims.  Two CTAs share an SM: one's waits are the other's
+// work.  896 rows a key/value head (two of 64 dims) over 32768 keys take 36.7 us with
+// the join, 410 TFLOP/s: 24.3 us for every 32768 keys (950 clocks a tile on an SM), and
+// 12.4 us whatever the length (2048 keys take 14.5), which are the launches, each CTA's
+// start up to its first scores, its parts' way out and the join; no measurement tells
+// these apart.  Three or four CTAs an SM, with the weights in the scores' place, take
+// as long.
 #include "prefix_attention.cuh"
 #include "tcgen05.cuh"
 

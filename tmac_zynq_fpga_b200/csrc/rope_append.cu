@@ -10,12 +10,13 @@
 // reference, and the result once to the cache's type.
 //
 // Bound: HBM, every value is read once and written once (32768 tokens of 16/4 heads of
-// 128, bf16, 91 us, 4560 GB/s; 512 tokens 3.5 us, 2 tokens 3.4, the launch).  Where
+// 128, bf16, 92.5 us, 4490 GB/s; 512 tokens 3.6 us, 2 tokens 3.3, the launch).  Where
 // the pointers, strides and head parts allow it a thread takes 8 adjoining values (16
 // bytes of a 16-bit type), or 8 pairs of halves, and keeps that place in a token for all
 // tokens of its CTA, the next one's values loaded beneath the work on this one's: 16-bit
 // values 98 -> 91 us and 21.3 -> 19.3 against places dealt out anew, 32-bit ones 34 ->
-// 36.6, 49 -> 50 and, of 512 tokens, 3.9 -> 3.5.  A CTA first looks up its tokens' pages,
+// 36.6, 49 -> 50 and, of 512 tokens, 3.9 -> 3.5 (then with fused multiply-adds, 1 to 2 %
+// faster, but rounding otherwise than the other kernel).  A CTA first looks up its tokens' pages,
 // cosines and sines into shared memory, so nothing but the values is waited for.  Other
 // layouts take one pair per thread.
 #include "serving.cuh"
